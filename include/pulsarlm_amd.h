@@ -250,6 +250,84 @@ int plm_gemm_int4_plain(const void* x, plm_dtype x_dtype, const int32_t* weight_
                         int64_t m, int64_t n, int64_t k, int64_t group_size, int64_t num_splits, void* y,
                         void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * MXFP4: microscaled 4-bit floating point. 32 consecutive K values share a scale 2^(b - 127), b one byte
+ * (255 reads as NaN), and are e2m1 codes: +-0, 0.5, 1, 1.5, 2, 3, 4, 6. A matrix [M, K] (K a multiple of
+ * 32) is codes uint8 [M, K/2], the lower K in the low half of a byte, and scales uint8 [M, K/32]. The
+ * reference has no counterpart of these entry points.
+ *
+ * plm_quantize_mxfp4: b = floor(log2(amax)) - 2 + 127, at least 0 (a block of zeros: 0); codes rounded to
+ * nearest, ties to the even code, saturating at 6. A block with an infinity or NaN gets b = 255, codes 0.
+ * x fp32, fp16 or bf16, 16-byte aligned. plm_dequantize_mxfp4 is its inverse, exact in bf16 and fp32 and
+ * rounded once to fp16 (largest values to infinity).
+ */
+int plm_quantize_mxfp4(const void* x, plm_dtype x_dtype, int64_t m, int64_t k, uint8_t* codes, uint8_t* scale,
+                       void* stream);
+int plm_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scale, int64_t m, int64_t k, void* out,
+                         plm_dtype out_dtype, void* stream);
+
+/* Repack an MXFP4 weight [N, K] for the products below: N and K at most 2^19, codes 16-byte aligned.
+ * The layout is opaque: 16 x 128 tiles of 1 KiB and their scales, padded with zeros. -1: invalid sizes. */
+int64_t plm_mxfp4_weight_bytes(int64_t n, int64_t k);
+int64_t plm_mxfp4_scale_bytes(int64_t n, int64_t k);
+int plm_repack_mxfp4(const uint8_t* codes, const uint8_t* scale, int64_t n, int64_t k, void* weight_out,
+                     void* scale_out, void* stream);
+
+/*
+ * y [M, N] = x [M, K] @ W^T in x_dtype (PLM_BF16 or PLM_FP16), W the repacked MXFP4 weight in x_dtype (exact
+ * in bf16, rounded once to fp16), fp32 sums. M N and M K at most 2^36. M == 0 or N == 0 returns PLM_OK
+ * without touching y; K == 0 sets y to zero. No workspace.
+ */
+int plm_gemm_mxfp4(const void* x, plm_dtype x_dtype, const void* weight, const void* scale,
+                   int64_t m, int64_t n, int64_t k, void* y, void* stream);
+
+/*
+ * The same with x quantized by the rule of plm_quantize_mxfp4 (W4A4): both operands' codes and scales go to
+ * the scaled matrix instruction. One token's x is quantized inside the product's kernel, longer ones' in a
+ * launch of its own into the workspace (256-byte aligned; its contents need not be set and mean nothing
+ * after the call).
+ */
+int64_t plm_gemm_mxfp4_w4a4_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int plm_gemm_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* weight, const void* scale,
+                        int64_t m, int64_t n, int64_t k, void* y, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* The input's gradient of plm_gemm_mxfp4: dx [M, K] = dy [M, N] @ W in `dtype`, dx 8-byte aligned.
+ * (The weights are codes and have none.) N == 0 sets dx to zero. Workspace as above. */
+int64_t plm_gemm_mxfp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int plm_gemm_mxfp4_grad(const void* dy, plm_dtype dtype, const void* weight, const void* scale,
+                        int64_t m, int64_t n, int64_t k, void* dx, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/*
+ * Gated feed-forward block in one kernel: h [M, N] = silu(g) u with g = x @ Wgate^T, u = x @ Wup^T in fp32,
+ * silu(g) = g / (1 + exp(-g)), rounded once, where plm_gemm and plm_silu_mul round g, u and silu(g), too.
+ * N is the intermediate size; gate_up, where it is not NULL, receives [g | u] (fp32 [M, 2 N]) for the
+ * gradient. Otherwise as plm_gemm_mxfp4.
+ */
+int plm_gated_mxfp4(const void* x, plm_dtype x_dtype, const void* gate_weight, const void* gate_scale,
+                    const void* up_weight, const void* up_scale, int64_t m, int64_t n, int64_t k,
+                    void* h, float* gate_up, void* stream);
+
+/* Its input's gradient from dh [M, N] and the kept gate_up: dx [M, K] = (dh u s (1 + g (1 - s))) @ Wgate +
+ * (dh g s) @ Wup, s = 1 / (1 + exp(-g)); the two factors are rounded to `dtype` for the products. */
+int64_t plm_gated_mxfp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int plm_gated_mxfp4_grad(const void* dh, const float* gate_up, plm_dtype dtype,
+                         const void* gate_weight, const void* gate_scale, const void* up_weight, const void* up_scale,
+                         int64_t m, int64_t n, int64_t k, void* dx, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/*
+ * The whole feed-forward block with 4-bit activations: y [M, K] = Q(h) @ Wdown^T, h = silu(g) u of Q(x) as in
+ * plm_gated_mxfp4, Q the rounding of plm_quantize_mxfp4; h is quantized from its fp32 values in the gated
+ * kernel and never stored in 16 bits. Wgate and Wup are [N, K], Wdown [K, N], N a multiple of 32.
+ */
+int64_t plm_mlp_mxfp4_w4a4_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int plm_mlp_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* gate_weight, const void* gate_scale,
+                       const void* up_weight, const void* up_scale, const void* down_weight, const void* down_scale,
+                       int64_t m, int64_t n, int64_t k, void* y, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -42,6 +42,21 @@ SIGNATURES = {
     "plm_gemm_int4_plain": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _SZ, _P]),
     "plm_route_top_k": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _P, _P, _P, _P]),
     "plm_silu_mul": (_INT, [_P, _INT, _I64, _I64, _P, _P]),
+    "plm_mxfp4_weight_bytes": (_I64, [_I64, _I64]),
+    "plm_mxfp4_scale_bytes": (_I64, [_I64, _I64]),
+    "plm_quantize_mxfp4": (_INT, [_P, _INT, _I64, _I64, _P, _P, _P]),
+    "plm_dequantize_mxfp4": (_INT, [_P, _P, _I64, _I64, _P, _INT, _P]),
+    "plm_repack_mxfp4": (_INT, [_P, _P, _I64, _I64, _P, _P, _P]),
+    "plm_gemm_mxfp4": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _P, _P]),
+    "plm_gemm_mxfp4_w4a4_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "plm_gemm_mxfp4_w4a4": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
+    "plm_gemm_mxfp4_grad_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "plm_gemm_mxfp4_grad": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
+    "plm_gated_mxfp4": (_INT, [_P, _INT, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P]),
+    "plm_gated_mxfp4_grad_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "plm_gated_mxfp4_grad": (_INT, [_P, _P, _INT, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
+    "plm_mlp_mxfp4_w4a4_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "plm_mlp_mxfp4_w4a4": (_INT, [_P, _INT, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
     "plm_moe": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _INT, _I64, _P, _P, _P, _SZ,
                        _P]),
 }
@@ -83,6 +98,12 @@ def gemm_workspace_bytes(fmt: int, m: int, n: int, k: int) -> int:
 @functools.lru_cache(maxsize=1024)
 def gemm_w8a8_workspace_bytes(m: int, n: int, k: int) -> int:
     return load().plm_gemm_w8a8_workspace_bytes(m, n, k)
+
+
+@functools.lru_cache(maxsize=1024)
+def mxfp4_bytes(name: str, *sizes: int) -> int:
+    """plm_mxfp4_weight_bytes and its like, by the name after plm_."""
+    return getattr(load(), "plm_" + name)(*sizes)
 
 
 def reload_tuning() -> None:

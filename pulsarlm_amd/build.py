@@ -23,7 +23,8 @@ BUILD = PKG / "_build"
 LIB = PKG / "libpulsarlm_amd.so"
 
 SOURCES = ["repack.hip", "gemm_decode.hip", "gemm_mfma.hip", "gemm_mfma_int4.hip", "gemm_mfma_fp8.hip", "gemm_mfma_a8.hip",
-           "gemm_mfma_grouped.hip", "gemm_rows_int4.hip", "gemm_rows_fp8.hip", "quant.hip", "moe.hip", "routing.hip", "gemm_plain.hip", "capi.hip"]
+           "gemm_mfma_grouped.hip", "gemm_rows_int4.hip", "gemm_rows_fp8.hip", "quant.hip", "moe.hip", "routing.hip", "gemm_plain.hip", "capi.hip",
+           "mxfp4_quant.hip", "mxfp4_rows.hip", "mxfp4_tiles_w4a16.hip", "mxfp4_tiles_w4a4.hip", "mxfp4_grad.hip", "mxfp4_api.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
@@ -42,9 +43,10 @@ FLAGS = [
 
 # Per-source flags. The MFMA kernel keeps its accumulators in VGPRs (the VGPR form of
 # v_mfma): with the default AGPR form the register allocator splits the accumulator set
-# between the two files and copies it back and forth every K step.
+# between the two files and copies it back and forth every K step. (mxfp4_tiles_w4a4's 256 sums a
+# lane fill the AGPRs exactly: it keeps the default.)
 SOURCE_FLAGS = {src: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-                for src in SOURCES if src.startswith(("gemm_mfma", "gemm_rows"))}
+                for src in SOURCES if src.startswith(("gemm_mfma", "gemm_rows", "mxfp4_tiles_w4a16", "mxfp4_grad"))}
 
 
 EXTRA_DEFINES: list[str] = []

@@ -1,0 +1,358 @@
+// Input gradients through MXFP4 weights: dx[M, K] = dy[M, N] @ W, and the gated block's, whose dy is
+// [d gate | d up] against the two weights one after the other (the sum runs on from one into the other).
+// The weights themselves are codes and have no gradient.
+//
+// The sum runs over N here, along which the tile layout is not contiguous and every row has its own block
+// scales, so the scaled matrix instruction cannot take the codes. A workgroup decodes its 64 x 256 slice of
+// W into LDS in 16 bits instead (exact in bf16), 32 codes to a lane under one scale, and the fragments are
+// read back with the transposing LDS read: 16 lanes fetch four rows of 16 columns and receive one column each.
+// * Tile (2 MT 16) x 256 columns, steps of 64 along N. dy and the codes of the step after next are requested
+//   to registers and go, the codes decoded, into the other of two LDS slots a step ahead. (dy by loads to
+//   LDS would be waited for in full before every transposing read: the compiler cannot tell them apart.)
+// * One barrier a step, before the matrix instructions of its second half, as in the forward kernel
+//   (mxfp4_tiles.hip): their operands are in registers, and the next step's first half is read meanwhile.
+// * Few tiles: the steps are split over workgroups, whose fp32 sums a second kernel adds in split order.
+#include "mxfp4.hpp"
+
+namespace plm {
+
+namespace {
+
+constexpr int kGradStep = 64;    // N of a step
+constexpr int kGradCols = 256;   // columns of a workgroup
+
+struct grad_args {
+    const uint16_t* dy;  // [M][pitch], zero past N up to a whole step
+    mx_matrix w0, w1;
+    uint16_t* dx;
+    float* partial;  // [splits][M][K]
+    int64_t pitch;
+    int m, k, ktiles, kgroups, strips;
+    int side_steps, steps, split_steps, splits;
+    int m_blocks, n_blocks;
+};
+
+typedef __attribute__((ext_vector_type(4))) short tr_t;
+
+template <bool BF16, int MT>
+__global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
+    constexpr int WN = 4, NS = 4, NW = 8, BM = 2 * MT * 16;
+    constexpr int XC = BM / 8, XPW = XC / NW;  // 1 KiB chunks of dy: 8 rows of 128 bytes
+    constexpr int XS = BM * 128, WS = kGradStep * kGradCols * 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * XS + 2 * WS];
+    uint8_t* wlds = lds + 2 * XS;
+
+    const int lane = threadIdx.x & 63;
+    const int wave = uniform(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const int col16 = lane & 15, kq = lane >> 4;
+
+    // Workgroups go round the 8 XCDs by id; each takes a run of the tiles, row block fastest (they share W).
+    const int tiles = a.m_blocks * a.n_blocks, xcd = blockIdx.x & 7;
+    const int lin = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (blockIdx.x >> 3);
+    const int row0 = lin % a.m_blocks * BM, nb = lin / a.m_blocks;
+    const int rows = min(BM, a.m - row0);
+    const int split = blockIdx.y;
+    const int lo = split * a.split_steps, hi = min(lo + a.split_steps, a.steps);
+
+    const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.dy + row0 * a.pitch, static_cast<uint32_t>(rows * a.pitch * 2));
+    struct step_data {
+        u32x4_t x[XPW], c;
+        uint32_t s;
+    };
+    // An opaque copy of the lane id: the offsets made from it are worked out where they are used, and take no
+    // registers from the sums.
+    auto own_lane = [&] {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        return l;
+    };
+    auto load_x = [&](step_data& b, int s) {
+        const int lane = own_lane();
+        const int past = s < hi ? 0 : kOOB, off = s < hi ? s * 128 : 0;
+#pragma unroll
+        for (int i = 0; i < XPW; ++i) {
+            const int r = 8 * (wave * XPW + i) + (lane >> 3);  // rows past the last are past the buffer's end
+            b.x[i] = buffer_load16(xr, (static_cast<int>(r * a.pitch * 2) + (lane & 7) * 16) | past, off);
+        }
+    };
+    auto write_x = [&](const step_data& b, int slot) {
+        const int lane = own_lane();
+#pragma unroll
+        for (int i = 0; i < XPW; ++i) {
+            const int r = 8 * (wave * XPW + i) + (lane >> 3);
+            *reinterpret_cast<u32x4_t*>(lds + slot * XS + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = b.x[i];  // 16-byte columns swizzled by row
+        }
+    };
+
+    // Wavefront w decodes one tile of a step: strip w / 2, K tile w % 2 (the second may lie past K).
+    const int kt = 2 * nb + (wave & 1);
+    auto load_w = [&](step_data& b, int s) {
+        const int lane = own_lane();
+        const int side = s >= a.side_steps ? 1 : 0, strip = 4 * (s - side * a.side_steps) + (wave >> 1);
+        const uint8_t* base = side ? a.w1.codes : a.w0.codes;
+        const uint32_t* sbase = side ? a.w1.scale : a.w0.scale;
+        const bool in = s < hi && strip < a.strips && kt < a.ktiles;
+        const int64_t at = in ? strip : 0, t = in ? kt : 0;
+        const int past = in ? 0 : kOOB;
+        b.c = buffer_load16(make_rsrc(base + (at * a.ktiles + t) * kSubTileBytes, kSubTileBytes), (lane * 16) | past);
+        b.s = buffer_load_u32(make_rsrc(sbase + (at * a.kgroups + (t >> 2)) * 64, 256u), (lane * 4) | past, 0);
+    };
+    // LDS row n (512 bytes): its 32-byte pieces are XOR-swizzled by f(n) = n % 4 + 4 ((n / 4 + n / 8) % 2),
+    // which sets apart both the eight rows that one write covers and the rows of one transposing read.
+    auto write_w = [&](const step_data& b, int slot) {
+        const int lane = own_lane(), col16 = lane & 15, kq = lane >> 4;
+        const int wrow = (wave >> 1) * 16 + col16, wf = (col16 & 3) | ((((col16 >> 2) ^ (col16 >> 3)) & 1) << 2);
+        uint8_t* base = wlds + slot * WS + wrow * 512;
+        const float s = mx_scale(b.s >> (8 * (kt & 3)) & 0xffu);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<u32x4_t*>(base + ((((wave & 1) * 8 + 2 * kq + (q >> 1)) ^ wf) << 5) + (q & 1) * 16) = mx_decode<BF16>(b.c[q], s);
+    };
+
+    u32x4_t x[MT], w[2][NS];  // fragments; x's are read again for the next half right after their use
+    struct lane_offsets {
+        int x, w;
+    };
+    auto fragment_offsets = [&] {
+        const int lane = own_lane(), col16 = lane & 15, kq = lane >> 4, f = (col16 >> 2) | ((kq & 1) << 2);
+        return lane_offsets{wm * MT * 2048 + col16 * 128 + ((kq ^ (col16 & 7)) << 4),
+                            (8 * kq + (col16 >> 2)) * 512 + (((wn * NS) ^ f) << 5) + (col16 & 3) * 8};
+    };
+    auto read_x = [&](const lane_offsets& o, int i, int slot, int t) {
+        x[i] = *reinterpret_cast<const u32x4_t*>(lds + slot * XS + (o.x ^ (t << 6)) + i * 2048);
+    };
+    auto read_w = [&](const lane_offsets& o, u32x4_t (&w)[NS], int j, int slot, int t) {
+        const uint8_t* p = wlds + slot * WS + t * 32 * 512;
+        const tr_t lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr_t*)(p + (o.w ^ (j << 5))));
+        const tr_t hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr_t*)(p + 2048 + (o.w ^ ((j ^ 4) << 5))));
+        const u32x2_t l = __builtin_bit_cast(u32x2_t, lo4), h = __builtin_bit_cast(u32x2_t, hi4);
+        w[j] = u32x4_t{l[0], l[1], h[0], h[1]};
+    };
+
+    f32x4_t acc[MT][NS];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    step_data b;
+    load_x(b, lo);
+    load_w(b, lo);
+    write_x(b, 0);
+    write_w(b, 0);
+    load_x(b, lo + 1);
+    load_w(b, lo + 1);
+    __syncthreads();
+    lane_offsets o = fragment_offsets();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) read_x(o, i, 0, 0);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) read_w(o, w[0], j, 0, 0);
+    int slot = 0;
+    for (int s = lo; s < hi; ++s) {
+        write_x(b, slot ^ 1);
+        write_w(b, slot ^ 1);
+        __builtin_amdgcn_sched_barrier(0);  // the next data go into the same registers
+        load_x(b, s + 2);
+        load_w(b, s + 2);
+        o = fragment_offsets();
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+#pragma unroll
+            for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(o, w[1], j, slot, 1);
+#pragma unroll
+            for (int j = 0; j < NS; ++j) acc[i][j] = mfma16x16x32<BF16>(w[0][j], x[i], acc[i][j]);
+            read_x(o, i, slot, 1);
+            __builtin_amdgcn_sched_barrier(0);  // the reads stay among the matrix instructions, half a step ahead
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        slot ^= 1;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+#pragma unroll
+            for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(o, w[0], j, slot, 0);
+#pragma unroll
+            for (int j = 0; j < NS; ++j) acc[i][j] = mfma16x16x32<BF16>(w[1][j], x[i], acc[i][j]);
+            read_x(o, i, slot, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int r = (wm * MT + i) * 16 + col16;
+        if (r >= rows) continue;
+        const int64_t row = row0 + r;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const int col = nb * kGradCols + (wn * NS + j) * 16 + 4 * kq;  // K is a multiple of 32
+            if (col >= a.k) continue;
+            const f32x4_t v = acc[i][j];
+            if (a.splits > 1) *reinterpret_cast<f32x4_t*>(a.partial + (static_cast<int64_t>(split) * a.m + row) * a.k + col) = v;
+            else *reinterpret_cast<uint2*>(a.dx + row * a.k + col) = make_uint2(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]));
+        }
+    }
+}
+
+// Sums over the splits, four values a thread.
+template <bool BF16>
+__global__ void __launch_bounds__(256) mx_grad_combine_kernel(const f32x4_t* __restrict__ partial, int64_t quads, int splits,
+                                                              uint2* __restrict__ dx) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= quads) return;
+    f32x4_t v = partial[i];
+    for (int s = 1; s < splits; ++s) v = v + partial[s * quads + i];
+    dx[i] = make_uint2(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]));
+}
+
+// The gated block's [d gate | d up], each padded with zeros to a whole step, rounded to the matrix
+// instruction's 16 bits: with s = sigmoid(g), d gate = dh u s (1 + g (1 - s)), d up = dh g s.
+// !GATED: a copy of dy padded so. Eight values a thread; WIDE: rows of whole 16-byte pieces.
+template <bool BF16, bool GATED, bool WIDE>
+__global__ void __launch_bounds__(256) mx_grad_rows_kernel(const uint16_t* __restrict__ dy, const float* __restrict__ gate_up,
+                                                           int64_t m, int n, int padded, uint16_t* __restrict__ out) {
+    const int per_row = padded / 8;
+    const int64_t total = m * per_row, step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; c < total; c += step) {
+        const int64_t row = c / per_row;
+        const int col = static_cast<int>(c % per_row) * 8;
+        auto load8 = [&](const uint16_t* p, uint32_t (&v)[8]) {
+            if (WIDE && col < n) {
+                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p + col);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[2 * i] = w[i] & 0xffffu, v[2 * i + 1] = w[i] >> 16;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = col + i < n ? p[col + i] : 0u;
+            }
+        };
+        auto store8 = [&](uint16_t* p, const uint32_t (&v)[8]) {
+            *reinterpret_cast<u32x4_t*>(p) = u32x4_t{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+        };
+        uint32_t d[8];
+        load8(dy + row * n, d);
+        if constexpr (!GATED) {
+            store8(out + row * padded + col, d);
+        } else {
+            auto load8f = [&](const float* p, float (&v)[8]) {
+                if (WIDE && col < n) {
+                    const f32x4_t a = reinterpret_cast<const f32x4_t*>(p + col)[0], b = reinterpret_cast<const f32x4_t*>(p + col)[1];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = col + i < n ? p[col + i] : 0.f;
+                }
+            };
+            float g[8], u[8];
+            uint32_t dg[8], du[8];
+            load8f(gate_up + row * 2 * n, g);
+            load8f(gate_up + row * 2 * n + n, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float dh = from_bits16<BF16>(d[i]), gf = g[i], uf = u[i];
+                const float s = mx_sigmoid(gf);
+                dg[i] = to_bits16<BF16>(dh * uf * s * (1.f + gf * (1.f - s)));
+                du[i] = to_bits16<BF16>(dh * gf * s);
+            }
+            store8(out + row * 2 * padded + col, dg);
+            store8(out + row * 2 * padded + padded + col, du);
+        }
+    }
+}
+
+struct grad_plan {
+    int mt;
+    int64_t m_blocks, n_blocks, steps, splits, split_steps;
+};
+grad_plan make_grad_plan(int64_t m, int64_t k, int64_t steps) {
+    grad_plan p{};
+    p.mt = m <= 64 ? 2 : 8;
+    p.m_blocks = ceil_div(m, 32 * p.mt);
+    p.n_blocks = ceil_div(k, kGradCols);
+    p.steps = steps;
+    const int64_t want = std::max<int64_t>(1, cu_count() / (p.m_blocks * p.n_blocks));
+    p.splits = std::max<int64_t>(1, std::min<int64_t>(want, steps / 8));
+    p.split_steps = ceil_div(steps, p.splits);
+    p.splits = ceil_div(steps, p.split_steps);
+    return p;
+}
+
+int64_t padded_n(int64_t n) { return round_up(n, kGradStep); }
+bool copies_dy(const void* dy, int64_t n) { return n % kGradStep != 0 || !aligned(dy, 16); }
+
+// Workspace: [rows in 16 bits][fp32 partial sums].
+int64_t rows_bytes(int64_t m, int64_t n, int sides) { return round_up(m * sides * padded_n(n) * 2, 256); }
+int64_t grad_bytes(int64_t m, int64_t n, int64_t k, int sides) {
+    const grad_plan p = make_grad_plan(m, k, sides * padded_n(n) / kGradStep);
+    return rows_bytes(m, n, sides) + (p.splits > 1 ? p.splits * m * k * 4 : 0);
+}
+
+template <bool BF16, bool GATED>
+void launch_rows(const void* dy, const void* gate_up, int64_t m, int64_t n, uint16_t* out, hipStream_t s) {
+    const int64_t padded = padded_n(n);
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(m * padded / 8, 256), int64_t{64} * cu_count()));
+    const auto* d = static_cast<const uint16_t*>(dy);
+    const auto* g = static_cast<const float*>(gate_up);
+    if (n % 8 == 0 && aligned(dy, 16) && aligned(gate_up, 16))
+        mx_grad_rows_kernel<BF16, GATED, true><<<grid, 256, 0, s>>>(d, g, m, static_cast<int>(n), static_cast<int>(padded), out);
+    else mx_grad_rows_kernel<BF16, GATED, false><<<grid, 256, 0, s>>>(d, g, m, static_cast<int>(n), static_cast<int>(padded), out);
+}
+
+template <bool BF16>
+int run(const char* op, bool gated, const void* dy, const void* gate_up, const mx_matrix& w0, const mx_matrix& w1, int64_t m, int64_t n,
+        int64_t k, void* dx, void* workspace, hipStream_t s) {
+    const int sides = gated ? 2 : 1;
+    const mx_dims d = make_mx_dims(n, k);
+    grad_args a{};
+    auto* rows = static_cast<uint16_t*>(workspace);
+    a.dy = static_cast<const uint16_t*>(dy);
+    a.pitch = n;
+    if (gated || copies_dy(dy, n)) {
+        if (gated) launch_rows<BF16, true>(dy, gate_up, m, n, rows, s);
+        else launch_rows<BF16, false>(dy, nullptr, m, n, rows, s);
+        PLM_HIP_LAUNCH_CHECK(op);
+        a.dy = rows;
+        a.pitch = sides * padded_n(n);
+    }
+    a.side_steps = static_cast<int>(padded_n(n) / kGradStep);
+    const grad_plan p = make_grad_plan(m, k, int64_t{sides} * a.side_steps);
+    a.w0 = w0;
+    a.w1 = w1;
+    a.dx = static_cast<uint16_t*>(dx);
+    a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + rows_bytes(m, n, sides));
+    a.m = static_cast<int>(m);
+    a.k = static_cast<int>(k);
+    a.ktiles = static_cast<int>(d.ktiles);
+    a.kgroups = static_cast<int>(d.kgroups);
+    a.strips = static_cast<int>(d.strips);
+    a.steps = static_cast<int>(p.steps);
+    a.splits = static_cast<int>(p.splits);
+    a.split_steps = static_cast<int>(p.split_steps);
+    a.m_blocks = static_cast<int>(p.m_blocks);
+    a.n_blocks = static_cast<int>(p.n_blocks);
+    const dim3 grid(static_cast<unsigned>(p.m_blocks * p.n_blocks), static_cast<unsigned>(p.splits));
+    if (p.mt == 2) mx_grad_kernel<BF16, 2><<<grid, 512, 0, s>>>(a);
+    else mx_grad_kernel<BF16, 8><<<grid, 512, 0, s>>>(a);
+    PLM_HIP_LAUNCH_CHECK(op);
+    if (p.splits > 1) {
+        const int64_t quads = m * k / 4;
+        mx_grad_combine_kernel<BF16><<<static_cast<unsigned>(ceil_div(quads, 256)), 256, 0, s>>>(
+            reinterpret_cast<const f32x4_t*>(a.partial), quads, a.splits, static_cast<uint2*>(dx));
+        PLM_HIP_LAUNCH_CHECK(op);
+    }
+    return PLM_OK;
+}
+
+}  // namespace
+
+int64_t mx_grad_bytes(int64_t m, int64_t n, int64_t k, bool gated) { return grad_bytes(m, n, k, gated ? 2 : 1); }
+
+int launch_mx_grad(const char* op, bool gated, bool bf16, const void* dy, const void* gate_up, const mx_matrix& w0, const mx_matrix& w1,
+                   int64_t m, int64_t n, int64_t k, void* dx, void* workspace, hipStream_t s) {
+    return bf16 ? run<true>(op, gated, dy, gate_up, w0, w1, m, n, k, dx, workspace, s)
+                : run<false>(op, gated, dy, gate_up, w0, w1, m, n, k, dx, workspace, s);
+}
+
+}  // namespace plm

@@ -1,0 +1,230 @@
+// MXFP4 quantizer, its inverse and the weights' repack. All stream: each value is read and written once,
+// so HBM bounds them (and a launch's latency, for one token).
+#include "mxfp4.hpp"
+
+namespace plm {
+
+namespace {
+
+// Eight consecutive values of T (uint16_t: bf16 or fp16 bits) as floats.
+template <typename T, bool BF16> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[2 * j] = from_bits16<BF16>(w[j] & 0xffffu);
+            v[2 * j + 1] = from_bits16<BF16>(w[j] >> 16);
+        }
+    }
+}
+
+template <int CTRL> __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    const int o = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, false);
+    return max(v, static_cast<uint32_t>(o));
+}
+
+// Four neighbouring lanes share a block, eight values each: 16-byte loads that are contiguous over the
+// wavefront, and the block's largest magnitude by two quad permutes.
+__device__ __forceinline__ uint32_t encode_in_quad(const float (&v)[8], uint32_t& b) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, mx_magnitude(v[i]));
+    top = quad_max<0xB1>(top);  // quad_perm [1,0,3,2]
+    top = quad_max<0x4E>(top);  // quad_perm [2,3,0,1]
+    b = mx_scale_byte(top);
+    return mx_encode8(v, b);
+}
+
+constexpr int kThreads = 256;
+
+template <typename T, bool BF16>
+__global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T* __restrict__ x, int64_t chunks, uint32_t* __restrict__ codes,
+                                                               uint8_t* __restrict__ scale) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; c < chunks; c += step) {  // whole quads
+        float v[8];
+        load8<T, BF16>(x + c * 8, v);
+        uint32_t b;
+        codes[c] = encode_in_quad(v, b);
+        if ((threadIdx.x & 3) == 0) scale[c >> 2] = static_cast<uint8_t>(b);
+    }
+}
+
+// One workgroup: 16 rows by a group of 4 K tiles, in the tile layout. A quad of lanes takes a block; the
+// four scale bytes of a lane's dword are the blocks that the quad meets in turn.
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads) mx_quantize_tiles_kernel(const uint16_t* __restrict__ x, int64_t m, int k, int ktiles,
+                                                                     int kgroups, uint8_t* __restrict__ codes,
+                                                                     uint32_t* __restrict__ scale) {
+    const int64_t strip = blockIdx.x / kgroups;
+    const int q = blockIdx.x % kgroups;
+    const int quad = threadIdx.x >> 2, part = threadIdx.x & 3;
+    const int64_t row = strip * 16 + (quad & 15);
+    const int block = quad >> 4;
+    float v[4][8];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int col = (4 * q + t) * kTileK + block * kMxBlock + part * 8;
+        if (row < m && col < k) load8<uint16_t, BF16>(x + row * k + col, v[t]);
+        else
+            for (int i = 0; i < 8; ++i) v[t][i] = 0.f;
+    }
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        uint32_t b;
+        const uint32_t c = encode_in_quad(v[t], b);
+        bytes |= b << (8 * t);
+        const int kt = 4 * q + t;
+        if (kt < ktiles) *reinterpret_cast<uint32_t*>(codes + (strip * ktiles + kt) * kSubTileBytes + quad * 16 + part * 4) = c;
+    }
+    if (part == 0) scale[(strip * kgroups + q) * 64 + quad] = bytes;
+}
+
+// OUT: 0 bf16, 1 fp16, 2 fp32. Eight codes a lane.
+template <int OUT>
+__global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scale,
+                                                                 int64_t chunks, void* __restrict__ out) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; c < chunks; c += step) {
+        const uint32_t w = codes[c];
+        const float s = mx_scale(scale[c >> 2]);
+        if constexpr (OUT == 2) {
+            typedef __attribute__((ext_vector_type(2))) float f2;
+            const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+            const f2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+            float4* o = reinterpret_cast<float4*>(out) + 2 * c;
+            o[0] = make_float4(a[0], a[1], b[0], b[1]);
+            o[1] = make_float4(d[0], d[1], e[0], e[1]);
+        } else {
+            reinterpret_cast<u32x4_t*>(out)[c] = mx_decode<OUT == 0>(w, s);
+        }
+    }
+}
+
+// One thread: 16 bytes of the tile layout, a row's block as it lies in the source.
+__global__ void __launch_bounds__(kThreads) mx_repack_codes_kernel(const uint8_t* __restrict__ codes, int64_t n, int64_t k, int64_t ktiles,
+                                                                   int64_t total, u32x4_t* __restrict__ out) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (i >= total) return;
+    const int lane = static_cast<int>(i & 63);
+    const int64_t tile = i >> 6, row = tile / ktiles * 16 + (lane & 15), block = tile % ktiles * 4 + (lane >> 4);
+    u32x4_t v = {0, 0, 0, 0};
+    if (row < n && block * kMxBlock < k) v = *reinterpret_cast<const u32x4_t*>(codes + row * (k / 2) + block * 16);
+    out[i] = v;
+}
+
+__global__ void __launch_bounds__(kThreads) mx_repack_scale_kernel(const uint8_t* __restrict__ scale, int64_t n, int64_t blocks,
+                                                                   int64_t kgroups, int64_t total, uint32_t* __restrict__ out) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (i >= total) return;
+    const int lane = static_cast<int>(i & 63);
+    const int64_t group = i >> 6, row = group / kgroups * 16 + (lane & 15), block0 = group % kgroups * 16 + (lane >> 4);
+    uint32_t v = 0;
+    for (int t = 0; t < 4; ++t) {
+        const int64_t block = block0 + 4 * t;
+        if (row < n && block < blocks) v |= static_cast<uint32_t>(scale[row * blocks + block]) << (8 * t);
+    }
+    out[i] = v;
+}
+
+unsigned stream_blocks(int64_t threads) {
+    return static_cast<unsigned>(std::min<int64_t>(ceil_div(threads, kThreads), int64_t{64} * cu_count()));
+}
+
+int check_blocks(const char* op, int64_t m, int64_t k) {
+    PLM_CHECK_ARG(m >= 0 && k >= 0, op, "sizes must be non-negative");
+    PLM_CHECK_ARG(k % kMxBlock == 0, op, "K must be a multiple of 32");
+    PLM_CHECK_ARG(k <= (int64_t{1} << 30) && m <= (int64_t{1} << 30), op, "sizes must be below 2^30");
+    return PLM_OK;
+}
+
+}  // namespace
+
+void launch_mx_quantize_tiles(const void* x, bool bf16, int64_t m, int64_t k, uint8_t* codes, uint32_t* scale, hipStream_t s) {
+    const mx_dims d = make_mx_dims(m, k);
+    const unsigned grid = static_cast<unsigned>(d.strips * d.kgroups);
+    const auto* xp = static_cast<const uint16_t*>(x);
+    const int kt = static_cast<int>(d.ktiles), kg = static_cast<int>(d.kgroups);
+    if (bf16) mx_quantize_tiles_kernel<true><<<grid, kThreads, 0, s>>>(xp, m, static_cast<int>(k), kt, kg, codes, scale);
+    else mx_quantize_tiles_kernel<false><<<grid, kThreads, 0, s>>>(xp, m, static_cast<int>(k), kt, kg, codes, scale);
+}
+
+}  // namespace plm
+
+using namespace plm;
+
+extern "C" {
+
+int64_t plm_mxfp4_weight_bytes(int64_t n, int64_t k) { return n < 0 || k < 0 ? -1 : make_mx_dims(n, k).tile_bytes(); }
+int64_t plm_mxfp4_scale_bytes(int64_t n, int64_t k) { return n < 0 || k < 0 ? -1 : make_mx_dims(n, k).scale_bytes(); }
+
+int plm_quantize_mxfp4(const void* x, plm_dtype x_dtype, int64_t m, int64_t k, uint8_t* codes, uint8_t* scale, void* stream) {
+    const char* op = "quantize_mxfp4";
+    clear_error();
+    PLM_CHECK_ARG(x_dtype == PLM_BF16 || x_dtype == PLM_FP16 || x_dtype == PLM_FP32, op, "x must be fp32, fp16 or bf16");
+    if (int rc = check_blocks(op, m, k)) return rc;
+    if (m == 0 || k == 0) return PLM_OK;
+    PLM_CHECK_ARG(x && codes && scale, op, "null pointer");
+    PLM_CHECK_ARG(aligned(x, 16), op, "x must be 16-byte aligned");
+    PLM_CHECK_ARG(aligned(codes, 4), op, "codes must be 4-byte aligned");
+    const int64_t chunks = m * (k / 8);
+    const unsigned grid = stream_blocks(chunks);
+    hipStream_t s = as_stream(stream);
+    auto* c = reinterpret_cast<uint32_t*>(codes);
+    if (x_dtype == PLM_BF16)
+        mx_quantize_kernel<uint16_t, true><<<grid, kThreads, 0, s>>>(static_cast<const uint16_t*>(x), chunks, c, scale);
+    else if (x_dtype == PLM_FP16)
+        mx_quantize_kernel<uint16_t, false><<<grid, kThreads, 0, s>>>(static_cast<const uint16_t*>(x), chunks, c, scale);
+    else mx_quantize_kernel<float, false><<<grid, kThreads, 0, s>>>(static_cast<const float*>(x), chunks, c, scale);
+    PLM_HIP_LAUNCH_CHECK(op);
+    return PLM_OK;
+}
+
+int plm_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scale, int64_t m, int64_t k, void* out, plm_dtype out_dtype,
+                         void* stream) {
+    const char* op = "dequantize_mxfp4";
+    clear_error();
+    PLM_CHECK_ARG(out_dtype == PLM_BF16 || out_dtype == PLM_FP16 || out_dtype == PLM_FP32, op, "out dtype must be fp32, fp16 or bf16");
+    if (int rc = check_blocks(op, m, k)) return rc;
+    if (m == 0 || k == 0) return PLM_OK;
+    PLM_CHECK_ARG(codes && scale && out, op, "null pointer");
+    PLM_CHECK_ARG(aligned(codes, 4), op, "codes must be 4-byte aligned");
+    PLM_CHECK_ARG(aligned(out, 16), op, "out must be 16-byte aligned");
+    const int64_t chunks = m * (k / 8);
+    const unsigned grid = stream_blocks(chunks);
+    hipStream_t s = as_stream(stream);
+    const auto* c = reinterpret_cast<const uint32_t*>(codes);
+    if (out_dtype == PLM_BF16) mx_dequantize_kernel<0><<<grid, kThreads, 0, s>>>(c, scale, chunks, out);
+    else if (out_dtype == PLM_FP16) mx_dequantize_kernel<1><<<grid, kThreads, 0, s>>>(c, scale, chunks, out);
+    else mx_dequantize_kernel<2><<<grid, kThreads, 0, s>>>(c, scale, chunks, out);
+    PLM_HIP_LAUNCH_CHECK(op);
+    return PLM_OK;
+}
+
+int plm_repack_mxfp4(const uint8_t* codes, const uint8_t* scale, int64_t n, int64_t k, void* weight_out, void* scale_out,
+                     void* stream) {
+    const char* op = "repack_mxfp4";
+    clear_error();
+    PLM_CHECK_ARG(n >= 0 && k >= 0, op, "sizes must be non-negative");
+    PLM_CHECK_ARG(k % kMxBlock == 0, op, "K must be a multiple of 32");
+    PLM_CHECK_ARG(n <= kMxMaxSize && k <= kMxMaxSize, op, "N and K must be at most 2^19");
+    if (n == 0 || k == 0) return PLM_OK;
+    PLM_CHECK_ARG(codes && scale && weight_out && scale_out, op, "null pointer");
+    PLM_CHECK_ARG(aligned(codes, 16) && aligned(weight_out, 16), op, "codes and weight_out must be 16-byte aligned");
+    PLM_CHECK_ARG(aligned(scale_out, 4), op, "scale_out must be 4-byte aligned");
+    const mx_dims d = make_mx_dims(n, k);
+    hipStream_t s = as_stream(stream);
+    const int64_t total = d.strips * d.ktiles * 64, words = d.strips * d.kgroups * 64;
+    mx_repack_codes_kernel<<<static_cast<unsigned>(ceil_div(total, kThreads)), kThreads, 0, s>>>(codes, n, k, d.ktiles, total,
+                                                                                               static_cast<u32x4_t*>(weight_out));
+    mx_repack_scale_kernel<<<static_cast<unsigned>(ceil_div(words, kThreads)), kThreads, 0, s>>>(scale, n, k / kMxBlock, d.kgroups, words,
+                                                                                              static_cast<uint32_t*>(scale_out));
+    PLM_HIP_LAUNCH_CHECK(op);
+    return PLM_OK;
+}
+
+}  // extern "C"

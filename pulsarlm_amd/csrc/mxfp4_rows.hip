@@ -1,0 +1,293 @@
+// MXFP4 products for few rows (one token to short prompts): y[M, N] = x[M, K] @ W^T, the gated block's
+// two products with its activation, and the same with 4-bit x.
+//
+// A workgroup owns RB blocks of 16 rows by SG strips of 16 weight rows over all of K; its wavefronts take
+// the K tiles round-robin, each holding all RB x SG accumulators of its own tiles, and their sums are added
+// through LDS in wavefront order. The weight bytes bound it (they are read once, by one wavefront each,
+// DW K tiles ahead in registers, nontemporal), so nothing is shared before the end and no barrier stands in
+// the K loop. K is not split over workgroups: 16-row strips alone give N / 16 of them, and with DW tiles in
+// flight per wavefront fewer than one workgroup to a CU already draw the memory's rate. x comes as:
+// * staged: all of x in LDS, where it is at most kStagedBytes (then two workgroups fit a CU). Rows past M
+//   are not stored, so their lanes read row M - 1 again. With 4-bit x the lane that holds a block's 32
+//   values quantizes them there: one launch, no scratch.
+// * a ring of two K tiles per wavefront, filled with loads to LDS.
+// * codes in the tile layout, straight to registers.
+// The weights are the matrix instruction's A operand and x its B operand, so that a lane ends with four
+// neighbouring columns of one row: 8-byte stores, and gate and up of a column in one lane.
+#include "mxfp4.hpp"
+
+namespace plm {
+
+namespace {
+
+enum mx_x { kXStaged, kXStagedQuantize, kXRing, kXCodes };
+constexpr int64_t kStagedBytes = 64 * 1024;
+
+struct rows_args {
+    const uint16_t* x;
+    mx_matrix xq, w0, w1;
+    mx_output out;
+    int m, k, ktiles, kgroups, strips, m_blocks;
+};
+
+constexpr int rows_waves(int xm, int rb) { return xm == kXRing && rb > 2 ? 4 : 8; }
+constexpr int rows_ahead(int sg) { return sg <= 2 ? 4 : 2; }
+
+template <int XM, bool BF16, int RB, int SG, mx_epilogue EPI>
+__global__ void __launch_bounds__(rows_waves(XM, RB) * 64) mx_rows_kernel(rows_args a) {
+    constexpr int NW = rows_waves(XM, RB);
+    constexpr int DW = rows_ahead(SG);
+    constexpr bool STAGED = XM == kXStaged || XM == kXStagedQuantize;
+    constexpr int P = EPI == kMxPlain ? SG : SG / 2;                 // strips of one matrix
+    constexpr int SLOT = RB * 4096;                                  // ring: a K tile of x
+    constexpr int XL = RB * 4;                                       // its loads of 1 KiB
+    constexpr int WL = 2 * SG;                                       // loads of a K tile's weights and scales
+    static_assert(!STAGED || RB == 1, "staged x is one row block");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t mx_lds[];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = uniform(threadIdx.x >> 6);
+    const int col16 = lane & 15, kq = lane >> 4;
+    const int strip0 = blockIdx.x / a.m_blocks * P, row0 = (blockIdx.x % a.m_blocks) * RB * 16;
+    const int rows = min(RB * 16, a.m - row0);
+    const int mine = min(P, a.strips - strip0);  // strips past N read zeros
+
+    const int64_t w_at = static_cast<int64_t>(strip0) * a.ktiles * kSubTileBytes, s_at = static_cast<int64_t>(strip0) * a.kgroups * 64;
+    const uint32_t w_bytes = static_cast<uint32_t>(mine) * a.ktiles * kSubTileBytes, s_bytes = static_cast<uint32_t>(mine) * a.kgroups * 256;
+    __amdgpu_buffer_rsrc_t wr[2] = {make_rsrc(a.w0.codes + w_at, w_bytes), make_rsrc(a.w0.codes + w_at, w_bytes)};
+    __amdgpu_buffer_rsrc_t sr[2] = {make_rsrc(a.w0.scale + s_at, s_bytes), make_rsrc(a.w0.scale + s_at, s_bytes)};
+    if constexpr (EPI != kMxPlain) {
+        wr[1] = make_rsrc(a.w1.codes + w_at, w_bytes);
+        sr[1] = make_rsrc(a.w1.scale + s_at, s_bytes);
+    }
+    const int x_pitch = STAGED ? a.kgroups * 1024 : 0;
+    const __amdgpu_buffer_rsrc_t xr =
+        XM == kXCodes ? make_rsrc(a.xq.codes + static_cast<int64_t>(row0 / 16) * a.ktiles * kSubTileBytes,
+                                  static_cast<uint32_t>((rows + 15) / 16) * a.ktiles * kSubTileBytes)
+                      : make_rsrc(a.x + static_cast<int64_t>(row0) * a.k, static_cast<uint32_t>(rows) * a.k * 2);
+    const __amdgpu_buffer_rsrc_t xsr =
+        XM == kXCodes ? make_rsrc(a.xq.scale + static_cast<int64_t>(row0 / 16) * a.kgroups * 64,
+                                  static_cast<uint32_t>((rows + 15) / 16) * a.kgroups * 256)
+                      : xr;
+
+    struct batch {
+        u32x4_t w[SG], x[XM == kXCodes ? RB : 1];
+        uint32_t s[SG], xs[XM == kXCodes ? RB : 1];
+    };
+    auto load = [&](batch& b, int kt) {
+        const bool in = kt < a.ktiles;
+        const int past = in ? 0 : kOOB, w_off = in ? kt * kSubTileBytes : 0, s_off = in ? (kt >> 2) * 256 + (kt & 3) : 0;
+#pragma unroll
+        for (int j = 0; j < SG; ++j) {
+            const int side = j / P, jj = j % P;
+            b.w[j] = buffer_load16_stream(wr[side], (jj * a.ktiles * kSubTileBytes + lane * 16) | past, w_off);
+            b.s[j] = __builtin_amdgcn_raw_buffer_load_b8(sr[side], (jj * a.kgroups * 256 + lane * 4) | past, s_off, 0);
+        }
+        if constexpr (XM == kXCodes) {
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+                b.x[i] = buffer_load16(xr, (i * a.ktiles * kSubTileBytes + lane * 16) | past, w_off);
+                b.xs[i] = __builtin_amdgcn_raw_buffer_load_b8(xsr, (i * a.kgroups * 256 + lane * 4) | past, s_off, 0);
+            }
+        }
+    };
+    // Ring: a load's 64 lanes fill four rows of 256 bytes; the 16-byte columns are XOR-swizzled by row, so
+    // that the 16 rows of a fragment read fall in different banks.
+    uint8_t* ring = mx_lds + wave * 2 * SLOT;
+    auto load_x = [&](int kt, int slot) {
+        if constexpr (XM == kXRing) {
+            const bool in = kt < a.ktiles;
+#pragma unroll
+            for (int i = 0; i < XL; ++i) {
+                const int r = 4 * i + (lane >> 4), c = (lane & 15) ^ (r & 15);
+                const bool ok = in && kt * kTileK + 8 * c < a.k;  // rows past `rows` are past the buffer's end
+                buffer_load_lds16(xr, ring + slot * SLOT + i * 1024, ok ? r * a.k * 2 + c * 16 : kOOB, in ? kt * 256 : 0);
+            }
+        }
+    };
+
+    f32x4_t acc[RB][SG];
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int j = 0; j < SG; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    int slot = 0;
+    auto multiply = [&](const batch& b, int kt) {
+        const uint8_t* xt[RB];
+        int swz = 0;
+        if constexpr (STAGED) {
+            const int r = min(col16, rows - 1);
+            xt[0] = mx_lds + r * x_pitch + kt * 256;
+            swz = r & 15;
+        } else if constexpr (XM == kXRing) {
+#pragma unroll
+            for (int i = 0; i < RB; ++i) xt[i] = ring + slot * SLOT + (16 * i + col16) * 256;
+            swz = col16;
+        }
+        if constexpr (XM == kXCodes) {
+#pragma unroll
+            for (int i = 0; i < RB; ++i)
+#pragma unroll
+                for (int j = 0; j < SG; ++j) acc[i][j] = mx_mfma<0, 0>(b.w[j], b.s[j], b.x[i], b.xs[i], acc[i][j]);
+        } else if constexpr (XM == kXStagedQuantize) {
+            float v[4][8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const u32x4_t f = *reinterpret_cast<const u32x4_t*>(xt[0] + (((4 * kq + q) ^ swz) << 4));
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    v[q][2 * h] = from_bits16<BF16>(f[h] & 0xffffu);
+                    v[q][2 * h + 1] = from_bits16<BF16>(f[h] >> 16);
+                    top = max(top, max(mx_magnitude(v[q][2 * h]), mx_magnitude(v[q][2 * h + 1])));
+                }
+            }
+            const uint32_t s = mx_scale_byte(top);
+            u32x4_t x;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = mx_encode8(v[q], s);
+#pragma unroll
+            for (int j = 0; j < SG; ++j) acc[0][j] = mx_mfma<0, 0>(b.w[j], b.s[j], x, s, acc[0][j]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                u32x4_t x[RB];
+#pragma unroll
+                for (int i = 0; i < RB; ++i) x[i] = *reinterpret_cast<const u32x4_t*>(xt[i] + (((4 * kq + q) ^ swz) << 4));
+#pragma unroll
+                for (int j = 0; j < SG; ++j) {
+                    const u32x4_t w = mx_decode<BF16>(b.w[j][q], mx_scale(b.s[j]));
+#pragma unroll
+                    for (int i = 0; i < RB; ++i) acc[i][j] = mfma16x16x32<BF16>(w, x[i], acc[i][j]);
+                }
+            }
+        }
+    };
+
+    batch b[DW];
+#pragma unroll
+    for (int d = 0; d < DW - 1; ++d) load(b[d], wave + d * NW);
+    if constexpr (STAGED) {
+        // Row r's K group q (512 values, 1 KiB), swizzled within each K tile.
+        for (int i = wave; i < rows * a.kgroups; i += NW) {
+            const int r = i / a.kgroups, q = i % a.kgroups;
+            const int c = (lane & 48) | ((lane & 15) ^ (r & 15)), at = q * 512 + c * 8;
+            buffer_load_lds16(xr, mx_lds + i * 1024, at < a.k ? (r * a.k + at) * 2 : kOOB, 0);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+    load_x(wave, 0);
+    for (int kt = wave; kt < a.ktiles; kt += DW * NW) {
+#pragma unroll
+        for (int d = 0; d < DW; ++d) {
+            const int cur = kt + d * NW;
+            if (cur >= a.ktiles) break;
+            load(b[(d + DW - 1) % DW], cur + (DW - 1) * NW);
+            if constexpr (XM == kXRing) {
+                // The other slot's reads are over; this slot's loads are older than this step's.
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                load_x(cur + NW, slot ^ 1);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(WL + XL) : "memory");
+            }
+            multiply(b[d], cur);
+            slot ^= 1;
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // requests past the last tile
+    __syncthreads();
+
+    // Sums over the wavefronts, in wavefront order.
+    f32x4_t* red = reinterpret_cast<f32x4_t*>(mx_lds);
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int j = 0; j < SG; ++j) red[((i * SG + j) * NW + wave) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    auto total = [&](int i, int j, int ln) {
+        const f32x4_t* p = red + (i * SG + j) * NW * 64 + ln;
+        f32x4_t v = p[0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v = v + p[w * 64];
+        return v;
+    };
+    constexpr int PER = EPI == kMxGatedCodes ? 1 : P;  // items of 64 lanes per row block
+    for (int u = threadIdx.x; u < RB * PER * 64; u += NW * 64) {
+        const int ln = u & 63, i = (u >> 6) / PER, p = (u >> 6) % PER;
+        const int r = 16 * i + (ln & 15);
+        if constexpr (EPI == kMxGatedCodes) {
+            static_assert(P == 2 || EPI != kMxGatedCodes, "a block is two strips");
+            const f32x4_t g[2] = {total(i, 0, ln), total(i, 1, ln)}, h[2] = {total(i, P, ln), total(i, P + 1, ln)};
+            if (16 * i < rows) mx_store_codes(a.out, row0 / 16 + i, strip0 >> 1, g, h);  // wave-uniform
+        } else {
+            const int col = (strip0 + p) * kTileN + 4 * (ln >> 4);
+            const f32x4_t v = total(i, p, ln);
+            if constexpr (EPI == kMxPlain) {
+                if (r < rows) mx_store_plain<BF16>(a.out, row0 + r, col, v);
+            } else {
+                const f32x4_t up = total(i, P + p, ln);
+                if (r < rows) mx_store_gated<BF16>(a.out, row0 + r, col, v, up);
+            }
+        }
+    }
+}
+
+template <int XM, bool BF16, int RB, int SG, mx_epilogue EPI> void launch(const mx_product& p, hipStream_t s) {
+    const mx_dims d = make_mx_dims(p.n, p.k);
+    rows_args a{};
+    a.x = p.x16;
+    a.xq = p.xq;
+    a.w0 = p.w0;
+    a.w1 = p.w1;
+    a.out = p.out;
+    a.m = static_cast<int>(p.m);
+    a.k = static_cast<int>(p.k);
+    a.ktiles = static_cast<int>(d.ktiles);
+    a.kgroups = static_cast<int>(d.kgroups);
+    a.strips = static_cast<int>(d.strips);
+    a.m_blocks = static_cast<int>(ceil_div(p.m, RB * 16));
+    constexpr int NW = rows_waves(XM, RB);
+    int64_t loop = 0;
+    if (XM == kXStaged || XM == kXStagedQuantize) loop = p.m * d.kgroups * 1024;
+    if (XM == kXRing) loop = int64_t{NW} * 2 * RB * 4096;
+    const int64_t lds = std::max<int64_t>(loop, int64_t{RB} * SG * NW * 1024);
+    constexpr int P = EPI == kMxPlain ? SG : SG / 2;
+    const int64_t grid = ceil_div(d.strips, P) * a.m_blocks;
+    mx_rows_kernel<XM, BF16, RB, SG, EPI><<<static_cast<unsigned>(grid), NW * 64, static_cast<size_t>(lds), s>>>(a);
+}
+
+template <int XM, bool BF16, int RB> void launch_sg(const mx_product& p, hipStream_t s) {
+    if constexpr (XM == kXCodes || XM == kXStagedQuantize) {
+        if (p.epilogue == kMxGatedCodes) return launch<XM, BF16, RB, 4, kMxGatedCodes>(p, s);
+    }
+    if constexpr (XM == kXStaged || XM == kXRing) {
+        if (p.epilogue == kMxGated) return launch<XM, BF16, RB, 2, kMxGated>(p, s);
+    }
+    launch<XM, BF16, RB, 1, kMxPlain>(p, s);
+}
+
+bool staged(const mx_product& p) { return p.m <= 16 && p.m * ceil_div(p.k, 512) * 1024 <= kStagedBytes; }
+
+template <bool BF16> void launch_typed(const mx_product& p, bool quantize_x, hipStream_t s) {
+    if (quantize_x) return launch_sg<kXStagedQuantize, BF16, 1>(p, s);
+    if (p.xq.codes != nullptr) {
+        if (p.m <= 16) launch_sg<kXCodes, BF16, 1>(p, s);
+        else if (p.m <= 32) launch_sg<kXCodes, BF16, 2>(p, s);
+        else launch_sg<kXCodes, BF16, 4>(p, s);
+    } else if (staged(p)) launch_sg<kXStaged, BF16, 1>(p, s);
+    else if (p.m <= 16) launch_sg<kXRing, BF16, 1>(p, s);
+    else if (p.m <= 32) launch_sg<kXRing, BF16, 2>(p, s);
+    else launch_sg<kXRing, BF16, 4>(p, s);
+}
+
+}  // namespace
+
+bool launch_mx_rows(const mx_product& p, bool quantize_x, hipStream_t s) {
+    if (p.m > 64 || (quantize_x && !staged(p))) return false;
+    if (p.bf16) launch_typed<true>(p, quantize_x, s);
+    else launch_typed<false>(p, quantize_x, s);
+    return true;
+}
+
+}  // namespace plm

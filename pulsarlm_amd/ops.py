@@ -385,3 +385,190 @@ def gemm_int4_split_cuda(x: torch.Tensor, weight_packed: torch.Tensor, weight_sc
     """gemm_int4_split_cuda (ops.hpp:287-297): the same with the K split forced to num_splits (>= 1)."""
     _require(num_splits >= 1, "gemm_int4", "num_splits must be >= 1")
     return _gemm_int4_plain("gemm_int4", x, weight_packed, weight_scale, group_size, num_splits)
+
+
+# ---------------------------------------------------------------------------
+# MXFP4: microscaled 4-bit floating point (no reference counterpart). 32 consecutive K values share a scale
+# 2^(b - 127) and are e2m1 codes; plain form: codes uint8 [M, K/2] (lower K in the low half), scale uint8 [M, K/32].
+# ---------------------------------------------------------------------------
+
+
+def _mx_contiguous(op: str, name: str, x: torch.Tensor, dtypes) -> None:
+    _require(x.is_cuda and x.dtype in dtypes, op, f"{name} must be a CUDA {'fp32, ' if len(dtypes) > 2 else ''}fp16 or bf16 tensor")
+    _require(x.dim() == 2 and x.is_contiguous(), op, f"{name} must be contiguous [rows, columns]")
+
+
+_HALF = (torch.float16, torch.bfloat16)
+
+
+def quantize_mxfp4_cuda(x: torch.Tensor):
+    """x [M, K] (fp32, fp16 or bf16, K a multiple of 32) -> (codes uint8 [M, K/2], scale uint8 [M, K/32]): scale byte
+    floor(log2(amax)) - 2 + 127 per block of 32, codes to nearest (ties to the even code), saturating at 6. A block
+    with an infinity or NaN gets scale byte 255, which reads as NaN."""
+    op = "quantize_mxfp4"
+    _mx_contiguous(op, "x", x, _DTYPES)
+    m, k = x.shape
+    _require(k % 32 == 0, op, "K must be a multiple of 32")
+    codes = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
+    scale = torch.empty((m, k // 32), dtype=torch.uint8, device=x.device)
+    with _on(x.device):
+        _call("plm_quantize_mxfp4", _ptr(x), _DTYPES[x.dtype], m, k, _ptr(codes), _ptr(scale), _stream(x.device))
+    return codes, scale
+
+
+def _mx_plain(op: str, codes: torch.Tensor, scale: torch.Tensor):
+    _require(codes.is_cuda and scale.is_cuda and codes.device == scale.device, op, "codes and scale must be on one CUDA device")
+    _require(codes.dtype == torch.uint8 and scale.dtype == torch.uint8 and codes.dim() == 2 and scale.dim() == 2, op,
+             "codes must be uint8 [N, K/2] and scale uint8 [N, K/32]")
+    n, k = codes.shape[0], 2 * codes.shape[1]
+    _require(k % 32 == 0, op, "K must be a multiple of 32")
+    _require(tuple(scale.shape) == (n, k // 32), op, "scale must be [N, K/32]")
+    return n, k
+
+
+def dequantize_mxfp4_cuda(codes: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values [M, K] that codes and scale stand for: exact in bf16 and fp32, rounded once to fp16."""
+    op = "dequantize_mxfp4"
+    m, k = _mx_plain(op, codes, scale)
+    _require(dtype in _DTYPES, op, "dtype must be fp32, fp16 or bf16")
+    out = torch.empty((m, k), dtype=dtype, device=codes.device)
+    with _on(codes.device):
+        _call("plm_dequantize_mxfp4", _ptr(codes.contiguous()), _ptr(scale.contiguous()), m, k, _ptr(out), _DTYPES[dtype],
+              _stream(codes.device))
+    return out
+
+
+def repack_mxfp4_cuda(codes: torch.Tensor, scale: torch.Tensor):
+    """An MXFP4 weight [N, K] (codes uint8 [N, K/2], scale uint8 [N, K/32]) for the products: (weight int32 1-D,
+    scale int32 [strips, groups, 64]), opaque, the plm tile layout of the format."""
+    op = "repack_mxfp4"
+    n, k = _mx_plain(op, codes, scale)
+    weight = torch.empty((_lib.mxfp4_bytes("mxfp4_weight_bytes", n, k) // 4,), dtype=torch.int32, device=codes.device)
+    packed = torch.empty(_mx_scale_shape(n, k), dtype=torch.int32, device=codes.device)
+    with _on(codes.device):
+        _call("plm_repack_mxfp4", _ptr(codes.contiguous()), _ptr(scale.contiguous()), n, k, _ptr(weight), _ptr(packed),
+              _stream(codes.device))
+    return weight, packed
+
+
+def _mx_scale_shape(n: int, k: int):
+    return -(-n // 16), -(-k // 512), 64
+
+
+def _mx_weight(op: str, x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, n: int, k: int) -> None:
+    _require(n >= 0 and k >= 0, op, "sizes must be non-negative")
+    _require(weight.device == x.device and scale.device == x.device, op, "x and the weights must be on one device")
+    _require(weight.dtype == torch.int32 and scale.dtype == torch.int32 and weight.is_contiguous() and scale.is_contiguous(), op,
+             "weight and scale must be contiguous int32, as repack_mxfp4 returns them")
+    _require(weight.numel() * 4 == _lib.mxfp4_bytes("mxfp4_weight_bytes", n, k), op, "weight has the wrong size for this shape")
+    _require(tuple(scale.shape) == _mx_scale_shape(n, k), op, "scale has the wrong shape for this N and K")
+
+
+def _mx_scratch(name: str, x: torch.Tensor, *sizes: int) -> torch.Tensor | None:
+    """Scratch of one call, from torch's allocator: a captured call's belongs to its graph."""
+    nbytes = _lib.mxfp4_bytes(name + "_workspace_bytes", *sizes)
+    return torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes > 0 else None
+
+
+def _mx_out(op: str, x: torch.Tensor, shape, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=x.dtype, device=x.device)
+    _require(out.dtype == x.dtype and out.device == x.device and tuple(out.shape) == shape and out.is_contiguous(), op,
+             f"out must be contiguous {list(shape)} of x's dtype and device")
+    return out
+
+
+def _mx_x(op: str, x: torch.Tensor):
+    _mx_contiguous(op, "x", x, _HALF)
+    _require(x.shape[1] % 32 == 0, op, "K must be a multiple of 32")
+    return x.shape
+
+
+def gemm_mxfp4_cuda(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, n: int, out=None) -> torch.Tensor:
+    """y [M, N] = x [M, K] @ W^T with an MXFP4 weight (repack_mxfp4_cuda) and 16-bit x, fp32 sums."""
+    op = "gemm_mxfp4"
+    m, k = _mx_x(op, x)
+    _mx_weight(op, x, weight, scale, n, k)
+    y = _mx_out(op, x, (m, n), out)
+    with _on(x.device):
+        _call("plm_gemm_mxfp4", _ptr(x), _DTYPES[x.dtype], _ptr(weight), _ptr(scale), m, n, k, _ptr(y), _stream(x.device))
+    return y
+
+
+def gemm_mxfp4_w4a4_cuda(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, n: int, out=None) -> torch.Tensor:
+    """W4A4: the same with x quantized as by quantize_mxfp4_cuda, on the fp4 matrix instruction."""
+    op = "gemm_mxfp4_w4a4"
+    m, k = _mx_x(op, x)
+    _mx_weight(op, x, weight, scale, n, k)
+    y = _mx_out(op, x, (m, n), out)
+    ws = _mx_scratch(op, x, m, n, k)
+    with _on(x.device):
+        _call("plm_gemm_mxfp4_w4a4", _ptr(x), _DTYPES[x.dtype], _ptr(weight), _ptr(scale), m, n, k, _ptr(y), _ptr(ws),
+              0 if ws is None else ws.numel(), _stream(x.device))
+    return y
+
+
+def gemm_mxfp4_grad_cuda(dy: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, k: int, out=None) -> torch.Tensor:
+    """The gradient of gemm_mxfp4_cuda's x: dx [M, K] = dy [M, N] @ W."""
+    op = "gemm_mxfp4_grad"
+    _mx_contiguous(op, "dy", dy, _HALF)
+    _require(k % 32 == 0, op, "K must be a multiple of 32")
+    m, n = dy.shape
+    _mx_weight(op, dy, weight, scale, n, k)
+    dx = _mx_out(op, dy, (m, k), out)
+    ws = _mx_scratch(op, dy, m, n, k)
+    with _on(dy.device):
+        _call("plm_gemm_mxfp4_grad", _ptr(dy), _DTYPES[dy.dtype], _ptr(weight), _ptr(scale), m, n, k, _ptr(dx), _ptr(ws),
+              0 if ws is None else ws.numel(), _stream(dy.device))
+    return dx
+
+
+def gated_mxfp4_cuda(x: torch.Tensor, gate: tuple, up: tuple, intermediate: int, keep_gate_up: bool = False):
+    """h [M, I] = silu(x @ Wgate^T) * (x @ Wup^T) in one kernel, from fp32 sums; gate and up are (weight, scale) pairs
+    of repack_mxfp4_cuda. keep_gate_up: (h, gate_up fp32 [M, 2 I]), what gated_mxfp4_grad_cuda takes."""
+    op = "gated_mxfp4"
+    m, k = _mx_x(op, x)
+    for w in (gate, up):
+        _mx_weight(op, x, w[0], w[1], intermediate, k)
+    h = torch.empty((m, intermediate), dtype=x.dtype, device=x.device)
+    gate_up = torch.empty((m, 2 * intermediate), dtype=torch.float32, device=x.device) if keep_gate_up else None
+    with _on(x.device):
+        _call("plm_gated_mxfp4", _ptr(x), _DTYPES[x.dtype], _ptr(gate[0]), _ptr(gate[1]), _ptr(up[0]), _ptr(up[1]), m,
+              intermediate, k, _ptr(h), _ptr(gate_up), _stream(x.device))
+    return (h, gate_up) if keep_gate_up else h
+
+
+def gated_mxfp4_grad_cuda(dh: torch.Tensor, gate_up: torch.Tensor, gate: tuple, up: tuple, hidden: int) -> torch.Tensor:
+    """The gradient of gated_mxfp4_cuda's x [M, hidden] from dh [M, I] and the gate_up that it kept."""
+    op = "gated_mxfp4_grad"
+    _mx_contiguous(op, "dh", dh, _HALF)
+    _require(hidden % 32 == 0, op, "K must be a multiple of 32")
+    m, n = dh.shape
+    _require(gate_up.dtype == torch.float32 and gate_up.device == dh.device and tuple(gate_up.shape) == (m, 2 * n) and
+             gate_up.is_contiguous(), op, "gate_up must be contiguous fp32 [M, 2 I] on dh's device")
+    for w in (gate, up):
+        _mx_weight(op, dh, w[0], w[1], n, hidden)
+    dx = torch.empty((m, hidden), dtype=dh.dtype, device=dh.device)
+    ws = _mx_scratch(op, dh, m, n, hidden)
+    with _on(dh.device):
+        _call("plm_gated_mxfp4_grad", _ptr(dh), _ptr(gate_up), _DTYPES[dh.dtype], _ptr(gate[0]), _ptr(gate[1]), _ptr(up[0]),
+              _ptr(up[1]), m, n, hidden, _ptr(dx), _ptr(ws), 0 if ws is None else ws.numel(), _stream(dh.device))
+    return dx
+
+
+def mlp_mxfp4_w4a4_cuda(x: torch.Tensor, gate: tuple, up: tuple, down: tuple, intermediate: int) -> torch.Tensor:
+    """The feed-forward block with 4-bit activations: y [M, K] = Q(h) @ Wdown^T, h = silu(g) u of Q(x), Q as
+    quantize_mxfp4_cuda; h is quantized from its fp32 values. Wgate, Wup [I, K], Wdown [K, I]; I a multiple of 32."""
+    op = "mlp_mxfp4_w4a4"
+    m, k = _mx_x(op, x)
+    _require(intermediate % 32 == 0, op, "the intermediate size must be a multiple of 32")
+    for w in (gate, up):
+        _mx_weight(op, x, w[0], w[1], intermediate, k)
+    _mx_weight(op, x, down[0], down[1], k, intermediate)
+    y = torch.empty_like(x)
+    ws = _mx_scratch(op, x, m, intermediate, k)
+    with _on(x.device):
+        _call("plm_mlp_mxfp4_w4a4", _ptr(x), _DTYPES[x.dtype], _ptr(gate[0]), _ptr(gate[1]), _ptr(up[0]), _ptr(up[1]),
+              _ptr(down[0]), _ptr(down[1]), m, intermediate, k, _ptr(y), _ptr(ws), 0 if ws is None else ws.numel(),
+              _stream(x.device))
+    return y
