@@ -6,9 +6,9 @@
 // 16-byte load per lane, the operand of v_mfma_scale_f32_16x16x128_f8f6f4 (whose lane group g carries
 // block g, with the block's scale in a byte of the lane's scale register) and, word j converted with
 // that one scale, the operand of v_mfma_f32_16x16x32 for K = 32 g + 8 j + 0..7. The scales are
-// [strips][groups of 4 K tiles][64 lanes] dwords, byte t that of K tile 4 q + t: one load serves 512 K
-// values and the matrix instruction picks the byte. Padding rows, and columns past K, hold code and
-// scale 0.
+// [groups of 4 strips][K tiles][64 lanes] dwords, byte j that of the group's strip j: one load serves a
+// wavefront's four strips, and the matrix instruction picks the byte. Padding rows of a weight, and columns
+// past K, hold code and scale 0.
 #pragma once
 
 #include <algorithm>
@@ -21,15 +21,15 @@ constexpr int kMxBlock = 32;
 constexpr int64_t kMxMaxSize = int64_t{1} << 19;  // N, K: the byte offsets of one workgroup's buffers stay below kOOB
 
 struct mx_dims {
-    int64_t strips, ktiles, kgroups;
+    int64_t strips, ktiles, groups;  // groups of 4 strips
     int64_t tile_bytes() const { return strips * ktiles * kSubTileBytes; }
-    int64_t scale_bytes() const { return strips * kgroups * 256; }
+    int64_t scale_bytes() const { return groups * ktiles * 256; }
 };
 inline mx_dims make_mx_dims(int64_t rows, int64_t k) {
     mx_dims d;
     d.strips = ceil_div(rows, kTileN);
     d.ktiles = ceil_div(k, kTileK);
-    d.kgroups = ceil_div(d.ktiles, 4);
+    d.groups = ceil_div(d.strips, 4);
     return d;
 }
 
@@ -104,8 +104,9 @@ struct mx_output {
     float* gate_up;      // kMxGated: [g | u] [M, 2 N], or null
     uint8_t* codes;      // kMxGatedCodes
     uint8_t* scale;
-    int n, ktiles, kgroups;  // columns; of the codes' layout
+    int n, ktiles;       // columns; K tiles of the codes' layout
     bool wide;               // four columns a store: N % 4 == 0 and 8-byte aligned pointers
+    bool lines;              // eight: N % 8 == 0 and y 16-byte aligned
 };
 
 template <bool BF16> __device__ __forceinline__ void mx_store4(uint16_t* p, int col, int n, bool wide, const float (&v)[4]) {
@@ -123,12 +124,8 @@ template <bool BF16> __device__ __forceinline__ void mx_store_plain(const mx_out
     const float f[4] = {v[0], v[1], v[2], v[3]};
     mx_store4<BF16>(o.y + row * o.n + col, col, o.n, o.wide, f);
 }
-template <bool BF16>
-__device__ __forceinline__ void mx_store_gated(const mx_output& o, int64_t row, int col, const f32x4_t& g, const f32x4_t& u) {
-    float h[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) h[r] = mx_gated(g[r], u[r]);
-    mx_store4<BF16>(o.y + row * o.n + col, col, o.n, o.wide, h);
+// [g | u] of columns col .. col + 3 of one row, where the caller keeps them.
+__device__ __forceinline__ void mx_store_gate_up(const mx_output& o, int64_t row, int col, const f32x4_t& g, const f32x4_t& u) {
     // Kept in 32 bits: rounded to 16 they cost the gradient as much as its own last rounding does (its error
     // against float64 is 3.0e-3 with bf16 g and u, 2.3e-3 with these; one bf16 rounding is 1.7e-3).
     if (o.gate_up != nullptr) {
@@ -141,6 +138,9 @@ __device__ __forceinline__ void mx_store_gated(const mx_output& o, int64_t row, 
                 if (col + r < o.n) p[r] = g[r], p[o.n + r] = u[r];
         }
     }
+}
+__device__ __forceinline__ f32x4_t mx_gated4(const f32x4_t& g, const f32x4_t& u) {
+    return f32x4_t{mx_gated(g[0], u[0]), mx_gated(g[1], u[1]), mx_gated(g[2], u[2]), mx_gated(g[3], u[3])};
 }
 // One block of 32 columns (slices 2 block and 2 block + 1 of 16) of 16 rows, held by a wavefront: lane
 // r + 16 g has row r's columns 4 g .. 4 g + 3 of either slice. All 64 lanes take part.
@@ -162,18 +162,15 @@ __device__ __forceinline__ void mx_store_codes(const mx_output& o, int strip, in
     uint16_t* c = reinterpret_cast<uint16_t*>(o.codes + tile * kSubTileBytes + at * 16) + (lane >> 4);
     c[0] = static_cast<uint16_t>(q);
     c[4] = static_cast<uint16_t>(q >> 16);
-    uint8_t* s = o.scale + ((static_cast<int64_t>(strip) * o.kgroups + (block >> 4)) * 64 + at) * 4 + (block >> 2 & 3);
+    uint8_t* s = o.scale + ((static_cast<int64_t>(strip >> 2) * o.ktiles + (block >> 2)) * 64 + at) * 4 + (strip & 3);
     if (lane < 16) *s = static_cast<uint8_t>(b);
-    // Blocks past the end: the last tile's codes are read, and the scale bytes of the whole group of 4 tiles.
-    if (32 * (block + 1) >= o.n) {
-        for (int e = block + 1; (e & 15) != 0; ++e) {
-            const int to = (lane & 15) + 16 * (e & 3);
-            if ((e >> 2) == (block >> 2)) {
-                uint16_t* z = reinterpret_cast<uint16_t*>(o.codes + tile * kSubTileBytes + to * 16) + (lane >> 4);
-                z[0] = 0;
-                z[4] = 0;
-            }
-            if (lane < 16) o.scale[((static_cast<int64_t>(strip) * o.kgroups + (block >> 4)) * 64 + to) * 4 + (e >> 2 & 3)] = 0;
+    if (32 * (block + 1) >= o.n) {  // the last tile's blocks past the end are read, too
+        for (int e = (block & 3) + 1; e < 4; ++e) {
+            c += 16 * 8;
+            s += 16 * 4;
+            c[0] = 0;
+            c[4] = 0;
+            if (lane < 16) *s = 0;
         }
     }
 }
@@ -183,6 +180,7 @@ inline mx_output mx_make_output(void* y, void* gate_up, int64_t n) {
     o.y = static_cast<uint16_t*>(y);
     o.gate_up = static_cast<float*>(gate_up);
     o.n = static_cast<int>(n);
+    o.lines = n % 8 == 0 && aligned(y, 16);
     o.wide = n % 4 == 0 && aligned(y, 8) && aligned(gate_up, 16);
     return o;
 }

@@ -181,7 +181,6 @@ int plm_mlp_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* gate_weight
     act.codes = hq.codes;
     act.scale = reinterpret_cast<uint8_t*>(hq.scale);
     act.ktiles = static_cast<int>(hd.ktiles);
-    act.kgroups = static_cast<int>(hd.kgroups);
     run_w4a4(product(x, x_dtype, matrix(gate_weight, gate_scale), matrix(up_weight, up_scale), m, n, k, kMxGatedCodes, act), xq, s);
     PLM_HIP_LAUNCH_CHECK(op);
     mx_product down = product(nullptr, x_dtype, matrix(down_weight, down_scale), {}, m, k, n, kMxPlain, mx_make_output(y, nullptr, k));

@@ -27,7 +27,7 @@ struct grad_args {
     uint16_t* dx;
     float* partial;  // [splits][M][K]
     int64_t pitch;
-    int m, k, ktiles, kgroups, strips;
+    int m, k, ktiles, strips;
     int side_steps, steps, split_steps, splits;
     int m_blocks, n_blocks;
 };
@@ -67,22 +67,15 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
         asm volatile("" : "+v"(l));
         return l;
     };
-    auto load_x = [&](step_data& b, int s) {
+    auto load_x = [&](step_data& b, int i, int s) {
         const int lane = own_lane();
         const int past = s < hi ? 0 : kOOB, off = s < hi ? s * 128 : 0;
-#pragma unroll
-        for (int i = 0; i < XPW; ++i) {
-            const int r = 8 * (wave * XPW + i) + (lane >> 3);  // rows past the last are past the buffer's end
-            b.x[i] = buffer_load16(xr, (static_cast<int>(r * a.pitch * 2) + (lane & 7) * 16) | past, off);
-        }
+        const int r = 8 * (wave * XPW + i) + (lane >> 3);  // rows past the last are past the buffer's end
+        b.x[i] = buffer_load16(xr, (static_cast<int>(r * a.pitch * 2) + (lane & 7) * 16) | past, off);
     };
-    auto write_x = [&](const step_data& b, int slot) {
-        const int lane = own_lane();
-#pragma unroll
-        for (int i = 0; i < XPW; ++i) {
-            const int r = 8 * (wave * XPW + i) + (lane >> 3);
-            *reinterpret_cast<u32x4_t*>(lds + slot * XS + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = b.x[i];  // 16-byte columns swizzled by row
-        }
+    auto write_x = [&](const step_data& b, int i, int slot) {
+        const int lane = own_lane(), r = 8 * (wave * XPW + i) + (lane >> 3);
+        *reinterpret_cast<u32x4_t*>(lds + slot * XS + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = b.x[i];  // 16-byte columns swizzled by row
     };
 
     // Wavefront w decodes one tile of a step: strip w / 2, K tile w % 2 (the second may lie past K).
@@ -96,18 +89,16 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
         const int64_t at = in ? strip : 0, t = in ? kt : 0;
         const int past = in ? 0 : kOOB;
         b.c = buffer_load16(make_rsrc(base + (at * a.ktiles + t) * kSubTileBytes, kSubTileBytes), (lane * 16) | past);
-        b.s = buffer_load_u32(make_rsrc(sbase + (at * a.kgroups + (t >> 2)) * 64, 256u), (lane * 4) | past, 0);
+        b.s = buffer_load_u32(make_rsrc(sbase + ((at >> 2) * a.ktiles + t) * 64, 256u), (lane * 4) | past, 0);
     };
     // LDS row n (512 bytes): its 32-byte pieces are XOR-swizzled by f(n) = n % 4 + 4 ((n / 4 + n / 8) % 2),
     // which sets apart both the eight rows that one write covers and the rows of one transposing read.
-    auto write_w = [&](const step_data& b, int slot) {
+    auto write_w = [&](const step_data& b, int q, int slot) {
         const int lane = own_lane(), col16 = lane & 15, kq = lane >> 4;
         const int wrow = (wave >> 1) * 16 + col16, wf = (col16 & 3) | ((((col16 >> 2) ^ (col16 >> 3)) & 1) << 2);
         uint8_t* base = wlds + slot * WS + wrow * 512;
-        const float s = mx_scale(b.s >> (8 * (kt & 3)) & 0xffu);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<u32x4_t*>(base + ((((wave & 1) * 8 + 2 * kq + (q >> 1)) ^ wf) << 5) + (q & 1) * 16) = mx_decode<BF16>(b.c[q], s);
+        const float s = mx_scale(b.s >> (8 * (wave >> 1)) & 0xffu);
+        *reinterpret_cast<u32x4_t*>(base + ((((wave & 1) * 8 + 2 * kq + (q >> 1)) ^ wf) << 5) + (q & 1) * 16) = mx_decode<BF16>(b.c[q], s);
     };
 
     u32x4_t x[MT], w[2][NS];  // fragments; x's are read again for the next half right after their use
@@ -137,11 +128,15 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
         for (int j = 0; j < NS; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     step_data b;
-    load_x(b, lo);
+#pragma unroll
+    for (int i = 0; i < XPW; ++i) load_x(b, i, lo);
     load_w(b, lo);
-    write_x(b, 0);
-    write_w(b, 0);
-    load_x(b, lo + 1);
+#pragma unroll
+    for (int i = 0; i < XPW; ++i) write_x(b, i, 0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) write_w(b, q, 0);
+#pragma unroll
+    for (int i = 0; i < XPW; ++i) load_x(b, i, lo + 1);
     load_w(b, lo + 1);
     __syncthreads();
     lane_offsets o = fragment_offsets();
@@ -151,14 +146,20 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
     for (int j = 0; j < NS; ++j) read_w(o, w[0], j, 0, 0);
     int slot = 0;
     for (int s = lo; s < hi; ++s) {
-        write_x(b, slot ^ 1);
-        write_w(b, slot ^ 1);
-        __builtin_amdgcn_sched_barrier(0);  // the next data go into the same registers
-        load_x(b, s + 2);
-        load_w(b, s + 2);
         o = fragment_offsets();
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
+            // The other slot is filled over the first rows of matrix instructions, and the data of the step
+            // after requested over the last ones into the same registers.
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (q * MT / 8 == i) write_w(b, q, slot ^ 1);
+#pragma unroll
+            for (int q = 0; q < XPW; ++q) {
+                if (q * MT / 8 == i) write_x(b, q, slot ^ 1);
+                if (MT / 2 + q * MT / 8 == i) load_x(b, q, s + 2);
+            }
+            if (i == MT - 1) load_w(b, s + 2);
 #pragma unroll
             for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(o, w[1], j, slot, 1);
 #pragma unroll
@@ -325,7 +326,6 @@ int run(const char* op, bool gated, const void* dy, const void* gate_up, const m
     a.m = static_cast<int>(m);
     a.k = static_cast<int>(k);
     a.ktiles = static_cast<int>(d.ktiles);
-    a.kgroups = static_cast<int>(d.kgroups);
     a.strips = static_cast<int>(d.strips);
     a.steps = static_cast<int>(p.steps);
     a.splits = static_cast<int>(p.splits);

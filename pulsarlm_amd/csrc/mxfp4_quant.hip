@@ -53,21 +53,20 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T* __restri
     }
 }
 
-// One workgroup: 16 rows by a group of 4 K tiles, in the tile layout. A quad of lanes takes a block; the
-// four scale bytes of a lane's dword are the blocks that the quad meets in turn.
+// One workgroup: a group of 4 strips (64 rows) by one K tile, in the tile layout. A quad of lanes takes a
+// block of each strip; the four scale bytes are its dword of the group's scales.
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads) mx_quantize_tiles_kernel(const uint16_t* __restrict__ x, int64_t m, int k, int ktiles,
-                                                                     int kgroups, uint8_t* __restrict__ codes,
+                                                                     int64_t strips, uint8_t* __restrict__ codes,
                                                                      uint32_t* __restrict__ scale) {
-    const int64_t strip = blockIdx.x / kgroups;
-    const int q = blockIdx.x % kgroups;
+    const int64_t group = blockIdx.x / ktiles;
+    const int kt = blockIdx.x % ktiles;
     const int quad = threadIdx.x >> 2, part = threadIdx.x & 3;
-    const int64_t row = strip * 16 + (quad & 15);
-    const int block = quad >> 4;
+    const int col = kt * kTileK + (quad >> 4) * kMxBlock + part * 8;
     float v[4][8];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        const int col = (4 * q + t) * kTileK + block * kMxBlock + part * 8;
+        const int64_t row = (4 * group + t) * 16 + (quad & 15);
         if (row < m && col < k) load8<uint16_t, BF16>(x + row * k + col, v[t]);
         else
             for (int i = 0; i < 8; ++i) v[t][i] = 0.f;
@@ -78,10 +77,10 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_tiles_kernel(const uint1
         uint32_t b;
         const uint32_t c = encode_in_quad(v[t], b);
         bytes |= b << (8 * t);
-        const int kt = 4 * q + t;
-        if (kt < ktiles) *reinterpret_cast<uint32_t*>(codes + (strip * ktiles + kt) * kSubTileBytes + quad * 16 + part * 4) = c;
+        const int64_t strip = 4 * group + t;
+        if (strip < strips) *reinterpret_cast<uint32_t*>(codes + (strip * ktiles + kt) * kSubTileBytes + quad * 16 + part * 4) = c;
     }
-    if (part == 0) scale[(strip * kgroups + q) * 64 + quad] = bytes;
+    if (part == 0) scale[(group * ktiles + kt) * 64 + quad] = bytes;
 }
 
 // OUT: 0 bf16, 1 fp16, 2 fp32. Eight codes a lane.
@@ -118,14 +117,14 @@ __global__ void __launch_bounds__(kThreads) mx_repack_codes_kernel(const uint8_t
 }
 
 __global__ void __launch_bounds__(kThreads) mx_repack_scale_kernel(const uint8_t* __restrict__ scale, int64_t n, int64_t blocks,
-                                                                   int64_t kgroups, int64_t total, uint32_t* __restrict__ out) {
+                                                                   int64_t ktiles, int64_t total, uint32_t* __restrict__ out) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
     if (i >= total) return;
     const int lane = static_cast<int>(i & 63);
-    const int64_t group = i >> 6, row = group / kgroups * 16 + (lane & 15), block0 = group % kgroups * 16 + (lane >> 4);
+    const int64_t tile = i >> 6, row0 = tile / ktiles * 64 + (lane & 15), block = tile % ktiles * 4 + (lane >> 4);
     uint32_t v = 0;
     for (int t = 0; t < 4; ++t) {
-        const int64_t block = block0 + 4 * t;
+        const int64_t row = row0 + 16 * t;
         if (row < n && block < blocks) v |= static_cast<uint32_t>(scale[row * blocks + block]) << (8 * t);
     }
     out[i] = v;
@@ -146,11 +145,11 @@ int check_blocks(const char* op, int64_t m, int64_t k) {
 
 void launch_mx_quantize_tiles(const void* x, bool bf16, int64_t m, int64_t k, uint8_t* codes, uint32_t* scale, hipStream_t s) {
     const mx_dims d = make_mx_dims(m, k);
-    const unsigned grid = static_cast<unsigned>(d.strips * d.kgroups);
+    const unsigned grid = static_cast<unsigned>(d.groups * d.ktiles);
     const auto* xp = static_cast<const uint16_t*>(x);
-    const int kt = static_cast<int>(d.ktiles), kg = static_cast<int>(d.kgroups);
-    if (bf16) mx_quantize_tiles_kernel<true><<<grid, kThreads, 0, s>>>(xp, m, static_cast<int>(k), kt, kg, codes, scale);
-    else mx_quantize_tiles_kernel<false><<<grid, kThreads, 0, s>>>(xp, m, static_cast<int>(k), kt, kg, codes, scale);
+    const int kt = static_cast<int>(d.ktiles);
+    if (bf16) mx_quantize_tiles_kernel<true><<<grid, kThreads, 0, s>>>(xp, m, static_cast<int>(k), kt, d.strips, codes, scale);
+    else mx_quantize_tiles_kernel<false><<<grid, kThreads, 0, s>>>(xp, m, static_cast<int>(k), kt, d.strips, codes, scale);
 }
 
 }  // namespace plm
@@ -218,10 +217,10 @@ int plm_repack_mxfp4(const uint8_t* codes, const uint8_t* scale, int64_t n, int6
     PLM_CHECK_ARG(aligned(scale_out, 4), op, "scale_out must be 4-byte aligned");
     const mx_dims d = make_mx_dims(n, k);
     hipStream_t s = as_stream(stream);
-    const int64_t total = d.strips * d.ktiles * 64, words = d.strips * d.kgroups * 64;
+    const int64_t total = d.strips * d.ktiles * 64, words = d.groups * d.ktiles * 64;
     mx_repack_codes_kernel<<<static_cast<unsigned>(ceil_div(total, kThreads)), kThreads, 0, s>>>(codes, n, k, d.ktiles, total,
                                                                                                static_cast<u32x4_t*>(weight_out));
-    mx_repack_scale_kernel<<<static_cast<unsigned>(ceil_div(words, kThreads)), kThreads, 0, s>>>(scale, n, k / kMxBlock, d.kgroups, words,
+    mx_repack_scale_kernel<<<static_cast<unsigned>(ceil_div(words, kThreads)), kThreads, 0, s>>>(scale, n, k / kMxBlock, d.ktiles, words,
                                                                                               static_cast<uint32_t*>(scale_out));
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;

@@ -27,22 +27,22 @@ struct rows_args {
     const uint16_t* x;
     mx_matrix xq, w0, w1;
     mx_output out;
-    int m, k, ktiles, kgroups, strips, m_blocks;
+    int m, k, ktiles, strips, m_blocks;
 };
 
-constexpr int rows_waves(int xm, int rb) { return xm == kXRing && rb > 2 ? 4 : 8; }
+constexpr int kWaves = 8;
 constexpr int rows_ahead(int sg) { return sg <= 2 ? 4 : 2; }
 
 template <int XM, bool BF16, int RB, int SG, mx_epilogue EPI>
-__global__ void __launch_bounds__(rows_waves(XM, RB) * 64) mx_rows_kernel(rows_args a) {
-    constexpr int NW = rows_waves(XM, RB);
+__global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
+    constexpr int NW = kWaves;
     constexpr int DW = rows_ahead(SG);
     constexpr bool STAGED = XM == kXStaged || XM == kXStagedQuantize;
     constexpr int P = EPI == kMxPlain ? SG : SG / 2;                 // strips of one matrix
     constexpr int SLOT = RB * 4096;                                  // ring: a K tile of x
     constexpr int XL = RB * 4;                                       // its loads of 1 KiB
     constexpr int WL = 2 * SG;                                       // loads of a K tile's weights and scales
-    static_assert(!STAGED || RB == 1, "staged x is one row block");
+    static_assert(RB == 1 || (!STAGED && (XM == kXCodes || RB == 2)), "staged x is one row block, the ring holds two");
     extern __shared__ __attribute__((aligned(1024))) uint8_t mx_lds[];
 
     const int lane = threadIdx.x & 63;
@@ -52,22 +52,21 @@ __global__ void __launch_bounds__(rows_waves(XM, RB) * 64) mx_rows_kernel(rows_a
     const int rows = min(RB * 16, a.m - row0);
     const int mine = min(P, a.strips - strip0);  // strips past N read zeros
 
-    const int64_t w_at = static_cast<int64_t>(strip0) * a.ktiles * kSubTileBytes, s_at = static_cast<int64_t>(strip0) * a.kgroups * 64;
-    const uint32_t w_bytes = static_cast<uint32_t>(mine) * a.ktiles * kSubTileBytes, s_bytes = static_cast<uint32_t>(mine) * a.kgroups * 256;
+    const int64_t w_at = static_cast<int64_t>(strip0) * a.ktiles * kSubTileBytes, s_at = static_cast<int64_t>(strip0 >> 2) * a.ktiles * 64;
+    const uint32_t w_bytes = static_cast<uint32_t>(mine) * a.ktiles * kSubTileBytes, s_bytes = static_cast<uint32_t>(a.ktiles) * 256;
     __amdgpu_buffer_rsrc_t wr[2] = {make_rsrc(a.w0.codes + w_at, w_bytes), make_rsrc(a.w0.codes + w_at, w_bytes)};
     __amdgpu_buffer_rsrc_t sr[2] = {make_rsrc(a.w0.scale + s_at, s_bytes), make_rsrc(a.w0.scale + s_at, s_bytes)};
     if constexpr (EPI != kMxPlain) {
         wr[1] = make_rsrc(a.w1.codes + w_at, w_bytes);
         sr[1] = make_rsrc(a.w1.scale + s_at, s_bytes);
     }
-    const int x_pitch = STAGED ? a.kgroups * 1024 : 0;
+    const int x_pitch = STAGED ? (a.ktiles + 3) / 4 * 1024 : 0;
     const __amdgpu_buffer_rsrc_t xr =
         XM == kXCodes ? make_rsrc(a.xq.codes + static_cast<int64_t>(row0 / 16) * a.ktiles * kSubTileBytes,
                                   static_cast<uint32_t>((rows + 15) / 16) * a.ktiles * kSubTileBytes)
                       : make_rsrc(a.x + static_cast<int64_t>(row0) * a.k, static_cast<uint32_t>(rows) * a.k * 2);
     const __amdgpu_buffer_rsrc_t xsr =
-        XM == kXCodes ? make_rsrc(a.xq.scale + static_cast<int64_t>(row0 / 16) * a.kgroups * 64,
-                                  static_cast<uint32_t>((rows + 15) / 16) * a.kgroups * 256)
+        XM == kXCodes ? make_rsrc(a.xq.scale + static_cast<int64_t>(row0 / 64) * a.ktiles * 64, static_cast<uint32_t>(a.ktiles) * 256)
                       : xr;
 
     struct batch {
@@ -76,18 +75,18 @@ __global__ void __launch_bounds__(rows_waves(XM, RB) * 64) mx_rows_kernel(rows_a
     };
     auto load = [&](batch& b, int kt) {
         const bool in = kt < a.ktiles;
-        const int past = in ? 0 : kOOB, w_off = in ? kt * kSubTileBytes : 0, s_off = in ? (kt >> 2) * 256 + (kt & 3) : 0;
+        const int past = in ? 0 : kOOB, w_off = in ? kt * kSubTileBytes : 0, s_off = in ? kt * 256 : 0;
 #pragma unroll
         for (int j = 0; j < SG; ++j) {
             const int side = j / P, jj = j % P;
             b.w[j] = buffer_load16_stream(wr[side], (jj * a.ktiles * kSubTileBytes + lane * 16) | past, w_off);
-            b.s[j] = __builtin_amdgcn_raw_buffer_load_b8(sr[side], (jj * a.kgroups * 256 + lane * 4) | past, s_off, 0);
+            b.s[j] = __builtin_amdgcn_raw_buffer_load_b8(sr[side], (lane * 4 + ((strip0 + jj) & 3)) | past, s_off, 0);
         }
         if constexpr (XM == kXCodes) {
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
                 b.x[i] = buffer_load16(xr, (i * a.ktiles * kSubTileBytes + lane * 16) | past, w_off);
-                b.xs[i] = __builtin_amdgcn_raw_buffer_load_b8(xsr, (i * a.kgroups * 256 + lane * 4) | past, s_off, 0);
+                b.xs[i] = __builtin_amdgcn_raw_buffer_load_b8(xsr, (lane * 4 + ((row0 / 16 + i) & 3)) | past, s_off, 0);
             }
         }
     };
@@ -166,18 +165,18 @@ __global__ void __launch_bounds__(rows_waves(XM, RB) * 64) mx_rows_kernel(rows_a
     };
 
     batch b[DW];
-#pragma unroll
-    for (int d = 0; d < DW - 1; ++d) load(b[d], wave + d * NW);
     if constexpr (STAGED) {
         // Row r's K group q (512 values, 1 KiB), swizzled within each K tile.
-        for (int i = wave; i < rows * a.kgroups; i += NW) {
-            const int r = i / a.kgroups, q = i % a.kgroups;
+        const int groups = x_pitch / 1024;
+        for (int i = wave; i < rows * groups; i += NW) {
+            const int r = i / groups, q = i % groups;
             const int c = (lane & 48) | ((lane & 15) ^ (r & 15)), at = q * 512 + c * 8;
             buffer_load_lds16(xr, mx_lds + i * 1024, at < a.k ? (r * a.k + at) * 2 : kOOB, 0);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
     }
+#pragma unroll
+    for (int d = 0; d < DW - 1; ++d) load(b[d], wave + d * NW);
+    if constexpr (STAGED) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((DW - 1) * WL) : "memory");  // x, not the weights
     load_x(wave, 0);
     for (int kt = wave; kt < a.ktiles; kt += DW * NW) {
 #pragma unroll
@@ -227,7 +226,10 @@ __global__ void __launch_bounds__(rows_waves(XM, RB) * 64) mx_rows_kernel(rows_a
                 if (r < rows) mx_store_plain<BF16>(a.out, row0 + r, col, v);
             } else {
                 const f32x4_t up = total(i, P + p, ln);
-                if (r < rows) mx_store_gated<BF16>(a.out, row0 + r, col, v, up);
+                if (r < rows) {
+                    mx_store_plain<BF16>(a.out, row0 + r, col, mx_gated4(v, up));
+                    mx_store_gate_up(a.out, row0 + r, col, v, up);
+                }
             }
         }
     }
@@ -244,12 +246,11 @@ template <int XM, bool BF16, int RB, int SG, mx_epilogue EPI> void launch(const 
     a.m = static_cast<int>(p.m);
     a.k = static_cast<int>(p.k);
     a.ktiles = static_cast<int>(d.ktiles);
-    a.kgroups = static_cast<int>(d.kgroups);
     a.strips = static_cast<int>(d.strips);
     a.m_blocks = static_cast<int>(ceil_div(p.m, RB * 16));
-    constexpr int NW = rows_waves(XM, RB);
+    constexpr int NW = kWaves;
     int64_t loop = 0;
-    if (XM == kXStaged || XM == kXStagedQuantize) loop = p.m * d.kgroups * 1024;
+    if (XM == kXStaged || XM == kXStagedQuantize) loop = p.m * ceil_div(d.ktiles, 4) * 1024;
     if (XM == kXRing) loop = int64_t{NW} * 2 * RB * 4096;
     const int64_t lds = std::max<int64_t>(loop, int64_t{RB} * SG * NW * 1024);
     constexpr int P = EPI == kMxPlain ? SG : SG / 2;
@@ -257,14 +258,23 @@ template <int XM, bool BF16, int RB, int SG, mx_epilogue EPI> void launch(const 
     mx_rows_kernel<XM, BF16, RB, SG, EPI><<<static_cast<unsigned>(grid), NW * 64, static_cast<size_t>(lds), s>>>(a);
 }
 
+// Strips of a matrix in a workgroup: as few as fill the GPU in one round, since more leave fewer workgroups to
+// draw on the memory, and fewer bring x once more each. One / two / four, us at M = 1 and 16: N 2048, K 2048
+// 3.3 / 4.0 / 4.6 and 4.2 / 4.8 / 5.7; N 4096, K 12288 8.2 / 8.8 / 14.1 and 11.7 / 13.6 / 17.2; N 6144, K 4096
+// 5.9 / 5.6 / 6.8 and 8.7 / 6.8 / 7.8; N 24576, K 4096 13.9 / 13.1 / 12.8 and 20.9 / 16.2 / 15.0.
 template <int XM, bool BF16, int RB> void launch_sg(const mx_product& p, hipStream_t s) {
+    const int64_t strips = ceil_div(p.n, kTileN), cus = cu_count();
+    if (p.epilogue == kMxPlain) {
+        if (strips <= cus) launch<XM, BF16, RB, 1, kMxPlain>(p, s);
+        else if (strips <= 2 * cus) launch<XM, BF16, RB, 2, kMxPlain>(p, s);
+        else launch<XM, BF16, RB, 4, kMxPlain>(p, s);
+    }
     if constexpr (XM == kXCodes || XM == kXStagedQuantize) {
-        if (p.epilogue == kMxGatedCodes) return launch<XM, BF16, RB, 4, kMxGatedCodes>(p, s);
+        if (p.epilogue == kMxGatedCodes) launch<XM, BF16, RB, 4, kMxGatedCodes>(p, s);  // a block is two strips of either
+    } else if (p.epilogue == kMxGated) {
+        if (strips <= cus) launch<XM, BF16, RB, 2, kMxGated>(p, s);
+        else launch<XM, BF16, RB, 4, kMxGated>(p, s);
     }
-    if constexpr (XM == kXStaged || XM == kXRing) {
-        if (p.epilogue == kMxGated) return launch<XM, BF16, RB, 2, kMxGated>(p, s);
-    }
-    launch<XM, BF16, RB, 1, kMxPlain>(p, s);
 }
 
 bool staged(const mx_product& p) { return p.m <= 16 && p.m * ceil_div(p.k, 512) * 1024 <= kStagedBytes; }
@@ -277,14 +287,25 @@ template <bool BF16> void launch_typed(const mx_product& p, bool quantize_x, hip
         else launch_sg<kXCodes, BF16, 4>(p, s);
     } else if (staged(p)) launch_sg<kXStaged, BF16, 1>(p, s);
     else if (p.m <= 16) launch_sg<kXRing, BF16, 1>(p, s);
-    else if (p.m <= 32) launch_sg<kXRing, BF16, 2>(p, s);
-    else launch_sg<kXRing, BF16, 4>(p, s);
+    else launch_sg<kXRing, BF16, 2>(p, s);
 }
 
 }  // namespace
 
+// Rows kernel or tiles, us. 16-bit x, M = 32: N 2048, K 2048 4.8 against 6.1; N 6144, K 4096 8.7, 10.3; N 4096, K 12288
+// 16.3, 21.9; but N 24576, K 4096 20.1, 18.0. M = 48 (four row blocks): 6.5 against 6.1; 12, 10.0; 26.7, 21.2. With
+// x as codes, M = 32: 7.1, 7.6; 9.8, 10.7; 14.7, 19.0; 18.1, 16.2 (M = 16 16.5, 15.1); M = 64: 8.9, 8.3; 12.3, 11.7;
+// but K 12288 18.6, 21.5.
 bool launch_mx_rows(const mx_product& p, bool quantize_x, hipStream_t s) {
-    if (p.m > 64 || (quantize_x && !staged(p))) return false;
+    const int64_t strips = ceil_div(p.n, kTileN) * (p.epilogue == kMxPlain ? 1 : 2), cus = cu_count();
+    const bool codes = p.xq.codes != nullptr;
+    if (quantize_x) {
+        if (!staged(p)) return false;
+    } else if (strips > 4 * cus) {
+        if (p.m > (codes ? 8 : 16)) return false;
+    } else if (p.m > (codes && p.k >= 8192 && strips <= 2 * cus ? 64 : 32)) {
+        return false;
+    }
     if (p.bf16) launch_typed<true>(p, quantize_x, s);
     else launch_typed<false>(p, quantize_x, s);
     return true;

@@ -18,6 +18,7 @@
 #pragma once
 
 #include <type_traits>
+#include <utility>
 
 #include "mxfp4.hpp"
 
@@ -29,25 +30,42 @@ struct tile_args {
     const uint16_t* x;
     mx_matrix xq, w0, w1;
     mx_output out;
-    int m, k, ktiles, kgroups, strips;
+    int m, k, ktiles, strips;
     int m_blocks, n_blocks, band;  // band: row blocks of an XCD's patch of work tiles
 };
 
-template <bool A4, bool BF16, mx_epilogue EPI, int WM, int WN, int MT, int NS, int S>
-__global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(tile_args a) {
+// f(integral_constant<int, 0>) .. f(integral_constant<int, N - 1>): the byte of a scale register that a matrix
+// instruction uses is part of the instruction.
+template <typename F, int... I> __device__ __forceinline__ void unrolled_(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F> __device__ __forceinline__ void unrolled(F f) {
+    unrolled_(f, std::make_integer_sequence<int, N>{});
+}
+
+// SL: the scales go through the stages, too; else (W4A16 only) to registers, a K tile ahead.
+// KG: groups of WM x WN wavefronts that take the K tiles in turn, each with stages of its own; their sums meet in LDS.
+template <bool A4, bool BF16, mx_epilogue EPI, int WM, int WN, int MT, int NS, int S, int KG, bool SL>
+__global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a) {
     constexpr int NW = WM * WN;
     constexpr int BM = WM * MT * 16, BS = WN * NS;
     constexpr int XC = A4 ? WM * MT : WM * MT * 4;  // 1 KiB chunks of x in a stage
-    constexpr int STAGE = (XC + BS) * 1024;
-    constexpr int LOADS = (XC + BS) / NW;
+    // Scale chunks of 256 bytes (4 strips each): x's, then the weights' (gate's, then up's).
+    constexpr int SIDES = EPI == kMxPlain ? 1 : 2;
+    constexpr int XG = A4 ? (WM * MT + 3) / 4 : 0, WG = (BS / SIDES + 3) / 4, SCC = XG + SIDES * WG;
+    constexpr int SCL = SL ? (SCC + NW - 1) / NW : 0;
+    constexpr int STAGE = (XC + BS) * 1024 + (SL ? SCC * 256 : 0);
+    constexpr int LOADS = (XC + BS) / NW + SCL;
     constexpr int SLICES = A4 ? 1 : 4;
+    static_assert((MT & (MT - 1)) == 0 && (NS & (NS - 1)) == 0 && (!A4 || WM % 2 == 0), "a wavefront's strips lie in whole groups, or in one");
     static_assert(XC % NW == 0 && BS % NW == 0, "every wavefront loads as many chunks");
     static_assert(EPI == kMxPlain || NS % 2 == 0, "gate and up in one wavefront");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[S * STAGE];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S * KG * STAGE];
 
     const int lane = threadIdx.x & 63;
-    const int wave = uniform(threadIdx.x >> 6);
+    const int group = KG == 1 ? 0 : uniform(threadIdx.x >> 6) / NW, wave = uniform(threadIdx.x >> 6) % NW;
     const int wm = wave / WN, wn = wave % WN;
+    uint8_t* stages = lds + group * STAGE;  // slot s at s KG STAGE
     const int col16 = lane & 15, kq = lane >> 4;
 
     // Workgroups go round the 8 XCDs by id: each takes one run of the work tiles, which are ordered in
@@ -60,11 +78,11 @@ __global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(tile_args a) {
     const int rows = min(BM, a.m - row0);
 
     // Local strip s: strip nb BS + s, or slice nb BS / 2 + s / 2 of the gate (s even) or up weight.
-    constexpr int SIDES = EPI == kMxPlain ? 1 : 2;
     const int strip0 = nb * (BS / SIDES);
     const int mine = min(BS / SIDES, a.strips - strip0);
-    const int64_t w_at = static_cast<int64_t>(strip0) * a.ktiles * kSubTileBytes, s_at = static_cast<int64_t>(strip0) * a.kgroups * 64;
-    const uint32_t w_bytes = static_cast<uint32_t>(mine) * a.ktiles * kSubTileBytes, s_bytes = static_cast<uint32_t>(mine) * a.kgroups * 256;
+    const int64_t w_at = static_cast<int64_t>(strip0) * a.ktiles * kSubTileBytes, s_at = static_cast<int64_t>(strip0 >> 2) * a.ktiles * 64;
+    const uint32_t w_bytes = static_cast<uint32_t>(mine) * a.ktiles * kSubTileBytes;
+    const uint32_t s_bytes = static_cast<uint32_t>(((strip0 & 3) + mine + 3) / 4) * a.ktiles * 256;
     __amdgpu_buffer_rsrc_t wr[2], sr[2];
     wr[0] = make_rsrc(a.w0.codes + w_at, w_bytes);
     sr[0] = make_rsrc(a.w0.scale + s_at, s_bytes);
@@ -75,20 +93,35 @@ __global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(tile_args a) {
         A4 ? make_rsrc(a.xq.codes + static_cast<int64_t>(row0 / 16) * a.ktiles * kSubTileBytes, static_cast<uint32_t>(x_strips) * a.ktiles * kSubTileBytes)
            : make_rsrc(a.x + static_cast<int64_t>(row0) * a.k, static_cast<uint32_t>(rows) * a.k * 2);
     const __amdgpu_buffer_rsrc_t xsr =
-        make_rsrc(a.xq.scale + static_cast<int64_t>(row0 / 16) * a.kgroups * 64, A4 ? static_cast<uint32_t>(x_strips) * a.kgroups * 256 : 0u);
+        make_rsrc(a.xq.scale + static_cast<int64_t>(row0 / 64) * a.ktiles * 64, A4 ? static_cast<uint32_t>((row0 % 64 / 16 + x_strips + 3) / 4) * a.ktiles * 256 : 0u);
 
-    // Chunk c of a stage: x's first (codes: strip c; 16-bit: rows 4 c .. 4 c + 3, their 16-byte columns
-    // XOR-swizzled by row), then the weight strips'. Past the end of either, zeros.
-    auto issue = [&](int kt, int slot) {
+    // The scale chunks that this wavefront loads (the last one again where there are fewer): chunk, its group
+    // of strips and buffer.
+    int scc[SCL + 1], scg[SCL + 1];
+    __amdgpu_buffer_rsrc_t scr[SCL + 1];
+#pragma unroll
+    for (int i = 0; i < SCL; ++i) {
+        const int c = min(wave * SCL + i, SCC - 1), w = c - XG;
+        scc[i] = c;
+        scg[i] = c < XG ? c : w % WG;
+        scr[i] = c < XG ? xsr : (w < WG ? sr[0] : sr[1]);
+    }
+
+    // Load l of the wavefront's LOADS for K tile kt. Chunk c of a stage: x's first (codes: strip c; 16-bit: rows
+    // 4 c .. 4 c + 3, their 16-byte columns XOR-swizzled by row), then the weight strips', then the scales'. Past
+    // the end of any, zeros.
+    constexpr int XL = XC / NW, WL = BS / NW;
+    auto issue_one = [&](int l, int turn, int slot) {
+        const int kt = turn * KG + group;
         const bool in = kt < a.ktiles;
         const int past = in ? 0 : kOOB, off = in ? kt : 0;
-        uint8_t* base = lds + slot * STAGE;
-        // W4A16: an opaque copy of the lane id, so that the offsets are worked out here and not kept in registers.
+        uint8_t* base = stages + slot * (KG * STAGE);
+        // The large W4A16 tile: an opaque copy of the lane id, so that the offsets are worked out here and not kept in
+        // registers, of which it has none to spare.
         int lane = threadIdx.x & 63;
-        if constexpr (!A4) asm volatile("" : "+v"(lane));
-#pragma unroll
-        for (int i = 0; i < XC / NW; ++i) {
-            const int c = wave * (XC / NW) + i;
+        if constexpr (!A4 && MT * NS >= 32) asm volatile("" : "+v"(lane));
+        if (l < XL) {
+            const int c = wave * XL + l;
             if constexpr (A4) {
                 buffer_load_lds16(xr, base + c * 1024, (c * a.ktiles * kSubTileBytes + lane * 16) | past, off * kSubTileBytes);
             } else {
@@ -96,50 +129,75 @@ __global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(tile_args a) {
                 const int at = kt * kTileK + col * 8 < a.k ? r * a.k * 2 + col * 16 : kOOB;
                 buffer_load_lds16(xr, base + c * 1024, at, off * 256);
             }
-        }
-#pragma unroll
-        for (int i = 0; i < BS / NW; ++i) {
-            const int c = wave * (BS / NW) + i, side = SIDES == 2 ? c & 1 : 0, strip = SIDES == 2 ? c >> 1 : c;
-            buffer_load_lds16(wr[side], base + (XC + c) * 1024, (strip * a.ktiles * kSubTileBytes + lane * 16) | past,
-                              off * kSubTileBytes);
+        } else if (l < XL + WL) {
+            const int c = wave * WL + l - XL, side = SIDES == 2 ? c & 1 : 0, strip = SIDES == 2 ? c >> 1 : c;
+            buffer_load_lds16(wr[side], base + (XC + c) * 1024, (strip * a.ktiles * kSubTileBytes + lane * 16) | past, off * kSubTileBytes);
+        } else {
+            const int i = l - XL - WL;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(scr[i], (__attribute__((address_space(3))) void*)(base + (XC + BS) * 1024 + scc[i] * 256), 4,
+                                                     (scg[i] * a.ktiles * 256 + lane * 4) | past, off * 256, 0, 0);
         }
     };
+    // The loads of a K tile stand among the matrix instructions, at places 0 .. SPREAD - 1 (one row of them
+    // each): requested all at once, a wavefront waits for the memory pipeline to take them (16 cycles each,
+    // one pipeline a CU) with its matrix unit idle.
+    auto issue_at = [&](int place, auto spread, int kt, int slot) {
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l)
+            if (l * decltype(spread)::value / LOADS == place) issue_one(l, kt, slot);
+    };
+    auto issue = [&](int kt, int slot) {
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l) issue_one(l, kt, slot);
+    };
 
-    // Scale dwords of a group of 4 K tiles.
+    const int x_at = row0 / 16 & 3, g_at = strip0 & 3;  // where the workgroup's first strips lie in their groups
+    // A lane's scale dwords of a K tile: the bytes of four strips each, shifted to start at the wavefront's own.
+    constexpr int XN = A4 ? (MT + 3) / 4 : 0, PN = NS / SIDES, WN4 = (PN + 3) / 4;
     struct scales {
-        uint32_t w[NS], x[A4 ? MT : 1];
+        uint32_t x[A4 ? XN : 1], w[SIDES][WN4];
     };
-    auto load_scales = [&](scales& s, int q) {
-        const int past = q < a.kgroups ? 0 : kOOB, off = q < a.kgroups ? q * 256 : 0;
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            const int sl = wn * NS + j, side = SIDES == 2 ? sl & 1 : 0, strip = SIDES == 2 ? sl >> 1 : sl;
-            s.w[j] = buffer_load_u32(sr[side], (strip * a.kgroups * 256 + lane * 4) | past, off);
-        }
+    auto read_scales = [&](scales& s, int slot) {
+        const uint8_t* base = stages + slot * (KG * STAGE) + (XC + BS) * 1024 + lane * 4;
         if constexpr (A4) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) s.x[i] = buffer_load_u32(xsr, ((wm * MT + i) * a.kgroups * 256 + lane * 4) | past, off);
+            for (int g = 0; g < XN; ++g)
+                s.x[g] = *reinterpret_cast<const uint32_t*>(base + ((x_at + wm * MT) / 4 + g) * 256) >> (8 * ((x_at + wm * MT) & 3));
         }
+#pragma unroll
+        for (int d = 0; d < SIDES; ++d)
+#pragma unroll
+            for (int g = 0; g < WN4; ++g)
+                s.w[d][g] = *reinterpret_cast<const uint32_t*>(base + (XG + d * WG + (g_at + wn * PN) / 4 + g) * 256) >> (8 * ((g_at + wn * PN) & 3));
     };
 
-    auto shift_scales = [&](scales& to, const scales& from, int by) {
+    auto load_scales = [&](scales& s, int turn) {
+        const int kt = turn * KG + group;
+        const int past = kt < a.ktiles ? 0 : kOOB, off = kt < a.ktiles ? kt * 256 : 0;
 #pragma unroll
-        for (int j = 0; j < NS; ++j) to.w[j] = from.w[j] >> by;
-        if constexpr (A4) {
+        for (int d = 0; d < SIDES; ++d)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) to.x[i] = from.x[i] >> by;
-        }
+            for (int g = 0; g < WN4; ++g)
+                s.w[d][g] = buffer_load_u32(sr[d], (((g_at + wn * PN) / 4 + g) * a.ktiles * 256 + lane * 4) | past, off);
+    };
+    auto shift_scales = [&](scales& s) {
+#pragma unroll
+        for (int d = 0; d < SIDES; ++d)
+#pragma unroll
+            for (int g = 0; g < WN4; ++g) s.w[d][g] >>= 8 * ((g_at + wn * PN) & 3);
     };
 
-    // Fragments. x's are read again for the next slice right after their use, the weights' a slice ahead.
-    u32x4_t x[MT], w[2][NS];
+    // Fragments. x's are read again right after their use, XB slices ahead (XB: as many as make that some hundred
+    // cycles, the time of an LDS read); the weights' a K tile ahead.
+    constexpr int XB = A4 ? 1 : (MT * NS >= 16 ? 1 : (MT * NS >= 8 ? 2 : 4));
+    u32x4_t x[XB][MT], w[2][NS];
     auto read_x = [&](int i, int slot, int t) {
-        const uint8_t* base = lds + slot * STAGE;
-        if constexpr (A4) x[i] = *reinterpret_cast<const u32x4_t*>(base + (wm * MT + i) * 1024 + lane * 16);
-        else x[i] = *reinterpret_cast<const u32x4_t*>(base + (wm * MT * 16 + i * 16 + col16) * 256 + (((4 * kq + t) ^ col16) << 4));
+        const uint8_t* base = stages + slot * (KG * STAGE);
+        if constexpr (A4) x[0][i] = *reinterpret_cast<const u32x4_t*>(base + (wm * MT + i) * 1024 + lane * 16);
+        else x[t % XB][i] = *reinterpret_cast<const u32x4_t*>(base + (wm * MT * 16 + i * 16 + col16) * 256 + (((4 * kq + t) ^ col16) << 4));
     };
     auto read_w = [&](u32x4_t (&to)[NS], int j, int slot) {
-        to[j] = *reinterpret_cast<const u32x4_t*>(lds + slot * STAGE + (XC + wn * NS + j) * 1024 + lane * 16);
+        to[j] = *reinterpret_cast<const u32x4_t*>(stages + slot * (KG * STAGE) + (XC + wn * NS + j) * 1024 + lane * 16);
     };
 
     f32x4_t acc[MT][NS];
@@ -148,96 +206,135 @@ __global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(tile_args a) {
 #pragma unroll
         for (int j = 0; j < NS; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-    scales sc, scn;
+    // W4A16: K tile kt's barrier stands before slice BAR, past which no wavefront reads its stage; the loads of
+    // K tile kt + S into it are spread over the slices from there on into the next K tile.
+    // It stands after the first BP rows of matrix instructions of a K tile (W4A4) or of slice BAR: the last reads
+    // before it, which it has to wait for, have landed by then.
+    constexpr int BAR = SLICES - XB, BP = A4 && MT * NS >= 64 ? 1 : 0;
+    constexpr int SPREAD = A4 ? MT - BP : std::min(SLICES * MT, (XB + 1) * MT - BP);
+    using spread_t = std::integral_constant<int, SPREAD>;
 #pragma unroll
-    for (int p = 0; p < S; ++p) {
-        if (p == S - 2) load_scales(sc, 0);  // where a turn before the first would have asked for them (see the counts below)
-        issue(p, p);
-    }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * LOADS) : "memory");
-
+    for (int p = 0; p < S - 1; ++p) issue(p, p);
+    // Of K tile S - 1 the loads that the first K tile's slices before BAR do not make.
 #pragma unroll
-    for (int i = 0; i < MT; ++i) read_x(i, 0, 0);
+    for (int place = 0; place < (A4 ? SPREAD : XB * MT - BP); ++place) issue_at(place, spread_t{}, S - 1, S - 1);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 2) * LOADS) : "memory");
+#pragma unroll
+    for (int t = 0; t < XB; ++t)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) read_x(i, 0, t);
 #pragma unroll
     for (int j = 0; j < NS; ++j) read_w(w[0], j, 0);
+    scales sc[2];
+    if constexpr (SL) {
+        read_scales(sc[0], 0);
+    } else {
+        load_scales(sc[0], 0);
+        shift_scales(sc[0]);
+    }
     int slot = 0;
+    const int turns = (a.ktiles + KG - 1) / KG;  // past the last K tile one of zeros
+    // K tile kt + 1 has landed when only the loads of S - 2 K tiles after it are left.
+    constexpr int LEFT = (S - 2) * LOADS;
+    static_assert(LEFT <= 63 && (SL || S == 2), "the counter's range; loads to registers are not counted");
     if constexpr (A4) {
-        // Loads after those of K tile kt + 1, which has to have landed: S - 2 K tiles' and the scales of the
-        // turns begun since.
-        constexpr int SC = NS + MT;
-        auto step = [&](int kt, const u32x4_t (&cur)[NS], u32x4_t (&next)[NS], auto older) {
+        auto step = [&](int kt, const u32x4_t (&cur)[NS], u32x4_t (&next)[NS], const scales& s, scales& s_next) {
             const int ns = slot + 1 == S ? 0 : slot + 1;
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(older)::value) : "memory");
-            issue(kt + S, slot);
+            unrolled<MT>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                if constexpr (i == BP) {
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+                    read_scales(s_next, ns);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
+                    for (int e = 0; e < BP; ++e) read_x(e, ns, 0);
+                }
+                if constexpr (i >= BP) {
+                    issue_at(i - BP, spread_t{}, kt + S, slot);
 #pragma unroll
-                for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(next, j, ns);
-#pragma unroll
-                for (int j = 0; j < NS; ++j) acc[i][j] = mx_mfma<0, 0>(cur[j], sc.w[j], x[i], sc.x[i], acc[i][j]);
-                read_x(i, ns, 0);
-                __builtin_amdgcn_sched_barrier(0);  // the reads stay among the matrix instructions, a K tile ahead
-            }
+                    for (int j = (i - BP) * NS / (MT - BP); j < (i + 1 - BP) * NS / (MT - BP); ++j) read_w(next, j, ns);
+                }
+                unrolled<NS>([&](auto jc) {
+                    constexpr int j = decltype(jc)::value, p = j / SIDES;
+                    acc[i][j] = mx_mfma<p & 3, i & 3>(cur[j], s.w[j % SIDES][p / 4], x[0][i], s.x[i / 4], acc[i][j]);
+                });
+                if constexpr (i >= BP) read_x(i, ns, 0);
+                __builtin_amdgcn_sched_barrier(0);  // reads and loads stay where they are
+            });
             slot = ns;
         };
-        // Two K tiles a turn; past an odd number of them one of zeros, whose scale bytes are zeros, too. No
-        // branch in a turn: the compiler would sink the matrix instructions past it, and past the reads.
-        for (int kt = 0; kt < a.ktiles; kt += 2) {
-            load_scales(scn, (kt + 2) >> 2);
-            step(kt, w[0], w[1], std::integral_constant<int, (S - 2) * LOADS + S / 2 * SC>{});
-            shift_scales(sc, sc, 8);
-            step(kt + 1, w[1], w[0], std::integral_constant<int, (S - 2) * LOADS + (S - 1) / 2 * SC>{});
-            shift_scales(sc, scn, (kt & 2) ? 0 : 16);
+        // Two K tiles a turn; past an odd number of them one of zeros. No branch in a turn: the compiler would
+        // sink the matrix instructions past it, and past the reads.
+        for (int kt = 0; kt < turns; kt += 2) {
+            step(kt, w[0], w[1], sc[0], sc[1]);
+            step(kt + 1, w[1], w[0], sc[1], sc[0]);
         }
     } else {
-        for (int kt = 0; kt < a.ktiles; ++kt) {
-            load_scales(scn, (kt + 1) >> 2);
+        int load_kt = S - 1, load_slot = S - 1;
+        for (int kt = 0; kt < turns; ++kt) {
             const int ns = slot + 1 == S ? 0 : slot + 1;
+            if constexpr (!SL) load_scales(sc[1], kt + 1);
             float s[NS];
 #pragma unroll
-            for (int j = 0; j < NS; ++j) s[j] = mx_scale(sc.w[j] & 0xffu);
+            for (int j = 0; j < NS; ++j) s[j] = mx_scale(sc[0].w[j % SIDES][j / SIDES / 4] >> (8 * (j / SIDES & 3)) & 0xffu);
 #pragma unroll
             for (int t = 0; t < SLICES; ++t) {
-                if (t == SLICES - 1) {
-                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * LOADS) : "memory");
-                    issue(kt + S, slot);
-                }
                 u32x4_t wf[NS];
 #pragma unroll
                 for (int j = 0; j < NS; ++j) wf[j] = mx_decode<BF16>(w[0][j][t], s[j]);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    if (t == SLICES - 1)
+                    if (t == BAR && i == BP) {
+                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+                        load_kt = kt + S;
+                        load_slot = slot;
+                        if constexpr (SL) read_scales(sc[1], ns);
 #pragma unroll
-                        for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(w[1], j, ns);
+                        for (int e = 0; e < BP; ++e) read_x(e, ns, (t + XB) % SLICES);
+                    }
+                    issue_at(((t - BAR + SLICES) * MT + i - BP) % (SLICES * MT), spread_t{}, load_kt, load_slot);
+                    if (t == SLICES - 1 && i >= BP)
 #pragma unroll
-                    for (int j = 0; j < NS; ++j) acc[i][j] = mfma16x16x32<BF16>(wf[j], x[i], acc[i][j]);
-                    read_x(i, t == SLICES - 1 ? ns : slot, (t + 1) & 3);
-                    __builtin_amdgcn_sched_barrier(0);  // the reads stay among the matrix instructions, a slice ahead
+                        for (int j = (i - BP) * NS / (MT - BP); j < (i + 1 - BP) * NS / (MT - BP); ++j) read_w(w[1], j, ns);
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) acc[i][j] = mfma16x16x32<BF16>(wf[j], x[t % XB][i], acc[i][j]);
+                    if (t != BAR || i >= BP) read_x(i, t >= BAR ? ns : slot, (t + XB) % SLICES);
+                    __builtin_amdgcn_sched_barrier(0);  // reads and loads stay where they are
                 }
             }
 #pragma unroll
             for (int j = 0; j < NS; ++j) w[0][j] = w[1][j];
-            shift_scales(sc, scn, 8 * ((kt + 1) & 3));
+            if constexpr (!SL) shift_scales(sc[1]);
+            sc[0] = sc[1];
             slot = ns;
         }
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // requests past the last K tile
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // requests past the last K tile; LDS is free
 
+    if constexpr (KG > 1) {
+        // In group order, so that the result does not depend on which is done first.
+        static_assert((KG - 1) * NW * MT * NS * 1024 <= S * KG * STAGE, "the sums fit");
+        f32x4_t* sums = reinterpret_cast<f32x4_t*>(lds);
+        if (group > 0)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int r = (wm * MT + i) * 16 + col16;
-        const int64_t row = row0 + r;
-        if constexpr (EPI == kMxPlain) {
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NS; ++j)
-                if (r < rows) mx_store_plain<BF16>(a.out, row, (strip0 + wn * NS + j) * kTileN + 4 * kq, acc[i][j]);
-        } else if constexpr (EPI == kMxGated) {
+                for (int j = 0; j < NS; ++j) sums[(((group - 1) * NW + wave) * MT * NS + i * NS + j) * 64 + lane] = acc[i][j];
+        __syncthreads();
+        if (group == 0)
 #pragma unroll
-            for (int j = 0; j < NS; j += 2)
-                if (r < rows) mx_store_gated<BF16>(a.out, row, (strip0 + (wn * NS + j) / 2) * kTileN + 4 * kq, acc[i][j], acc[i][j + 1]);
-        } else {
-            static_assert(EPI != kMxGatedCodes || NS % 4 == 0, "whole blocks");
+            for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) acc[i][j] = acc[i][j] + sums[((g * NW + wave) * MT * NS + i * NS + j) * 64 + lane];
+        __syncthreads();
+        if (group > 0) return;
+    }
+
+    if constexpr (EPI == kMxGatedCodes) {
+        static_assert(EPI != kMxGatedCodes || NS % 4 == 0, "whole blocks");
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int j = 0; j + 3 < NS; j += 4) {
                 const f32x4_t g[2] = {acc[i][j], acc[i][j + 2]}, u[2] = {acc[i][j + 1], acc[i][j + 3]};
@@ -245,11 +342,64 @@ __global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(tile_args a) {
                 if ((wm * MT + i) * 16 < rows && block * kMxBlock < a.out.n)  // wave-uniform
                     mx_store_codes(a.out, row0 / 16 + wm * MT + i, block, g, u);
             }
+    } else {
+        // A lane has four columns of one row, a quarter of a 32-byte piece. RB row blocks at a time go through the
+        // wavefront's own part of LDS (pitch padded by 16 bytes) and leave as 16 bytes a lane, whole rows of the
+        // wavefront's tile.
+        constexpr int COLS = PN * 16, PITCH = COLS * 2 + 16, CH = COLS / 8;
+        constexpr int FIT = S * KG * STAGE / (NW * 16 * PITCH), RB = FIT >= MT ? MT : (FIT >= 4 ? 4 : 2);
+        static_assert(FIT >= 2 || MT == 1, "the rows fit");
+        uint8_t* mine_lds = lds + wave * RB * 16 * PITCH;
+        const int col0 = (strip0 + wn * PN) * kTileN;
+        auto value = [&](int i, int p) {
+            return EPI == kMxPlain ? acc[i][p] : mx_gated4(acc[i][SIDES * p], acc[i][SIDES * p + SIDES - 1]);
+        };
+        if (EPI == kMxGated && a.out.gate_up != nullptr) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int r = (wm * MT + i) * 16 + col16;
+                if (r < rows)
+#pragma unroll
+                    for (int p = 0; p < PN; ++p)
+                        mx_store_gate_up(a.out, row0 + r, col0 + p * 16 + 4 * kq, acc[i][SIDES * p], acc[i][SIDES * p + SIDES - 1]);
+            }
+        }
+        if (!a.out.lines) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int r = (wm * MT + i) * 16 + col16;
+                if (r < rows)
+#pragma unroll
+                    for (int p = 0; p < PN; ++p) mx_store_plain<BF16>(a.out, row0 + r, col0 + p * 16 + 4 * kq, value(i, p));
+            }
+            return;
+        }
+#pragma unroll
+        for (int i0 = 0; i0 < MT; i0 += RB) {
+            const int r0 = (wm * MT + i0) * 16;
+            if (r0 >= rows) break;
+#pragma unroll
+            for (int i = i0; i < i0 + RB; ++i)
+#pragma unroll
+                for (int p = 0; p < PN; ++p) {
+                    const f32x4_t v = value(i, p);
+                    *reinterpret_cast<uint2*>(mine_lds + ((i - i0) * 16 + col16) * PITCH + (p * 16 + 4 * kq) * 2) =
+                        make_uint2(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]));
+                }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int c0 = 0; c0 < RB * 16 * CH; c0 += 64) {
+                const int c = c0 + lane, r = c / CH, col = col0 + c % CH * 8;
+                if (c < RB * 16 * CH && r0 + r < rows && col < a.out.n)
+                    *reinterpret_cast<u32x4_t*>(a.out.y + (row0 + r0 + r) * static_cast<int64_t>(a.out.n) + col) =
+                        *reinterpret_cast<const u32x4_t*>(mine_lds + r * PITCH + c % CH * 16);
+            }
+            __builtin_amdgcn_wave_barrier();
         }
     }
 }
 
-template <bool A4, bool BF16, mx_epilogue EPI, int WM, int WN, int MT, int NS, int S> void launch(const mx_product& p, hipStream_t s) {
+template <bool A4, bool BF16, mx_epilogue EPI, int WM, int WN, int MT, int NS, int S, int KG = 1, bool SL = true> void launch(const mx_product& p, hipStream_t s) {
     const mx_dims d = make_mx_dims(p.n, p.k);
     tile_args a{};
     a.x = p.x16;
@@ -260,23 +410,64 @@ template <bool A4, bool BF16, mx_epilogue EPI, int WM, int WN, int MT, int NS, i
     a.m = static_cast<int>(p.m);
     a.k = static_cast<int>(p.k);
     a.ktiles = static_cast<int>(d.ktiles);
-    a.kgroups = static_cast<int>(d.kgroups);
     a.strips = static_cast<int>(d.strips);
     constexpr int BS = WN * NS / (EPI == kMxPlain ? 1 : 2);
     a.m_blocks = static_cast<int>(ceil_div(p.m, WM * MT * 16));
     a.n_blocks = static_cast<int>(ceil_div(d.strips, BS));
     a.band = 4;
-    mx_tile_kernel<A4, BF16, EPI, WM, WN, MT, NS, S><<<static_cast<unsigned>(a.m_blocks) * a.n_blocks, WM * WN * 64, 0, s>>>(a);
+    mx_tile_kernel<A4, BF16, EPI, WM, WN, MT, NS, S, KG, SL><<<static_cast<unsigned>(a.m_blocks) * a.n_blocks, WM * WN * KG * 64, 0, s>>>(a);
+}
+
+// The tile shapes, and which of them takes a call: the least of rounds x K tiles x time of a K tile. The times (us)
+// were measured with one workgroup on the GPU and with every slot taken; between the two they grow with the
+// share of slots taken, as the workgroups share the L2s and the clock. {rows, columns, workgroups a CU, lone, full}
+struct tile_cost {
+    int rows, cols, per_cu;
+    double lone, full;
+};
+constexpr tile_cost kTiles16[] = {{256, 256, 1, 2.35, 2.70}, {128, 256, 1, 1.10, 1.50}, {128, 128, 2, 1.20, 1.70}, {128, 128, 1, 0.69, 0.95},
+                                  {64, 128, 1, 0.36, 0.52},  {64, 64, 1, 0.29, 0.36},   {32, 64, 1, 0.18, 0.27},   {32, 64, 2, 0.20, 0.38}};
+constexpr tile_cost kTiles4[] = {{256, 256, 1, 0.60, 0.95}, {128, 256, 1, 0.40, 0.62}, {128, 128, 2, 0.33, 0.62},
+                                 {64, 128, 2, 0.23, 0.38},  {64, 64, 2, 0.18, 0.24}};
+
+template <int N> double tile_estimate(const tile_cost (&shapes)[N], int count, int64_t m, int64_t n, int64_t ktiles, int* best) {
+    double least = 1e300;
+    for (int i = 0; i < count; ++i) {
+        const tile_cost& c = shapes[i];
+        const int64_t tiles = ceil_div(m, c.rows) * ceil_div(n, c.cols), slots = int64_t{c.per_cu} * cu_count();
+        const double fill = std::min(1.0, static_cast<double>(tiles) / slots);
+        const double t = ceil_div(tiles, slots) * ktiles * (c.lone + (c.full - c.lone) * fill);
+        if (t < least) least = t, *best = i;
+    }
+    return least;
 }
 
 template <bool A4, bool BF16, mx_epilogue EPI> void launch_shape(const mx_product& p, hipStream_t s) {
-    const int64_t wide = ceil_div(p.m, 256) * ceil_div(p.n * (EPI == kMxPlain ? 1 : 2), 256);
+    const int64_t n = p.n * (EPI == kMxPlain ? 1 : 2), ktiles = ceil_div(p.k, kTileK);
+    int shape = 0;
+    if constexpr (A4) tile_estimate(kTiles4, EPI == kMxGatedCodes ? 4 : 5, p.m, n, ktiles, &shape);  // a block is in one wavefront: NS = 4
+    else tile_estimate(kTiles16, 8, p.m, n, ktiles, &shape);
     if constexpr (A4) {
-        if (wide >= cu_count()) launch<A4, BF16, EPI, 2, 2, 8, 8, 4>(p, s);
-        else launch<A4, BF16, EPI, 2, 2, 4, 4, 4>(p, s);
+        switch (shape) {
+            case 0: return launch<A4, BF16, EPI, 2, 4, 8, 4, 4>(p, s);
+            case 1: return launch<A4, BF16, EPI, 2, 4, 4, 4, 6>(p, s);
+            case 2: return launch<A4, BF16, EPI, 2, 2, 4, 4, 4>(p, s);
+            case 3: return launch<A4, BF16, EPI, 2, 2, 2, 4, 6>(p, s);
+            default:
+                if constexpr (EPI != kMxGatedCodes) return launch<A4, BF16, EPI, 2, 2, 2, 2, 4, 2>(p, s);
+        }
     } else {
-        if (wide >= cu_count()) launch<A4, BF16, EPI, 2, 4, 8, 4, 2>(p, s);
-        else launch<A4, BF16, EPI, 2, 2, 4, 4, 2>(p, s);
+        constexpr bool G = EPI == kMxGated;  // gate and up in one wavefront: an even number of strips
+        switch (shape) {
+            case 0: return launch<A4, BF16, EPI, 2, 4, 8, 4, 2, 1, false>(p, s);
+            case 1: return launch<A4, BF16, EPI, 1, 8, 8, 2, 3>(p, s);
+            case 2: return launch<A4, BF16, EPI, 1, 4, 8, 2, 2, 1, false>(p, s);
+            case 3: return launch<A4, BF16, EPI, 2, 4, 4, 2, 3>(p, s);
+            case 4: return launch<A4, BF16, EPI, 1, 4, 4, 2, 3, 2>(p, s);
+            case 5: return launch<A4, BF16, EPI, 2, 2, 2, 2, 3, 2>(p, s);
+            case 6: return launch<A4, BF16, EPI, 2, 2, 1, 2, 3, 4>(p, s);
+            default: return launch<A4, BF16, EPI, G ? 2 : 1, G ? 2 : 4, G ? 1 : 2, G ? 2 : 1, 3, 2>(p, s);
+        }
     }
 }
 

@@ -440,7 +440,7 @@ def dequantize_mxfp4_cuda(codes: torch.Tensor, scale: torch.Tensor, dtype=torch.
 
 def repack_mxfp4_cuda(codes: torch.Tensor, scale: torch.Tensor):
     """An MXFP4 weight [N, K] (codes uint8 [N, K/2], scale uint8 [N, K/32]) for the products: (weight int32 1-D,
-    scale int32 [strips, groups, 64]), opaque, the plm tile layout of the format."""
+    scale int32 [groups, K tiles, 64]), opaque, the plm tile layout of the format."""
     op = "repack_mxfp4"
     n, k = _mx_plain(op, codes, scale)
     weight = torch.empty((_lib.mxfp4_bytes("mxfp4_weight_bytes", n, k) // 4,), dtype=torch.int32, device=codes.device)
@@ -452,7 +452,7 @@ def repack_mxfp4_cuda(codes: torch.Tensor, scale: torch.Tensor):
 
 
 def _mx_scale_shape(n: int, k: int):
-    return -(-n // 16), -(-k // 512), 64
+    return -(-n // 64), -(-k // 128), 64
 
 
 def _mx_weight(op: str, x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, n: int, k: int) -> None:

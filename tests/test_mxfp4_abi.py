@@ -129,7 +129,7 @@ def test_sizes():
     lib = _lib.load()
     assert lib.plm_mxfp4_weight_bytes(4096, 4096) == 4096 * 4096 // 2
     assert lib.plm_mxfp4_scale_bytes(4096, 4096) == 4096 * 4096 // 32
-    assert lib.plm_mxfp4_weight_bytes(17, 160) == 2 * 2 * 1024 and lib.plm_mxfp4_scale_bytes(17, 160) == 2 * 256
+    assert lib.plm_mxfp4_weight_bytes(17, 160) == 2 * 2 * 1024 and lib.plm_mxfp4_scale_bytes(17, 160) == 2 * 256 and lib.plm_mxfp4_scale_bytes(65, 160) == 4 * 256
     assert lib.plm_mxfp4_weight_bytes(-1, 32) == -1 and lib.plm_mxfp4_scale_bytes(4, -32) == -1
     assert lib.plm_gemm_mxfp4_w4a4_workspace_bytes(0, 4, 64) == lib.plm_mlp_mxfp4_w4a4_workspace_bytes(4, 0, 64) == 0
     assert lib.plm_gemm_mxfp4_w4a4_workspace_bytes(300, 48, 1056) >= 300 * 1056 // 2 + 300 * 1056 // 32
@@ -137,7 +137,7 @@ def test_sizes():
 
 def test_python_refuses_host_tensors_and_wrong_shapes():
     x = torch.zeros(4, 64, dtype=torch.bfloat16)
-    w, s = torch.zeros(48 * 128 // 8, dtype=torch.int32), torch.zeros(3, 1, 64, dtype=torch.int32)
+    w, s = torch.zeros(48 * 128 // 8, dtype=torch.int32), torch.zeros(1, 1, 64, dtype=torch.int32)
     c, b = torch.zeros(48, 32, dtype=torch.uint8), torch.zeros(48, 2, dtype=torch.uint8)
     for op, f in (("quantize_mxfp4", lambda: ops.quantize_mxfp4_cuda(x)), ("dequantize_mxfp4", lambda: ops.dequantize_mxfp4_cuda(c, b)),
                   ("repack_mxfp4", lambda: ops.repack_mxfp4_cuda(c, b)), ("gemm_mxfp4", lambda: ops.gemm_mxfp4_cuda(x, w, s, 48)),
@@ -148,3 +148,11 @@ def test_python_refuses_host_tensors_and_wrong_shapes():
                   ("mlp_mxfp4_w4a4", lambda: ops.mlp_mxfp4_w4a4_cuda(x, (w, s), (w, s), (w, s), 48))):
         with pytest.raises(RuntimeError, match=f"^{op}: .*CUDA"):
             f()
+
+
+def test_python_and_library_agree_on_the_scales():
+    lib = _lib.load()
+    for n in (0, 1, 16, 63, 64, 65, 200, 4096):
+        for k in (0, 32, 128, 160, 544, 4128):
+            g, t, lanes = ops._mx_scale_shape(n, k)
+            assert 4 * g * t * lanes == lib.plm_mxfp4_scale_bytes(n, k)
