@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
     constexpr int XC = BM / 8, XPW = XC / NW;  // 1 KiB chunks of dy: 8 rows of 128 bytes
     constexpr int XS = BM * 128, WS = kGradStep * kGradCols * 2;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * XS + 2 * WS];
-    uint8_t* wlds = lds + 2 * XS;
+    constexpr int S0 = 2 * XS;  // W's slots
 
     const int lane = threadIdx.x & 63;
     const int wave = uniform(threadIdx.x >> 6);
@@ -60,63 +60,47 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
         u32x4_t x[XPW], c;
         uint32_t s;
     };
-    // An opaque copy of the lane id: the offsets made from it are worked out where they are used, and take no
-    // registers from the sums.
-    auto own_lane = [&] {
-        int l = lane;
-        asm volatile("" : "+v"(l));
-        return l;
-    };
+    // A load's range check covers both its offsets (checked on the GPU): past the end the wave-uniform one is kOOB,
+    // and the lanes' own never change.
+    const int x_from = static_cast<int>((lane >> 3) * a.pitch * 2) + (lane & 7) * 16;
     auto load_x = [&](step_data& b, int i, int s) {
-        const int lane = own_lane();
-        const int past = s < hi ? 0 : kOOB, off = s < hi ? s * 128 : 0;
-        const int r = 8 * (wave * XPW + i) + (lane >> 3);  // rows past the last are past the buffer's end
-        b.x[i] = buffer_load16(xr, (static_cast<int>(r * a.pitch * 2) + (lane & 7) * 16) | past, off);
+        const int at = s * 128 + 8 * (wave * XPW + i) * static_cast<int>(a.pitch * 2);  // rows past the last are past the buffer's end
+        b.x[i] = buffer_load16(xr, x_from, s < hi ? at : kOOB);
     };
+    const int x_to = wave * XPW * 1024 + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);  // 16-byte columns swizzled by row
     auto write_x = [&](const step_data& b, int i, int slot) {
-        const int lane = own_lane(), r = 8 * (wave * XPW + i) + (lane >> 3);
-        *reinterpret_cast<u32x4_t*>(lds + slot * XS + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = b.x[i];  // 16-byte columns swizzled by row
+        *reinterpret_cast<u32x4_t*>(lds + slot * XS + x_to + i * 1024) = b.x[i];
     };
 
     // Wavefront w decodes one tile of a step: strip w / 2, K tile w % 2 (the second may lie past K).
     const int kt = 2 * nb + (wave & 1);
     auto load_w = [&](step_data& b, int s) {
-        const int lane = own_lane();
         const int side = s >= a.side_steps ? 1 : 0, strip = 4 * (s - side * a.side_steps) + (wave >> 1);
         const uint8_t* base = side ? a.w1.codes : a.w0.codes;
         const uint32_t* sbase = side ? a.w1.scale : a.w0.scale;
         const bool in = s < hi && strip < a.strips && kt < a.ktiles;
         const int64_t at = in ? strip : 0, t = in ? kt : 0;
-        const int past = in ? 0 : kOOB;
-        b.c = buffer_load16(make_rsrc(base + (at * a.ktiles + t) * kSubTileBytes, kSubTileBytes), (lane * 16) | past);
-        b.s = buffer_load_u32(make_rsrc(sbase + ((at >> 2) * a.ktiles + t) * 64, 256u), (lane * 4) | past, 0);
+        b.c = buffer_load16(make_rsrc(base + (at * a.ktiles + t) * kSubTileBytes, kSubTileBytes), lane * 16, in ? 0 : kOOB);
+        b.s = buffer_load_u32(make_rsrc(sbase + ((at >> 2) * a.ktiles + t) * 64, 256u), lane * 4, in ? 0 : kOOB);
     };
     // LDS row n (512 bytes): its 32-byte pieces are XOR-swizzled by f(n) = n % 4 + 4 ((n / 4 + n / 8) % 2),
     // which sets apart both the eight rows that one write covers and the rows of one transposing read.
+    const int w_to = S0 + ((wave >> 1) * 16 + col16) * 512 +
+                     ((((wave & 1) * 8 + 2 * kq) ^ ((col16 & 3) | ((((col16 >> 2) ^ (col16 >> 3)) & 1) << 2))) << 5);
     auto write_w = [&](const step_data& b, int q, int slot) {
-        const int lane = own_lane(), col16 = lane & 15, kq = lane >> 4;
-        const int wrow = (wave >> 1) * 16 + col16, wf = (col16 & 3) | ((((col16 >> 2) ^ (col16 >> 3)) & 1) << 2);
-        uint8_t* base = wlds + slot * WS + wrow * 512;
         const float s = mx_scale(b.s >> (8 * (wave >> 1)) & 0xffu);
-        *reinterpret_cast<u32x4_t*>(base + ((((wave & 1) * 8 + 2 * kq + (q >> 1)) ^ wf) << 5) + (q & 1) * 16) = mx_decode<BF16>(b.c[q], s);
+        *reinterpret_cast<u32x4_t*>(lds + slot * WS + (w_to ^ ((q >> 1) << 5)) + (q & 1) * 16) = mx_decode<BF16>(b.c[q], s);
     };
 
     u32x4_t x[MT], w[2][NS];  // fragments; x's are read again for the next half right after their use
-    struct lane_offsets {
-        int x, w;
-    };
-    auto fragment_offsets = [&] {
-        const int lane = own_lane(), col16 = lane & 15, kq = lane >> 4, f = (col16 >> 2) | ((kq & 1) << 2);
-        return lane_offsets{wm * MT * 2048 + col16 * 128 + ((kq ^ (col16 & 7)) << 4),
-                            (8 * kq + (col16 >> 2)) * 512 + (((wn * NS) ^ f) << 5) + (col16 & 3) * 8};
-    };
-    auto read_x = [&](const lane_offsets& o, int i, int slot, int t) {
-        x[i] = *reinterpret_cast<const u32x4_t*>(lds + slot * XS + (o.x ^ (t << 6)) + i * 2048);
-    };
-    auto read_w = [&](const lane_offsets& o, u32x4_t (&w)[NS], int j, int slot, int t) {
-        const uint8_t* p = wlds + slot * WS + t * 32 * 512;
-        const tr_t lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr_t*)(p + (o.w ^ (j << 5))));
-        const tr_t hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr_t*)(p + 2048 + (o.w ^ ((j ^ 4) << 5))));
+    const int x_at = wm * MT * 2048 + col16 * 128 + ((kq ^ (col16 & 7)) << 4);
+    const int w_at = S0 + (8 * kq + (col16 >> 2)) * 512 + (((wn * NS) ^ ((col16 >> 2) | ((kq & 1) << 2))) << 5) + (col16 & 3) * 8;
+    auto read_x = [&](int i, int slot, int t) { x[i] = *reinterpret_cast<const u32x4_t*>(lds + slot * XS + (x_at ^ (t << 6)) + i * 2048); };
+    auto read_w = [&](u32x4_t (&w)[NS], int j, int slot, int t) {
+        const int at = slot * WS + w_at;
+        const tr_t lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr_t*)(lds + (at ^ (j << 5)) + t * 16384));
+        const tr_t hi4 =
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr_t*)(lds + (at ^ ((j ^ 4) << 5)) + t * 16384 + 2048));
         const u32x2_t l = __builtin_bit_cast(u32x2_t, lo4), h = __builtin_bit_cast(u32x2_t, hi4);
         w[j] = u32x4_t{l[0], l[1], h[0], h[1]};
     };
@@ -139,14 +123,12 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
     for (int i = 0; i < XPW; ++i) load_x(b, i, lo + 1);
     load_w(b, lo + 1);
     __syncthreads();
-    lane_offsets o = fragment_offsets();
 #pragma unroll
-    for (int i = 0; i < MT; ++i) read_x(o, i, 0, 0);
+    for (int i = 0; i < MT; ++i) read_x(i, 0, 0);
 #pragma unroll
-    for (int j = 0; j < NS; ++j) read_w(o, w[0], j, 0, 0);
+    for (int j = 0; j < NS; ++j) read_w(w[0], j, 0, 0);
     int slot = 0;
     for (int s = lo; s < hi; ++s) {
-        o = fragment_offsets();
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             // The other slot is filled over the first rows of matrix instructions, and the data of the step
@@ -161,10 +143,10 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
             }
             if (i == MT - 1) load_w(b, s + 2);
 #pragma unroll
-            for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(o, w[1], j, slot, 1);
+            for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(w[1], j, slot, 1);
 #pragma unroll
             for (int j = 0; j < NS; ++j) acc[i][j] = mfma16x16x32<BF16>(w[0][j], x[i], acc[i][j]);
-            read_x(o, i, slot, 1);
+            read_x(i, slot, 1);
             __builtin_amdgcn_sched_barrier(0);  // the reads stay among the matrix instructions, half a step ahead
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -172,10 +154,10 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
-            for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(o, w[0], j, slot, 0);
+            for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(w[0], j, slot, 0);
 #pragma unroll
             for (int j = 0; j < NS; ++j) acc[i][j] = mfma16x16x32<BF16>(w[1][j], x[i], acc[i][j]);
-            read_x(o, i, slot, 0);
+            read_x(i, slot, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -267,17 +249,31 @@ struct grad_plan {
     int mt;
     int64_t m_blocks, n_blocks, steps, splits, split_steps;
 };
+// The tile height and the split with the least estimated time (us): steps of the busiest CU, each 0.76 / 1.0 /
+// 1.55 us at 64 / 128 / 256 rows, and the fp32 sums, written and read by a kernel more at 5.5 TB/s (they mostly stay in
+// the caches). Measured against the best of 24 forced choices (N 4096, K 4096): M = 48 16.6 of 16.6 us, M = 333
+// 29.7 of 29.7, M = 1000 47.4 of 47.4, M = 2000 72 of 72; 64, 256 and 256 rows unsplit take 20, 61 and 100 us there.
 grad_plan make_grad_plan(int64_t m, int64_t k, int64_t steps) {
-    grad_plan p{};
-    p.mt = m <= 64 ? 2 : 8;
-    p.m_blocks = ceil_div(m, 32 * p.mt);
-    p.n_blocks = ceil_div(k, kGradCols);
-    p.steps = steps;
-    const int64_t want = std::max<int64_t>(1, cu_count() / (p.m_blocks * p.n_blocks));
-    p.splits = std::max<int64_t>(1, std::min<int64_t>(want, steps / 8));
-    p.split_steps = ceil_div(steps, p.splits);
-    p.splits = ceil_div(steps, p.split_steps);
-    return p;
+    grad_plan best{};
+    double least = 1e300;
+    const int64_t cus = cu_count();
+    for (int mt = 2; mt <= 8; mt *= 2) {
+        grad_plan p{};
+        p.mt = mt;
+        p.m_blocks = ceil_div(m, 32 * mt);
+        p.n_blocks = ceil_div(k, kGradCols);
+        p.steps = steps;
+        const double step = mt == 2 ? 0.76 : (mt == 4 ? 1.0 : 1.55);
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(steps / 8, 2 * cus / (p.m_blocks * p.n_blocks)));
+        for (int64_t splits = 1; splits <= most; ++splits) {
+            p.split_steps = ceil_div(steps, splits);
+            p.splits = ceil_div(steps, p.split_steps);
+            const int64_t rounds = ceil_div(p.m_blocks * p.n_blocks * p.splits, cus);
+            const double t = rounds * (p.split_steps * step + 4.) + (p.splits > 1 ? 2. + p.splits * m * k * 8 / 5.5e6 : 0.);
+            if (t < least) least = t, best = p;
+        }
+    }
+    return best;
 }
 
 int64_t padded_n(int64_t n) { return round_up(n, kGradStep); }
@@ -334,6 +330,7 @@ int run(const char* op, bool gated, const void* dy, const void* gate_up, const m
     a.n_blocks = static_cast<int>(p.n_blocks);
     const dim3 grid(static_cast<unsigned>(p.m_blocks * p.n_blocks), static_cast<unsigned>(p.splits));
     if (p.mt == 2) mx_grad_kernel<BF16, 2><<<grid, 512, 0, s>>>(a);
+    else if (p.mt == 4) mx_grad_kernel<BF16, 4><<<grid, 512, 0, s>>>(a);
     else mx_grad_kernel<BF16, 8><<<grid, 512, 0, s>>>(a);
     PLM_HIP_LAUNCH_CHECK(op);
     if (p.splits > 1) {

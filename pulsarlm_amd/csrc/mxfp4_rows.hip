@@ -74,19 +74,18 @@ __global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
         uint32_t s[SG], xs[XM == kXCodes ? RB : 1];
     };
     auto load = [&](batch& b, int kt) {
-        const bool in = kt < a.ktiles;
-        const int past = in ? 0 : kOOB, w_off = in ? kt * kSubTileBytes : 0, s_off = in ? kt * 256 : 0;
+        const bool in = kt < a.ktiles;  // a load's range check covers both its offsets
 #pragma unroll
         for (int j = 0; j < SG; ++j) {
             const int side = j / P, jj = j % P;
-            b.w[j] = buffer_load16_stream(wr[side], (jj * a.ktiles * kSubTileBytes + lane * 16) | past, w_off);
-            b.s[j] = __builtin_amdgcn_raw_buffer_load_b8(sr[side], (lane * 4 + ((strip0 + jj) & 3)) | past, s_off, 0);
+            b.w[j] = buffer_load16_stream(wr[side], lane * 16, in ? (jj * a.ktiles + kt) * kSubTileBytes : kOOB);
+            b.s[j] = __builtin_amdgcn_raw_buffer_load_b8(sr[side], lane * 4, in ? kt * 256 + ((strip0 + jj) & 3) : kOOB, 0);
         }
         if constexpr (XM == kXCodes) {
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
-                b.x[i] = buffer_load16(xr, (i * a.ktiles * kSubTileBytes + lane * 16) | past, w_off);
-                b.xs[i] = __builtin_amdgcn_raw_buffer_load_b8(xsr, (lane * 4 + ((row0 / 16 + i) & 3)) | past, s_off, 0);
+                b.x[i] = buffer_load16(xr, lane * 16, in ? (i * a.ktiles + kt) * kSubTileBytes : kOOB);
+                b.xs[i] = __builtin_amdgcn_raw_buffer_load_b8(xsr, lane * 4, in ? kt * 256 + ((row0 / 16 + i) & 3) : kOOB, 0);
             }
         }
     };

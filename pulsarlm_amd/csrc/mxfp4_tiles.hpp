@@ -110,32 +110,29 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
     // Load l of the wavefront's LOADS for K tile kt. Chunk c of a stage: x's first (codes: strip c; 16-bit: rows
     // 4 c .. 4 c + 3, their 16-byte columns XOR-swizzled by row), then the weight strips', then the scales'. Past
     // the end of any, zeros.
+    // A load's range check covers both its offsets (checked on the GPU): the lanes' own hardly change, and past the
+    // end the wave-uniform one is kOOB.
     constexpr int XL = XC / NW, WL = BS / NW;
+    const int x_row = (lane >> 4) * a.k * 2, x_col = ((lane & 15) ^ (lane >> 4)) << 4;
     auto issue_one = [&](int l, int turn, int slot) {
         const int kt = turn * KG + group;
         const bool in = kt < a.ktiles;
-        const int past = in ? 0 : kOOB, off = in ? kt : 0;
         uint8_t* base = stages + slot * (KG * STAGE);
-        // The large W4A16 tile: an opaque copy of the lane id, so that the offsets are worked out here and not kept in
-        // registers, of which it has none to spare.
-        int lane = threadIdx.x & 63;
-        if constexpr (!A4 && MT * NS >= 32) asm volatile("" : "+v"(lane));
         if (l < XL) {
             const int c = wave * XL + l;
             if constexpr (A4) {
-                buffer_load_lds16(xr, base + c * 1024, (c * a.ktiles * kSubTileBytes + lane * 16) | past, off * kSubTileBytes);
+                buffer_load_lds16(xr, base + c * 1024, lane * 16, in ? (c * a.ktiles + kt) * kSubTileBytes : kOOB);
             } else {
-                const int r = 4 * c + (lane >> 4), col = (lane & 15) ^ (r & 15);
-                const int at = kt * kTileK + col * 8 < a.k ? r * a.k * 2 + col * 16 : kOOB;
-                buffer_load_lds16(xr, base + c * 1024, at, off * 256);
+                const int col = x_col ^ ((c & 3) << 6);  // the lane's row 4 c + lane / 16, its column swizzled by row % 16
+                buffer_load_lds16(xr, base + c * 1024, col < (a.k - kt * kTileK) * 2 ? x_row + col : kOOB, in ? kt * 256 + c * a.k * 8 : kOOB);
             }
         } else if (l < XL + WL) {
             const int c = wave * WL + l - XL, side = SIDES == 2 ? c & 1 : 0, strip = SIDES == 2 ? c >> 1 : c;
-            buffer_load_lds16(wr[side], base + (XC + c) * 1024, (strip * a.ktiles * kSubTileBytes + lane * 16) | past, off * kSubTileBytes);
+            buffer_load_lds16(wr[side], base + (XC + c) * 1024, lane * 16, in ? (strip * a.ktiles + kt) * kSubTileBytes : kOOB);
         } else {
             const int i = l - XL - WL;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(scr[i], (__attribute__((address_space(3))) void*)(base + (XC + BS) * 1024 + scc[i] * 256), 4,
-                                                     (scg[i] * a.ktiles * 256 + lane * 4) | past, off * 256, 0, 0);
+                                                     lane * 4, in ? (scg[i] * a.ktiles + kt) * 256 : kOOB, 0, 0);
         }
     };
     // The loads of a K tile stand among the matrix instructions, at places 0 .. SPREAD - 1 (one row of them

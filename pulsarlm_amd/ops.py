@@ -394,8 +394,10 @@ def gemm_int4_split_cuda(x: torch.Tensor, weight_packed: torch.Tensor, weight_sc
 
 
 def _mx_contiguous(op: str, name: str, x: torch.Tensor, dtypes) -> None:
-    _require(x.is_cuda and x.dtype in dtypes, op, f"{name} must be a CUDA {'fp32, ' if len(dtypes) > 2 else ''}fp16 or bf16 tensor")
-    _require(x.dim() == 2 and x.is_contiguous(), op, f"{name} must be contiguous [rows, columns]")
+    if not (x.is_cuda and x.dtype in dtypes):
+        _require(False, op, f"{name} must be a CUDA {'fp32, ' if len(dtypes) > 2 else ''}fp16 or bf16 tensor")
+    if not (x.dim() == 2 and x.is_contiguous()):
+        _require(False, op, f"{name} must be contiguous [rows, columns]")
 
 
 _HALF = (torch.float16, torch.bfloat16)
@@ -457,11 +459,12 @@ def _mx_scale_shape(n: int, k: int):
 
 def _mx_weight(op: str, x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, n: int, k: int) -> None:
     _require(n >= 0 and k >= 0, op, "sizes must be non-negative")
-    _require(weight.device == x.device and scale.device == x.device, op, "x and the weights must be on one device")
-    _require(weight.dtype == torch.int32 and scale.dtype == torch.int32 and weight.is_contiguous() and scale.is_contiguous(), op,
+    at = x.get_device()
+    _require(weight.get_device() == at and scale.get_device() == at, op, "x and the weights must be on one device")
+    _require(weight.dtype is torch.int32 and scale.dtype is torch.int32 and weight.is_contiguous() and scale.is_contiguous(), op,
              "weight and scale must be contiguous int32, as repack_mxfp4 returns them")
     _require(weight.numel() * 4 == _lib.mxfp4_bytes("mxfp4_weight_bytes", n, k), op, "weight has the wrong size for this shape")
-    _require(tuple(scale.shape) == _mx_scale_shape(n, k), op, "scale has the wrong shape for this N and K")
+    _require(scale.shape == _mx_scale_shape(n, k), op, "scale has the wrong shape for this N and K")
 
 
 def _mx_scratch(name: str, x: torch.Tensor, *sizes: int) -> torch.Tensor | None:
@@ -472,7 +475,7 @@ def _mx_scratch(name: str, x: torch.Tensor, *sizes: int) -> torch.Tensor | None:
 
 def _mx_out(op: str, x: torch.Tensor, shape, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=x.dtype, device=x.device)
+        return x.new_empty(shape)
     _require(out.dtype == x.dtype and out.device == x.device and tuple(out.shape) == shape and out.is_contiguous(), op,
              f"out must be contiguous {list(shape)} of x's dtype and device")
     return out
