@@ -1,5 +1,5 @@
 // linear over the pulsarlm_amd ops: the reference's dense/fp8 linear
-// (pulsarlm-core/src/engine/model/linear.cpp:14-41) plus an int4 alternative.
+// (pulsarlm-core/src/engine/model/linear.cpp:14-41) plus int4 and MXFP4 alternatives.
 // Quantized weights are repacked once, at construction, as the reference does.
 #include "linear.hpp"
 
@@ -10,7 +10,7 @@
 
 namespace pulsarlm {
 
-linear::linear(std::variant<at::Tensor, quant_weight> weight) : weight(std::move(weight)) {}
+linear::linear(std::variant<at::Tensor, quant_weight, mxfp4_weight> weight) : weight(std::move(weight)) {}
 
 linear linear::dense(at::Tensor weight) { return linear(std::move(weight)); }
 
@@ -36,11 +36,21 @@ linear linear::int4(const at::Tensor& weight_packed, const at::Tensor& scale, st
     return linear(quant_weight{std::move(w), std::move(s), weight_packed.size(0), block_n, group_size, false});
 }
 
+linear linear::mxfp4(const at::Tensor& codes, const at::Tensor& scale, bool w4a4) {
+    auto [w, s] = repack_mxfp4_cuda(codes, scale);
+    return linear(mxfp4_weight{std::move(w), std::move(s), codes.size(0), w4a4});
+}
+
 at::Tensor linear::apply(const at::Tensor& x) const {
     if (const auto* dense = std::get_if<at::Tensor>(&weight)) return at::linear(x, *dense);
-    const quant_weight& w = std::get<quant_weight>(weight);
     std::vector<std::int64_t> sizes = x.sizes().vec();
     const at::Tensor rows = x.reshape({-1, sizes.back()}).contiguous();
+    if (const auto* mx = std::get_if<mxfp4_weight>(&weight)) {
+        sizes.back() = mx->n;
+        return (mx->w4a4 ? gemm_mxfp4_w4a4_cuda(rows, mx->weight, mx->scale, mx->n) : gemm_mxfp4_cuda(rows, mx->weight, mx->scale, mx->n))
+            .view(sizes);
+    }
+    const quant_weight& w = std::get<quant_weight>(weight);
     sizes.back() = w.n;
     const at::Tensor y = w.fp8 ? gemm_fp8_marlin_cuda(rows, w.weight_marlin, w.scale_marlin, w.n, w.block_n, w.group_size)
                                : gemm_int4_marlin_cuda(rows, w.weight_marlin, w.scale_marlin, w.n, w.block_n,

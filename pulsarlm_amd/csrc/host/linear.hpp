@@ -1,6 +1,6 @@
-// y = x @ W^T over x's last dim for a dense, fp8 or int4 weight: the reference's
+// y = x @ W^T over x's last dim for a dense, fp8, int4 or MXFP4 weight: the reference's
 // linear (pulsarlm-core/inc/pulsarlm/engine/model/linear.hpp:13-35,
-// src/engine/model/linear.cpp:19-41) with an int4 alternative next to fp8.
+// src/engine/model/linear.cpp:19-41) with int4 and MXFP4 alternatives next to fp8.
 #pragma once
 
 #include <ATen/ATen.h>
@@ -19,10 +19,16 @@ class linear {
         std::int64_t group_size;
         bool fp8;
     };
+    struct mxfp4_weight {
+        at::Tensor weight;
+        at::Tensor scale;
+        std::int64_t n;
+        bool w4a4;
+    };
 
-    std::variant<at::Tensor, quant_weight> weight;
+    std::variant<at::Tensor, quant_weight, mxfp4_weight> weight;
 
-    explicit linear(std::variant<at::Tensor, quant_weight> weight);
+    explicit linear(std::variant<at::Tensor, quant_weight, mxfp4_weight> weight);
 
   public:
     // weight [N, K] in x's dtype.
@@ -41,6 +47,9 @@ class linear {
     // weight_packed int32 [N, K/8] (8 signed int4 per int32, least significant first); same scale rule.
     static linear int4(const at::Tensor& weight_packed, const at::Tensor& scale, std::int64_t block_n,
                        std::int64_t group_size);
+
+    // codes uint8 [N, K/2], scale uint8 [N, K/32] (quantize_mxfp4_cuda's form); w4a4: x is quantized so, too.
+    static linear mxfp4(const at::Tensor& codes, const at::Tensor& scale, bool w4a4);
 
     at::Tensor apply(const at::Tensor& x) const;
 };

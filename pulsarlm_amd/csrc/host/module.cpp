@@ -22,10 +22,20 @@ PYBIND11_MODULE(_host, m) {
     m.def("silu_mul_cuda", &pulsarlm::silu_mul_cuda);
     m.def("gemm_int4_cuda", &pulsarlm::gemm_int4_cuda);
     m.def("gemm_int4_split_cuda", &pulsarlm::gemm_int4_split_cuda);
+    m.def("quantize_mxfp4_cuda", &pulsarlm::quantize_mxfp4_cuda);
+    m.def("dequantize_mxfp4_cuda", &pulsarlm::dequantize_mxfp4_cuda);
+    m.def("repack_mxfp4_cuda", &pulsarlm::repack_mxfp4_cuda);
+    m.def("gemm_mxfp4_cuda", &pulsarlm::gemm_mxfp4_cuda);
+    m.def("gemm_mxfp4_w4a4_cuda", &pulsarlm::gemm_mxfp4_w4a4_cuda);
+    m.def("gemm_mxfp4_grad_cuda", &pulsarlm::gemm_mxfp4_grad_cuda);
+    m.def("gated_mxfp4_cuda", &pulsarlm::gated_mxfp4_cuda);
+    m.def("gated_mxfp4_grad_cuda", &pulsarlm::gated_mxfp4_grad_cuda);
+    m.def("mlp_mxfp4_w4a4_cuda", &pulsarlm::mlp_mxfp4_w4a4_cuda);
     py::class_<pulsarlm::linear>(m, "linear")
         .def_static("dense", &pulsarlm::linear::dense)
         .def_static("fp8", &pulsarlm::linear::fp8)
         .def_static("fp8_rows", &pulsarlm::linear::fp8_rows)
         .def_static("int4", &pulsarlm::linear::int4)
+        .def_static("mxfp4", &pulsarlm::linear::mxfp4)
         .def("apply", &pulsarlm::linear::apply);
 }

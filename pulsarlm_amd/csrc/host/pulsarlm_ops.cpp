@@ -324,4 +324,165 @@ at::Tensor gemm_int4_split_cuda(const at::Tensor& x, const at::Tensor& weight_pa
     return gemm_int4_plain("gemm_int4", x, weight_packed, weight_scale, group_size, num_splits);
 }
 
+namespace {
+
+void mx_rows(const char* op, const char* name, const at::Tensor& x) {
+    TORCH_CHECK(x.is_cuda() && (x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16), op, ": ", name,
+                " must be a CUDA fp16 or bf16 tensor");
+    TORCH_CHECK(x.dim() == 2 && x.is_contiguous(), op, ": ", name, " must be contiguous [rows, columns]");
+}
+
+std::pair<int64_t, int64_t> mx_plain(const char* op, const at::Tensor& codes, const at::Tensor& scale) {
+    TORCH_CHECK(codes.is_cuda() && scale.is_cuda() && codes.device() == scale.device(), op,
+                ": codes and scale must be on one CUDA device");
+    TORCH_CHECK(codes.scalar_type() == at::kByte && scale.scalar_type() == at::kByte && codes.dim() == 2 && scale.dim() == 2, op,
+                ": codes must be uint8 [N, K/2] and scale uint8 [N, K/32]");
+    const int64_t n = codes.size(0), k = 2 * codes.size(1);
+    TORCH_CHECK(k % 32 == 0, op, ": K must be a multiple of 32");
+    TORCH_CHECK(scale.size(0) == n && scale.size(1) == k / 32, op, ": scale must be [N, K/32]");
+    return {n, k};
+}
+
+std::vector<int64_t> mx_scale_shape(int64_t n, int64_t k) { return {ceil_div(n, 64), ceil_div(k, 128), 64}; }
+
+void mx_weight(const char* op, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, int64_t n, int64_t k) {
+    TORCH_CHECK(n >= 0 && k >= 0, op, ": sizes must be non-negative");
+    TORCH_CHECK(weight.device() == x.device() && scale.device() == x.device(), op, ": x and the weights must be on one device");
+    TORCH_CHECK(weight.scalar_type() == at::kInt && scale.scalar_type() == at::kInt && weight.is_contiguous() && scale.is_contiguous(),
+                op, ": weight and scale must be contiguous int32, as repack_mxfp4 returns them");
+    TORCH_CHECK(weight.numel() * 4 == plm_mxfp4_weight_bytes(n, k), op, ": weight has the wrong size for this shape");
+    TORCH_CHECK(scale.sizes().vec() == mx_scale_shape(n, k), op, ": scale has the wrong shape for this N and K");
+}
+
+// Scratch of one call, from the caching allocator: a captured call's belongs to its graph.
+at::Tensor mx_scratch(const at::Tensor& x, int64_t bytes) {
+    return bytes > 0 ? at::empty({bytes}, x.options().dtype(at::kByte)) : at::Tensor();
+}
+size_t mx_bytes(const at::Tensor& t) { return t.defined() ? static_cast<size_t>(t.numel()) : 0; }
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> quantize_mxfp4_cuda(const at::Tensor& x) {
+    const char* op = "quantize_mxfp4";
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(), op, ": x must be a contiguous CUDA [M, K]");
+    TORCH_CHECK(x.size(1) % 32 == 0, op, ": K must be a multiple of 32");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor codes = at::empty({x.size(0), x.size(1) / 2}, x.options().dtype(at::kByte));
+    at::Tensor scale = at::empty({x.size(0), x.size(1) / 32}, x.options().dtype(at::kByte));
+    check_rc(plm_quantize_mxfp4(x.data_ptr(), dtype_of(op, x.scalar_type()), x.size(0), x.size(1),
+                                static_cast<uint8_t*>(codes.data_ptr()), static_cast<uint8_t*>(scale.data_ptr()), stream_of(x)));
+    return {codes, scale};
+}
+
+at::Tensor dequantize_mxfp4_cuda(const at::Tensor& codes, const at::Tensor& scale, at::ScalarType dtype) {
+    const char* op = "dequantize_mxfp4";
+    const auto [m, k] = mx_plain(op, codes, scale);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+    const at::Tensor c = codes.contiguous(), s = scale.contiguous();
+    at::Tensor out = at::empty({m, k}, codes.options().dtype(dtype));
+    check_rc(plm_dequantize_mxfp4(static_cast<const uint8_t*>(c.data_ptr()), static_cast<const uint8_t*>(s.data_ptr()), m, k,
+                                  out.data_ptr(), dtype_of(op, dtype), stream_of(codes)));
+    return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> repack_mxfp4_cuda(const at::Tensor& codes, const at::Tensor& scale) {
+    const auto [n, k] = mx_plain("repack_mxfp4", codes, scale);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+    const at::Tensor c = codes.contiguous(), s = scale.contiguous();
+    at::Tensor weight = at::empty({plm_mxfp4_weight_bytes(n, k) / 4}, codes.options().dtype(at::kInt));
+    at::Tensor packed = at::empty(mx_scale_shape(n, k), codes.options().dtype(at::kInt));
+    check_rc(plm_repack_mxfp4(static_cast<const uint8_t*>(c.data_ptr()), static_cast<const uint8_t*>(s.data_ptr()), n, k,
+                              weight.data_ptr(), packed.data_ptr(), stream_of(codes)));
+    return {weight, packed};
+}
+
+at::Tensor gemm_mxfp4_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, int64_t n) {
+    const char* op = "gemm_mxfp4";
+    mx_rows(op, "x", x);
+    mx_weight(op, x, weight, scale, n, x.size(1));
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor y = at::empty({x.size(0), n}, x.options());
+    check_rc(plm_gemm_mxfp4(x.data_ptr(), dtype_of(op, x.scalar_type()), weight.data_ptr(), scale.data_ptr(), x.size(0), n, x.size(1),
+                            y.data_ptr(), stream_of(x)));
+    return y;
+}
+
+at::Tensor gemm_mxfp4_w4a4_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, int64_t n) {
+    const char* op = "gemm_mxfp4_w4a4";
+    mx_rows(op, "x", x);
+    mx_weight(op, x, weight, scale, n, x.size(1));
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor y = at::empty({x.size(0), n}, x.options());
+    const at::Tensor ws = mx_scratch(x, plm_gemm_mxfp4_w4a4_workspace_bytes(x.size(0), n, x.size(1)));
+    check_rc(plm_gemm_mxfp4_w4a4(x.data_ptr(), dtype_of(op, x.scalar_type()), weight.data_ptr(), scale.data_ptr(), x.size(0), n,
+                                 x.size(1), y.data_ptr(), ptr(ws), mx_bytes(ws), stream_of(x)));
+    return y;
+}
+
+at::Tensor gemm_mxfp4_grad_cuda(const at::Tensor& dy, const at::Tensor& weight, const at::Tensor& scale, int64_t k) {
+    const char* op = "gemm_mxfp4_grad";
+    mx_rows(op, "dy", dy);
+    mx_weight(op, dy, weight, scale, dy.size(1), k);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
+    at::Tensor dx = at::empty({dy.size(0), k}, dy.options());
+    const at::Tensor ws = mx_scratch(dy, plm_gemm_mxfp4_grad_workspace_bytes(dy.size(0), dy.size(1), k));
+    check_rc(plm_gemm_mxfp4_grad(dy.data_ptr(), dtype_of(op, dy.scalar_type()), weight.data_ptr(), scale.data_ptr(), dy.size(0),
+                                 dy.size(1), k, dx.data_ptr(), ptr(ws), mx_bytes(ws), stream_of(dy)));
+    return dx;
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_mxfp4_cuda(const at::Tensor& x, const at::Tensor& gate_weight, const at::Tensor& gate_scale,
+                                                    const at::Tensor& up_weight, const at::Tensor& up_scale,
+                                                    int64_t intermediate, bool keep_gate_up) {
+    const char* op = "gated_mxfp4";
+    mx_rows(op, "x", x);
+    mx_weight(op, x, gate_weight, gate_scale, intermediate, x.size(1));
+    mx_weight(op, x, up_weight, up_scale, intermediate, x.size(1));
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor h = at::empty({x.size(0), intermediate}, x.options());
+    at::Tensor gate_up = keep_gate_up ? at::empty({x.size(0), 2 * intermediate}, x.options().dtype(at::kFloat)) : at::Tensor();
+    check_rc(plm_gated_mxfp4(x.data_ptr(), dtype_of(op, x.scalar_type()), gate_weight.data_ptr(), gate_scale.data_ptr(),
+                             up_weight.data_ptr(), up_scale.data_ptr(), x.size(0), intermediate, x.size(1), h.data_ptr(),
+                             static_cast<float*>(ptr(gate_up)), stream_of(x)));
+    return {h, gate_up};
+}
+
+at::Tensor gated_mxfp4_grad_cuda(const at::Tensor& dh, const at::Tensor& gate_up, const at::Tensor& gate_weight,
+                                 const at::Tensor& gate_scale, const at::Tensor& up_weight, const at::Tensor& up_scale,
+                                 int64_t hidden) {
+    const char* op = "gated_mxfp4_grad";
+    mx_rows(op, "dh", dh);
+    const int64_t m = dh.size(0), n = dh.size(1);
+    TORCH_CHECK(gate_up.scalar_type() == at::kFloat && gate_up.device() == dh.device() && gate_up.dim() == 2 && gate_up.size(0) == m &&
+                    gate_up.size(1) == 2 * n && gate_up.is_contiguous(),
+                op, ": gate_up must be contiguous fp32 [M, 2 I] on dh's device");
+    mx_weight(op, dh, gate_weight, gate_scale, n, hidden);
+    mx_weight(op, dh, up_weight, up_scale, n, hidden);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(dh.device());
+    at::Tensor dx = at::empty({m, hidden}, dh.options());
+    const at::Tensor ws = mx_scratch(dh, plm_gated_mxfp4_grad_workspace_bytes(m, n, hidden));
+    check_rc(plm_gated_mxfp4_grad(dh.data_ptr(), static_cast<const float*>(gate_up.data_ptr()), dtype_of(op, dh.scalar_type()),
+                                  gate_weight.data_ptr(), gate_scale.data_ptr(), up_weight.data_ptr(), up_scale.data_ptr(), m, n, hidden,
+                                  dx.data_ptr(), ptr(ws), mx_bytes(ws), stream_of(dh)));
+    return dx;
+}
+
+at::Tensor mlp_mxfp4_w4a4_cuda(const at::Tensor& x, const at::Tensor& gate_weight, const at::Tensor& gate_scale,
+                               const at::Tensor& up_weight, const at::Tensor& up_scale, const at::Tensor& down_weight,
+                               const at::Tensor& down_scale, int64_t intermediate) {
+    const char* op = "mlp_mxfp4_w4a4";
+    mx_rows(op, "x", x);
+    const int64_t m = x.size(0), k = x.size(1);
+    mx_weight(op, x, gate_weight, gate_scale, intermediate, k);
+    mx_weight(op, x, up_weight, up_scale, intermediate, k);
+    mx_weight(op, x, down_weight, down_scale, k, intermediate);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor y = at::empty({m, k}, x.options());
+    const at::Tensor ws = mx_scratch(x, plm_mlp_mxfp4_w4a4_workspace_bytes(m, intermediate, k));
+    check_rc(plm_mlp_mxfp4_w4a4(x.data_ptr(), dtype_of(op, x.scalar_type()), gate_weight.data_ptr(), gate_scale.data_ptr(),
+                                up_weight.data_ptr(), up_scale.data_ptr(), down_weight.data_ptr(), down_scale.data_ptr(), m,
+                                intermediate, k, y.data_ptr(), ptr(ws), mx_bytes(ws), stream_of(x)));
+    return y;
+}
+
 }  // namespace pulsarlm

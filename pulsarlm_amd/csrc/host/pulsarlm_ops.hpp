@@ -88,4 +88,35 @@ at::Tensor gemm_int4_cuda(const at::Tensor& x, const at::Tensor& weight_packed, 
 at::Tensor gemm_int4_split_cuda(const at::Tensor& x, const at::Tensor& weight_packed,
                                 const at::Tensor& weight_scale, int64_t group_size, int64_t num_splits);
 
+// ---- MXFP4: microscaled 4-bit floating point (no counterpart in ops.hpp). 32 consecutive K values share a
+// scale 2^(b - 127) and are e2m1 codes; include/pulsarlm_amd.h has the rules. ----
+
+// x [M, K] fp32, fp16 or bf16 -> (codes uint8 [M, K/2], scale uint8 [M, K/32]), and back.
+std::tuple<at::Tensor, at::Tensor> quantize_mxfp4_cuda(const at::Tensor& x);
+at::Tensor dequantize_mxfp4_cuda(const at::Tensor& codes, const at::Tensor& scale, at::ScalarType dtype);
+
+// A weight [N, K] in that form, repacked for the products: (weight int32 1-D, scale int32 [groups, K tiles, 64]).
+std::tuple<at::Tensor, at::Tensor> repack_mxfp4_cuda(const at::Tensor& codes, const at::Tensor& scale);
+
+// y [M, N] = x [M, K] @ W^T, with 16-bit x and with x quantized as by quantize_mxfp4_cuda.
+at::Tensor gemm_mxfp4_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, int64_t n);
+at::Tensor gemm_mxfp4_w4a4_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, int64_t n);
+
+// The gradient of gemm_mxfp4_cuda's x: dx [M, K] = dy [M, N] @ W.
+at::Tensor gemm_mxfp4_grad_cuda(const at::Tensor& dy, const at::Tensor& weight, const at::Tensor& scale, int64_t k);
+
+// (h [M, I] = silu(x @ Wgate^T) * (x @ Wup^T), gate_up fp32 [M, 2 I] where keep_gate_up, else undefined), and the
+// gradient of its x [M, hidden] from dh and that gate_up.
+std::tuple<at::Tensor, at::Tensor> gated_mxfp4_cuda(const at::Tensor& x, const at::Tensor& gate_weight, const at::Tensor& gate_scale,
+                                                    const at::Tensor& up_weight, const at::Tensor& up_scale,
+                                                    int64_t intermediate, bool keep_gate_up);
+at::Tensor gated_mxfp4_grad_cuda(const at::Tensor& dh, const at::Tensor& gate_up, const at::Tensor& gate_weight,
+                                 const at::Tensor& gate_scale, const at::Tensor& up_weight, const at::Tensor& up_scale,
+                                 int64_t hidden);
+
+// The feed-forward block with 4-bit activations: y [M, K] = Q(h) @ Wdown^T, h of Q(x).
+at::Tensor mlp_mxfp4_w4a4_cuda(const at::Tensor& x, const at::Tensor& gate_weight, const at::Tensor& gate_scale,
+                               const at::Tensor& up_weight, const at::Tensor& up_scale, const at::Tensor& down_weight,
+                               const at::Tensor& down_scale, int64_t intermediate);
+
 }  // namespace pulsarlm
