@@ -22,7 +22,8 @@ int check_sizes(const char* op, plm_dtype x_dtype, int64_t m, int64_t n, int64_t
     PLM_CHECK_ARG(m >= 0 && n >= 0 && k >= 0, op, "sizes must be non-negative");
     PLM_CHECK_ARG(k % kMxBlock == 0, op, "K must be a multiple of 32");
     PLM_CHECK_ARG(n <= kMxMaxSize && k <= kMxMaxSize, op, "N and K must be at most 2^19");
-    PLM_CHECK_ARG(m <= (int64_t{1} << 30) && m * std::max(n, k) <= (int64_t{1} << 36), op, "M must be at most 2^30, M N and M K at most 2^36");
+    // A grid of at most 2^32 work-items, and offsets of one workgroup below kOOB.
+    PLM_CHECK_ARG(m <= (int64_t{1} << 24) && m * std::max(n, k) <= (int64_t{1} << 36), op, "M must be at most 2^24, M N and M K at most 2^36");
     return PLM_OK;
 }
 int check_weight(const char* op, const void* weight, const void* scale) {

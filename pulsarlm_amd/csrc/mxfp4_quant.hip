@@ -107,27 +107,29 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const uint32_t*
 // One thread: 16 bytes of the tile layout, a row's block as it lies in the source.
 __global__ void __launch_bounds__(kThreads) mx_repack_codes_kernel(const uint8_t* __restrict__ codes, int64_t n, int64_t k, int64_t ktiles,
                                                                    int64_t total, u32x4_t* __restrict__ out) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= total) return;
-    const int lane = static_cast<int>(i & 63);
-    const int64_t tile = i >> 6, row = tile / ktiles * 16 + (lane & 15), block = tile % ktiles * 4 + (lane >> 4);
-    u32x4_t v = {0, 0, 0, 0};
-    if (row < n && block * kMxBlock < k) v = *reinterpret_cast<const u32x4_t*>(codes + row * (k / 2) + block * 16);
-    out[i] = v;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += step) {
+        const int lane = static_cast<int>(i & 63);
+        const int64_t tile = i >> 6, row = tile / ktiles * 16 + (lane & 15), block = tile % ktiles * 4 + (lane >> 4);
+        u32x4_t v = {0, 0, 0, 0};
+        if (row < n && block * kMxBlock < k) v = *reinterpret_cast<const u32x4_t*>(codes + row * (k / 2) + block * 16);
+        out[i] = v;
+    }
 }
 
 __global__ void __launch_bounds__(kThreads) mx_repack_scale_kernel(const uint8_t* __restrict__ scale, int64_t n, int64_t blocks,
                                                                    int64_t ktiles, int64_t total, uint32_t* __restrict__ out) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= total) return;
-    const int lane = static_cast<int>(i & 63);
-    const int64_t tile = i >> 6, row0 = tile / ktiles * 64 + (lane & 15), block = tile % ktiles * 4 + (lane >> 4);
-    uint32_t v = 0;
-    for (int t = 0; t < 4; ++t) {
-        const int64_t row = row0 + 16 * t;
-        if (row < n && block < blocks) v |= static_cast<uint32_t>(scale[row * blocks + block]) << (8 * t);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += step) {
+        const int lane = static_cast<int>(i & 63);
+        const int64_t tile = i >> 6, row0 = tile / ktiles * 64 + (lane & 15), block = tile % ktiles * 4 + (lane >> 4);
+        uint32_t v = 0;
+        for (int t = 0; t < 4; ++t) {
+            const int64_t row = row0 + 16 * t;
+            if (row < n && block < blocks) v |= static_cast<uint32_t>(scale[row * blocks + block]) << (8 * t);
+        }
+        out[i] = v;
     }
-    out[i] = v;
 }
 
 unsigned stream_blocks(int64_t threads) {
@@ -218,10 +220,9 @@ int plm_repack_mxfp4(const uint8_t* codes, const uint8_t* scale, int64_t n, int6
     const mx_dims d = make_mx_dims(n, k);
     hipStream_t s = as_stream(stream);
     const int64_t total = d.strips * d.ktiles * 64, words = d.groups * d.ktiles * 64;
-    mx_repack_codes_kernel<<<static_cast<unsigned>(ceil_div(total, kThreads)), kThreads, 0, s>>>(codes, n, k, d.ktiles, total,
-                                                                                               static_cast<u32x4_t*>(weight_out));
-    mx_repack_scale_kernel<<<static_cast<unsigned>(ceil_div(words, kThreads)), kThreads, 0, s>>>(scale, n, k / kMxBlock, d.ktiles, words,
-                                                                                              static_cast<uint32_t*>(scale_out));
+    mx_repack_codes_kernel<<<stream_blocks(total), kThreads, 0, s>>>(codes, n, k, d.ktiles, total, static_cast<u32x4_t*>(weight_out));
+    mx_repack_scale_kernel<<<stream_blocks(words), kThreads, 0, s>>>(scale, n, k / kMxBlock, d.ktiles, words,
+                                                                     static_cast<uint32_t*>(scale_out));
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;
 }

@@ -434,9 +434,9 @@ def dequantize_mxfp4_cuda(codes: torch.Tensor, scale: torch.Tensor, dtype=torch.
     m, k = _mx_plain(op, codes, scale)
     _require(dtype in _DTYPES, op, "dtype must be fp32, fp16 or bf16")
     out = torch.empty((m, k), dtype=dtype, device=codes.device)
+    codes, scale = codes.contiguous(), scale.contiguous()  # both live until the call: copies do not share memory
     with _on(codes.device):
-        _call("plm_dequantize_mxfp4", _ptr(codes.contiguous()), _ptr(scale.contiguous()), m, k, _ptr(out), _DTYPES[dtype],
-              _stream(codes.device))
+        _call("plm_dequantize_mxfp4", _ptr(codes), _ptr(scale), m, k, _ptr(out), _DTYPES[dtype], _stream(codes.device))
     return out
 
 
@@ -447,9 +447,9 @@ def repack_mxfp4_cuda(codes: torch.Tensor, scale: torch.Tensor):
     n, k = _mx_plain(op, codes, scale)
     weight = torch.empty((_lib.mxfp4_bytes("mxfp4_weight_bytes", n, k) // 4,), dtype=torch.int32, device=codes.device)
     packed = torch.empty(_mx_scale_shape(n, k), dtype=torch.int32, device=codes.device)
+    codes, scale = codes.contiguous(), scale.contiguous()
     with _on(codes.device):
-        _call("plm_repack_mxfp4", _ptr(codes.contiguous()), _ptr(scale.contiguous()), n, k, _ptr(weight), _ptr(packed),
-              _stream(codes.device))
+        _call("plm_repack_mxfp4", _ptr(codes), _ptr(scale), n, k, _ptr(weight), _ptr(packed), _stream(codes.device))
     return weight, packed
 
 

@@ -69,8 +69,8 @@ PRODUCTS = {gemm: "gemm_mxfp4", w4a4: "gemm_mxfp4_w4a4", grad: "gemm_mxfp4_grad"
     ({"k": 80}, "K must be a multiple of 32"),
     ({"k": (1 << 19) + 32}, "N and K must be at most 2^19"),
     ({"n": (1 << 19) + 32}, "N and K must be at most 2^19"),
-    ({"m": (1 << 30) + 1}, "M must be at most 2^30"),
-    ({"m": 1 << 20, "k": 1 << 17}, "M must be at most 2^30"),
+    ({"m": (1 << 24) + 1}, "M must be at most 2^24"),
+    ({"m": 1 << 20, "k": 1 << 17}, "M must be at most 2^24"),
     ({"w": None}, "null pointer"),
     ({"s": None}, "null pointer"),
     ({"w": ODD}, "weight must be 16-byte aligned"),
