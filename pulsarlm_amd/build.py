@@ -43,10 +43,9 @@ FLAGS = [
 
 # Per-source flags. The MFMA kernel keeps its accumulators in VGPRs (the VGPR form of
 # v_mfma): with the default AGPR form the register allocator splits the accumulator set
-# between the two files and copies it back and forth every K step. (mxfp4_tiles_w4a4's 256 sums a
-# lane fill the AGPRs exactly: it keeps the default.)
+# between the two files and copies it back and forth every K step.
 SOURCE_FLAGS = {src: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-                for src in SOURCES if src.startswith(("gemm_mfma", "gemm_rows", "mxfp4_tiles_w4a16", "mxfp4_grad"))}
+                for src in SOURCES if src.startswith(("gemm_mfma", "gemm_rows", "mxfp4_tiles", "mxfp4_grad"))}
 
 
 EXTRA_DEFINES: list[str] = []

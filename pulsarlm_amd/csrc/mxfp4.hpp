@@ -194,10 +194,13 @@ struct mx_product {
     mx_matrix xq;
     mx_matrix w0, w1;
     int64_t m, n, k;
+    float* partial;  // W4A4, plain: room for the sums of K splits (mx_tiles_w4a4_bytes), or null
     bool bf16;
     mx_epilogue epilogue;
     mx_output out;
 };
+// out[i] = sum over s of partial[s][i], in order of s; count a multiple of 4, out 8-byte aligned.
+void launch_mx_combine(bool bf16, const float* partial, int64_t count, int splits, uint16_t* out, hipStream_t s);
 // The kernel for few rows: true where it has launched. quantize_x: it quantizes x16 itself.
 bool launch_mx_rows(const mx_product& p, bool quantize_x, hipStream_t s);
 

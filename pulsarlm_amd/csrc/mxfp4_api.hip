@@ -7,6 +7,7 @@ namespace plm {
 int zero_output(const char* op, void* y, int64_t m, int64_t n, hipStream_t s);
 void launch_mx_tiles_w4a16(const mx_product& p, hipStream_t s);
 void launch_mx_tiles_w4a4(const mx_product& p, hipStream_t s);
+int64_t mx_tiles_w4a4_bytes(int64_t m, int64_t n, int64_t k);
 int64_t mx_grad_bytes(int64_t m, int64_t n, int64_t k, bool gated);
 int launch_mx_grad(const char* op, bool gated, bool bf16, const void* dy, const void* gate_up, const mx_matrix& w0, const mx_matrix& w1,
                    int64_t m, int64_t n, int64_t k, void* dx, void* workspace, hipStream_t s);
@@ -49,7 +50,7 @@ int check_workspace(const char* op, const void* workspace, size_t have, int64_t 
     return PLM_OK;
 }
 
-// Codes of [M, K] in a workspace: [tiles][scales].
+// Codes of [M, K] in a workspace: [tiles][scales]. After them, the sums of K splits.
 struct codes_room {
     int64_t tiles, total;
 };
@@ -114,7 +115,7 @@ int plm_gemm_mxfp4(const void* x, plm_dtype x_dtype, const void* weight, const v
 }
 
 int64_t plm_gemm_mxfp4_w4a4_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return m <= 0 || n <= 0 || k <= 0 ? 0 : room(m, k).total;
+    return m <= 0 || n <= 0 || k <= 0 ? 0 : room(m, k).total + mx_tiles_w4a4_bytes(m, n, k);
 }
 
 int plm_gemm_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* weight, const void* scale, int64_t m, int64_t n, int64_t k, void* y,
@@ -128,8 +129,10 @@ int plm_gemm_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* weight, co
     if (k == 0) return zero_output(op, y, m, n, s);
     if (int rc = check_weight(op, weight, scale)) return rc;
     if (int rc = check_workspace(op, workspace, workspace_bytes, plm_gemm_mxfp4_w4a4_workspace_bytes(m, n, k))) return rc;
-    run_w4a4(product(x, x_dtype, matrix(weight, scale), {}, m, n, k, kMxPlain, mx_make_output(y, nullptr, n)),
-             place(workspace, 0, room(m, k)), s);
+    const codes_room r = room(m, k);
+    mx_product p = product(x, x_dtype, matrix(weight, scale), {}, m, n, k, kMxPlain, mx_make_output(y, nullptr, n));
+    p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + r.total);
+    run_w4a4(p, place(workspace, 0, r), s);
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;
 }
@@ -157,7 +160,7 @@ int plm_gated_mxfp4(const void* x, plm_dtype x_dtype, const void* gate_weight, c
 }
 
 int64_t plm_mlp_mxfp4_w4a4_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return m <= 0 || n <= 0 || k <= 0 ? 0 : room(m, k).total + room(m, n).total;
+    return m <= 0 || n <= 0 || k <= 0 ? 0 : room(m, k).total + room(m, n).total + mx_tiles_w4a4_bytes(m, k, n);
 }
 
 int plm_mlp_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* gate_weight, const void* gate_scale, const void* up_weight,
@@ -186,6 +189,7 @@ int plm_mlp_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* gate_weight
     PLM_HIP_LAUNCH_CHECK(op);
     mx_product down = product(nullptr, x_dtype, matrix(down_weight, down_scale), {}, m, k, n, kMxPlain, mx_make_output(y, nullptr, k));
     down.xq = hq.in();
+    down.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + xr.total + hr.total);
     if (!launch_mx_rows(down, false, s)) launch_mx_tiles_w4a4(down, s);
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;

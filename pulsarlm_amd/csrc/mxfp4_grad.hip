@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
 
 // Sums over the splits, four values a thread.
 template <bool BF16>
-__global__ void __launch_bounds__(256) mx_grad_combine_kernel(const f32x4_t* __restrict__ partial, int64_t quads, int splits,
+__global__ void __launch_bounds__(256) mx_combine_kernel(const f32x4_t* __restrict__ partial, int64_t quads, int splits,
                                                               uint2* __restrict__ dx) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= quads) return;
@@ -334,15 +334,22 @@ int run(const char* op, bool gated, const void* dy, const void* gate_up, const m
     else mx_grad_kernel<BF16, 8><<<grid, 512, 0, s>>>(a);
     PLM_HIP_LAUNCH_CHECK(op);
     if (p.splits > 1) {
-        const int64_t quads = m * k / 4;
-        mx_grad_combine_kernel<BF16><<<static_cast<unsigned>(ceil_div(quads, 256)), 256, 0, s>>>(
-            reinterpret_cast<const f32x4_t*>(a.partial), quads, a.splits, static_cast<uint2*>(dx));
+        launch_mx_combine(BF16, a.partial, m * k, a.splits, a.dx, s);
         PLM_HIP_LAUNCH_CHECK(op);
     }
     return PLM_OK;
 }
 
 }  // namespace
+
+void launch_mx_combine(bool bf16, const float* partial, int64_t count, int splits, uint16_t* out, hipStream_t s) {
+    const int64_t quads = count / 4;
+    const unsigned grid = static_cast<unsigned>(ceil_div(quads, 256));
+    const auto* p = reinterpret_cast<const f32x4_t*>(partial);
+    auto* o = reinterpret_cast<uint2*>(out);
+    if (bf16) mx_combine_kernel<true><<<grid, 256, 0, s>>>(p, quads, splits, o);
+    else mx_combine_kernel<false><<<grid, 256, 0, s>>>(p, quads, splits, o);
+}
 
 int64_t mx_grad_bytes(int64_t m, int64_t n, int64_t k, bool gated) { return grad_bytes(m, n, k, gated ? 2 : 1); }
 

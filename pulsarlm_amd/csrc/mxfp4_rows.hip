@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
     constexpr int SLOT = RB * 4096;                                  // ring: a K tile of x
     constexpr int XL = RB * 4;                                       // its loads of 1 KiB
     constexpr int WL = 2 * SG;                                       // loads of a K tile's weights and scales
-    static_assert(RB == 1 || (!STAGED && (XM == kXCodes || RB == 2)), "staged x is one row block, the ring holds two");
+    static_assert(RB == 1 || (!STAGED && RB == 2), "staged x is one row block");
     extern __shared__ __attribute__((aligned(1024))) uint8_t mx_lds[];
 
     const int lane = threadIdx.x & 63;
@@ -282,8 +282,7 @@ template <bool BF16> void launch_typed(const mx_product& p, bool quantize_x, hip
     if (quantize_x) return launch_sg<kXStagedQuantize, BF16, 1>(p, s);
     if (p.xq.codes != nullptr) {
         if (p.m <= 16) launch_sg<kXCodes, BF16, 1>(p, s);
-        else if (p.m <= 32) launch_sg<kXCodes, BF16, 2>(p, s);
-        else launch_sg<kXCodes, BF16, 4>(p, s);
+        else launch_sg<kXCodes, BF16, 2>(p, s);
     } else if (staged(p)) launch_sg<kXStaged, BF16, 1>(p, s);
     else if (p.m <= 16) launch_sg<kXRing, BF16, 1>(p, s);
     else launch_sg<kXRing, BF16, 2>(p, s);
@@ -294,7 +293,7 @@ template <bool BF16> void launch_typed(const mx_product& p, bool quantize_x, hip
 // Rows kernel or tiles, us. 16-bit x, M = 32: N 2048, K 2048 4.8 against 6.1; N 6144, K 4096 8.7, 10.3; N 4096, K 12288
 // 16.3, 21.9; but N 24576, K 4096 20.1, 18.0. M = 48 (four row blocks): 6.5 against 6.1; 12, 10.0; 26.7, 21.2. With
 // x as codes, M = 32: 7.1, 7.6; 9.8, 10.7; 14.7, 19.0; 18.1, 16.2 (M = 16 16.5, 15.1); M = 64: 8.9, 8.3; 12.3, 11.7;
-// but K 12288 18.6, 21.5.
+// K 12288 18.6, 17.1 (the tiles' K split).
 bool launch_mx_rows(const mx_product& p, bool quantize_x, hipStream_t s) {
     const int64_t strips = ceil_div(p.n, kTileN) * (p.epilogue == kMxPlain ? 1 : 2), cus = cu_count();
     const bool codes = p.xq.codes != nullptr;
@@ -302,7 +301,7 @@ bool launch_mx_rows(const mx_product& p, bool quantize_x, hipStream_t s) {
         if (!staged(p)) return false;
     } else if (strips > 4 * cus) {
         if (p.m > (codes ? 8 : 16)) return false;
-    } else if (p.m > (codes && p.k >= 8192 && strips <= 2 * cus ? 64 : 32)) {
+    } else if (p.m > 32) {
         return false;
     }
     if (p.bf16) launch_typed<true>(p, quantize_x, s);

@@ -3,16 +3,18 @@
 // matrix instruction, W4A4), plain or with the gated block's activation as the epilogue.
 //
 // * A workgroup owns BM = WM MT 16 rows by BS = WN NS strips; its WM x WN wavefronts own MT x NS products of
-//   16 x 16 each. The large W4A4 tile is 256 x 256 with four wavefronts of 128 x 128: each operand byte
-//   read from LDS then feeds eight matrix instructions, which is what LDS bandwidth needs (the operands of
-//   one K tile take 64 KiB of reads in 1024 cycles of matrix instructions). W4A16 has four times the cycles
-//   for 2.5 times the bytes: eight wavefronts of 128 x 64, whose sums fit the vector registers.
+//   16 x 16 each. The large tile is 256 x 256 with eight wavefronts of 128 x 64, whose 128 sums a lane leave the
+//   registers for the operands of two K tiles. (Four of 128 x 128 read a third less from LDS, but LDS is busy a
+//   quarter of the time, and one wavefront a SIMD leaves its matrix unit idle at every wait.)
 // * The operands of a K tile (128) go from memory straight into one of S LDS stages. One barrier a K tile
 //   stands before its last slice's matrix instructions, whose operands are in registers by then: past it
 //   every wavefront has read the stage, which the loads of K tile kt + S may overwrite, and K tile kt + 1 has
 //   landed, so that its first slice is read while those instructions run. W4A4 has one slice a K tile,
 //   W4A16 four of 32 K values.
 // * The weights are the A operand and x the B operand: a lane ends with four neighbouring columns of a row.
+// * What bounds it (M = 4096, N 24576, K 4096): W4A16 546 us, 1511 TFLOP/s, what the library's 16-bit product makes
+//   (1410-1455); W4A4 214 us, 3850 TFLOP/s, with the matrix units busy 55% of the cycles (70% at K 24576) at 1.7-1.9
+//   GHz. The same FLOPs at N 4096, K 24576, with a sixth of the stores, take 216 us: the clock gives way to the load.
 // * Gated: local strips 2 p and 2 p + 1 are gate and up of one 16-column slice, so that both halves of an
 //   output are in one lane.
 #pragma once
@@ -31,6 +33,8 @@ struct tile_args {
     mx_matrix xq, w0, w1;
     mx_output out;
     int m, k, ktiles, strips;
+    float* partial;                // W4A4: [splits][M][N] sums of split_tiles K tiles each, or null
+    int split_tiles;
     int m_blocks, n_blocks, band;  // band: row blocks of an XCD's patch of work tiles
 };
 
@@ -76,6 +80,9 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
     const int band_rows = min(a.band, a.m_blocks - first), in_band = lin - first * a.n_blocks;
     const int nb = in_band / band_rows, row0 = (first + in_band % band_rows) * BM;
     const int rows = min(BM, a.m - row0);
+    // The workgroup's K tiles.
+    const int kt_first = A4 ? static_cast<int>(blockIdx.y) * a.split_tiles : 0;
+    const int kt_end = A4 ? min(kt_first + a.split_tiles, a.ktiles) : a.ktiles;
 
     // Local strip s: strip nb BS + s, or slice nb BS / 2 + s / 2 of the gate (s even) or up weight.
     const int strip0 = nb * (BS / SIDES);
@@ -115,8 +122,8 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
     constexpr int XL = XC / NW, WL = BS / NW;
     const int x_row = (lane >> 4) * a.k * 2, x_col = ((lane & 15) ^ (lane >> 4)) << 4;
     auto issue_one = [&](int l, int turn, int slot) {
-        const int kt = turn * KG + group;
-        const bool in = kt < a.ktiles;
+        const int kt = kt_first + turn * KG + group;
+        const bool in = kt < kt_end;
         uint8_t* base = stages + slot * (KG * STAGE);
         if (l < XL) {
             const int c = wave * XL + l;
@@ -205,16 +212,14 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
 
     // W4A16: K tile kt's barrier stands before slice BAR, past which no wavefront reads its stage; the loads of
     // K tile kt + S into it are spread over the slices from there on into the next K tile.
-    // It stands after the first BP rows of matrix instructions of a K tile (W4A4) or of slice BAR: the last reads
-    // before it, which it has to wait for, have landed by then.
-    constexpr int BAR = SLICES - XB, BP = A4 && MT * NS >= 64 ? 1 : 0;
-    constexpr int SPREAD = A4 ? MT - BP : std::min(SLICES * MT, (XB + 1) * MT - BP);
+    constexpr int BAR = SLICES - XB;
+    constexpr int SPREAD = A4 ? MT : std::min(SLICES * MT, (XB + 1) * MT);
     using spread_t = std::integral_constant<int, SPREAD>;
 #pragma unroll
     for (int p = 0; p < S - 1; ++p) issue(p, p);
     // Of K tile S - 1 the loads that the first K tile's slices before BAR do not make.
 #pragma unroll
-    for (int place = 0; place < (A4 ? SPREAD : XB * MT - BP); ++place) issue_at(place, spread_t{}, S - 1, S - 1);
+    for (int place = 0; place < (A4 ? SPREAD : XB * MT); ++place) issue_at(place, spread_t{}, S - 1, S - 1);
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 2) * LOADS) : "memory");
 #pragma unroll
     for (int t = 0; t < XB; ++t)
@@ -230,7 +235,7 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
         shift_scales(sc[0]);
     }
     int slot = 0;
-    const int turns = (a.ktiles + KG - 1) / KG;  // past the last K tile one of zeros
+    const int turns = (kt_end - kt_first + KG - 1) / KG;  // past the last K tile one of zeros
     // K tile kt + 1 has landed when only the loads of S - 2 K tiles after it are left.
     constexpr int LEFT = (S - 2) * LOADS;
     static_assert(LEFT <= 63 && (SL || S == 2), "the counter's range; loads to registers are not counted");
@@ -239,22 +244,18 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
             const int ns = slot + 1 == S ? 0 : slot + 1;
             unrolled<MT>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
-                if constexpr (i == BP) {
+                if constexpr (i == 0) {
                     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
                     read_scales(s_next, ns);
-#pragma unroll
-                    for (int e = 0; e < BP; ++e) read_x(e, ns, 0);
                 }
-                if constexpr (i >= BP) {
-                    issue_at(i - BP, spread_t{}, kt + S, slot);
+                issue_at(i, spread_t{}, kt + S, slot);
 #pragma unroll
-                    for (int j = (i - BP) * NS / (MT - BP); j < (i + 1 - BP) * NS / (MT - BP); ++j) read_w(next, j, ns);
-                }
+                for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(next, j, ns);
                 unrolled<NS>([&](auto jc) {
                     constexpr int j = decltype(jc)::value, p = j / SIDES;
                     acc[i][j] = mx_mfma<p & 3, i & 3>(cur[j], s.w[j % SIDES][p / 4], x[0][i], s.x[i / 4], acc[i][j]);
                 });
-                if constexpr (i >= BP) read_x(i, ns, 0);
+                read_x(i, ns, 0);
                 __builtin_amdgcn_sched_barrier(0);  // reads and loads stay where they are
             });
             slot = ns;
@@ -280,21 +281,19 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
                 for (int j = 0; j < NS; ++j) wf[j] = mx_decode<BF16>(w[0][j][t], s[j]);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    if (t == BAR && i == BP) {
+                    if (t == BAR && i == 0) {
                         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
                         load_kt = kt + S;
                         load_slot = slot;
                         if constexpr (SL) read_scales(sc[1], ns);
-#pragma unroll
-                        for (int e = 0; e < BP; ++e) read_x(e, ns, (t + XB) % SLICES);
                     }
-                    issue_at(((t - BAR + SLICES) * MT + i - BP) % (SLICES * MT), spread_t{}, load_kt, load_slot);
-                    if (t == SLICES - 1 && i >= BP)
+                    issue_at(((t - BAR + SLICES) * MT + i) % (SLICES * MT), spread_t{}, load_kt, load_slot);
+                    if (t == SLICES - 1)
 #pragma unroll
-                        for (int j = (i - BP) * NS / (MT - BP); j < (i + 1 - BP) * NS / (MT - BP); ++j) read_w(w[1], j, ns);
+                        for (int j = i * NS / MT; j < (i + 1) * NS / MT; ++j) read_w(w[1], j, ns);
 #pragma unroll
                     for (int j = 0; j < NS; ++j) acc[i][j] = mfma16x16x32<BF16>(wf[j], x[t % XB][i], acc[i][j]);
-                    if (t != BAR || i >= BP) read_x(i, t >= BAR ? ns : slot, (t + XB) % SLICES);
+                    read_x(i, t >= BAR ? ns : slot, (t + XB) % SLICES);
                     __builtin_amdgcn_sched_barrier(0);  // reads and loads stay where they are
                 }
             }
@@ -361,6 +360,22 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
                         mx_store_gate_up(a.out, row0 + r, col0 + p * 16 + 4 * kq, acc[i][SIDES * p], acc[i][SIDES * p + SIDES - 1]);
             }
         }
+        if constexpr (A4 && EPI == kMxPlain) {
+            if (a.partial != nullptr) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const int r = (wm * MT + i) * 16 + col16;
+                    float* to = a.partial + (static_cast<int64_t>(blockIdx.y) * a.m + row0 + r) * a.out.n;
+                    if (r < rows)
+#pragma unroll
+                        for (int p = 0; p < PN; ++p) {
+                            const int col = col0 + p * 16 + 4 * kq;  // N is a multiple of 4
+                            if (col < a.out.n) *reinterpret_cast<f32x4_t*>(to + col) = acc[i][p];
+                        }
+                }
+                return;
+            }
+        }
         if (!a.out.lines) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -396,7 +411,7 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
     }
 }
 
-template <bool A4, bool BF16, mx_epilogue EPI, int WM, int WN, int MT, int NS, int S, int KG = 1, bool SL = true> void launch(const mx_product& p, hipStream_t s) {
+template <bool A4, bool BF16, mx_epilogue EPI, int WM, int WN, int MT, int NS, int S, int KG = 1, bool SL = true> void launch(const mx_product& p, int splits, hipStream_t s) {
     const mx_dims d = make_mx_dims(p.n, p.k);
     tile_args a{};
     a.x = p.x16;
@@ -412,7 +427,10 @@ template <bool A4, bool BF16, mx_epilogue EPI, int WM, int WN, int MT, int NS, i
     a.m_blocks = static_cast<int>(ceil_div(p.m, WM * MT * 16));
     a.n_blocks = static_cast<int>(ceil_div(d.strips, BS));
     a.band = 4;
-    mx_tile_kernel<A4, BF16, EPI, WM, WN, MT, NS, S, KG, SL><<<static_cast<unsigned>(a.m_blocks) * a.n_blocks, WM * WN * KG * 64, 0, s>>>(a);
+    a.split_tiles = static_cast<int>(ceil_div(d.ktiles, splits));
+    a.partial = splits > 1 ? p.partial : nullptr;
+    const dim3 grid(static_cast<unsigned>(a.m_blocks) * a.n_blocks, static_cast<unsigned>(splits));
+    mx_tile_kernel<A4, BF16, EPI, WM, WN, MT, NS, S, KG, SL><<<grid, WM * WN * KG * 64, 0, s>>>(a);
 }
 
 // The tile shapes, and which of them takes a call: the least of rounds x K tiles x time of a K tile. The times (us)
@@ -427,43 +445,63 @@ constexpr tile_cost kTiles16[] = {{256, 256, 1, 2.35, 2.70}, {128, 256, 1, 1.10,
 constexpr tile_cost kTiles4[] = {{256, 256, 1, 0.60, 0.95}, {128, 256, 1, 0.40, 0.62}, {128, 128, 2, 0.33, 0.62},
                                  {64, 128, 2, 0.23, 0.38},  {64, 64, 2, 0.18, 0.24}};
 
-template <int N> double tile_estimate(const tile_cost (&shapes)[N], int count, int64_t m, int64_t n, int64_t ktiles, int* best) {
+struct tile_choice {
+    int shape, splits;
+};
+// The first `count` shapes, and up to most_splits parts of the K tiles, whose fp32 sums a kernel more adds: that and
+// their way through memory take 8 us and more, which only a long K with few tiles gives back. Split / not, us: M = 64,
+// N 5120, K 17408 23.6 / 28.9; M = 48, N 4096, K 12288 15.6 / 19.9; but M = 200, N 4096, K 12288 26.7 / 21.2, and
+// M = 24, N 6144, K 4096 13.2 / 10.7.
+template <int N> tile_choice choose_tile(const tile_cost (&shapes)[N], int count, int64_t m, int64_t n, int64_t ktiles, int64_t most_splits) {
+    tile_choice best{0, 1};
     double least = 1e300;
     for (int i = 0; i < count; ++i) {
         const tile_cost& c = shapes[i];
         const int64_t tiles = ceil_div(m, c.rows) * ceil_div(n, c.cols), slots = int64_t{c.per_cu} * cu_count();
-        const double fill = std::min(1.0, static_cast<double>(tiles) / slots);
-        const double t = ceil_div(tiles, slots) * ktiles * (c.lone + (c.full - c.lone) * fill);
-        if (t < least) least = t, *best = i;
+        const int64_t most = std::max<int64_t>(1, std::min({most_splits, ktiles / 4, slots / tiles}));
+        for (int64_t splits = 1; splits <= most; ++splits) {
+            const int64_t each = ceil_div(ktiles, splits);
+            if (ceil_div(ktiles, each) != splits) continue;  // no part without a K tile
+            const double fill = std::min(1.0, static_cast<double>(tiles * splits) / slots);
+            const double t = ceil_div(tiles * splits, slots) * each * (c.lone + (c.full - c.lone) * fill) +
+                             (splits > 1 ? 8. + splits * m * n * 8 / 5.5e6 : 0.);
+            if (t < least) least = t, best = {i, static_cast<int>(splits)};
+        }
     }
-    return least;
+    return best;
+}
+// W4A4, plain: where N is not a multiple of 4, the sums are not whole quads.
+tile_choice choose_w4a4(int64_t m, int64_t n, int64_t k, bool may_split) {
+    return choose_tile(kTiles4, 5, m, n, ceil_div(k, kTileK), may_split && n % 4 == 0 ? 16 : 1);
 }
 
 template <bool A4, bool BF16, mx_epilogue EPI> void launch_shape(const mx_product& p, hipStream_t s) {
-    const int64_t n = p.n * (EPI == kMxPlain ? 1 : 2), ktiles = ceil_div(p.k, kTileK);
-    int shape = 0;
-    if constexpr (A4) tile_estimate(kTiles4, EPI == kMxGatedCodes ? 4 : 5, p.m, n, ktiles, &shape);  // a block is in one wavefront: NS = 4
-    else tile_estimate(kTiles16, 8, p.m, n, ktiles, &shape);
+    tile_choice c;
+    if constexpr (A4 && EPI == kMxPlain) c = choose_w4a4(p.m, p.n, p.k, p.partial != nullptr && p.out.wide);
+    else if constexpr (A4) c = choose_tile(kTiles4, 4, p.m, 2 * p.n, ceil_div(p.k, kTileK), 1);  // a block is in one wavefront: NS = 4
+    else c = choose_tile(kTiles16, 8, p.m, p.n * (EPI == kMxPlain ? 1 : 2), ceil_div(p.k, kTileK), 1);
+    const int shape = c.shape, splits = c.splits;
     if constexpr (A4) {
         switch (shape) {
-            case 0: return launch<A4, BF16, EPI, 2, 4, 8, 4, 4>(p, s);
-            case 1: return launch<A4, BF16, EPI, 2, 4, 4, 4, 6>(p, s);
-            case 2: return launch<A4, BF16, EPI, 2, 2, 4, 4, 4>(p, s);
-            case 3: return launch<A4, BF16, EPI, 2, 2, 2, 4, 6>(p, s);
+            case 0: launch<A4, BF16, EPI, 2, 4, 8, 4, 4>(p, splits, s); break;
+            case 1: launch<A4, BF16, EPI, 2, 4, 4, 4, 6>(p, splits, s); break;
+            case 2: launch<A4, BF16, EPI, 2, 2, 4, 4, 4>(p, splits, s); break;
+            case 3: launch<A4, BF16, EPI, 2, 2, 2, 4, 6>(p, splits, s); break;
             default:
-                if constexpr (EPI != kMxGatedCodes) return launch<A4, BF16, EPI, 2, 2, 2, 2, 4, 2>(p, s);
+                if constexpr (EPI != kMxGatedCodes) launch<A4, BF16, EPI, 2, 2, 2, 2, 4, 2>(p, splits, s);
         }
+        if (splits > 1) launch_mx_combine(p.bf16, p.partial, p.m * p.n, splits, p.out.y, s);
     } else {
         constexpr bool G = EPI == kMxGated;  // gate and up in one wavefront: an even number of strips
         switch (shape) {
-            case 0: return launch<A4, BF16, EPI, 2, 4, 8, 4, 2, 1, false>(p, s);
-            case 1: return launch<A4, BF16, EPI, 1, 8, 8, 2, 3>(p, s);
-            case 2: return launch<A4, BF16, EPI, 1, 4, 8, 2, 2, 1, false>(p, s);
-            case 3: return launch<A4, BF16, EPI, 2, 4, 4, 2, 3>(p, s);
-            case 4: return launch<A4, BF16, EPI, 1, 4, 4, 2, 3, 2>(p, s);
-            case 5: return launch<A4, BF16, EPI, 2, 2, 2, 2, 3, 2>(p, s);
-            case 6: return launch<A4, BF16, EPI, 2, 2, 1, 2, 3, 4>(p, s);
-            default: return launch<A4, BF16, EPI, G ? 2 : 1, G ? 2 : 4, G ? 1 : 2, G ? 2 : 1, 3, 2>(p, s);
+            case 0: return launch<A4, BF16, EPI, 2, 4, 8, 4, 2, 1, false>(p, splits, s);
+            case 1: return launch<A4, BF16, EPI, 1, 8, 8, 2, 3>(p, splits, s);
+            case 2: return launch<A4, BF16, EPI, 1, 4, 8, 2, 2, 1, false>(p, splits, s);
+            case 3: return launch<A4, BF16, EPI, 2, 4, 4, 2, 3>(p, splits, s);
+            case 4: return launch<A4, BF16, EPI, 1, 4, 4, 2, 3, 2>(p, splits, s);
+            case 5: return launch<A4, BF16, EPI, 2, 2, 2, 2, 3, 2>(p, splits, s);
+            case 6: return launch<A4, BF16, EPI, 2, 2, 1, 2, 3, 4>(p, splits, s);
+            default: return launch<A4, BF16, EPI, G ? 2 : 1, G ? 2 : 4, G ? 1 : 2, G ? 2 : 1, 3, 2>(p, splits, s);
         }
     }
 }

@@ -9,4 +9,10 @@ void launch_mx_tiles_w4a4(const mx_product& p, hipStream_t s) {
     else launch_shape<true, false, kMxPlain>(p, s);
 }
 
+// Workspace of the K splits' sums.
+int64_t mx_tiles_w4a4_bytes(int64_t m, int64_t n, int64_t k) {
+    const tile_choice c = choose_w4a4(m, n, k, true);
+    return c.splits > 1 ? c.splits * m * n * 4 : 0;
+}
+
 }  // namespace plm

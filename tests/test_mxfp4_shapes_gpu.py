@@ -73,12 +73,43 @@ def test_rows_gated_strips(m):
     mx.within(ops.gated_mxfp4_cuda(x, wg.packed, wu.packed, n), ref, err, "h")
 
 
-@pytest.mark.parametrize("m", [33, 64])
-@pytest.mark.parametrize("n", [48, 4200])
-def test_rows_long_k(m, n):
-    k = 8224
-    w, x = mx.Weight(n, k, seed=n), mx.rows(m, k, torch.bfloat16, seed=m)
-    mx.within(ops.gemm_mxfp4_w4a4_cuda(x, *w.packed, n), *mx.product(mx.rounded(x), w.dense), "W4A4")
+# K in parts whose sums a second kernel adds (N a multiple of 4), whole, and in parts of which the last is shorter.
+@BOTH
+@pytest.mark.parametrize("m,n,k", [(33, 48, 8224), (64, 4200, 8224), (33, 50, 8224), (48, 2052, 17408), (70, 100, 4128)])
+def test_k_split(m, n, k, dtype):
+    w, x = mx.Weight(n, k, seed=n), mx.rows(m, k, mx.DT[dtype], seed=m)
+    y = ops.gemm_mxfp4_w4a4_cuda(x, *w.packed, n)
+    mx.within(y, *mx.product(mx.rounded(x), w.dense), "W4A4")
+    assert torch.equal(y, ops.gemm_mxfp4_w4a4_cuda(x, *w.packed, n))
+    # Where y is not aligned for it, K is not split: another order of the sums.
+    room = torch.full((m * n + 8,), 7.0, dtype=x.dtype, device="cuda")
+    mx.within(ops.gemm_mxfp4_w4a4_cuda(x, *w.packed, n, out=room[1 : 1 + m * n].view(m, n)), *mx.product(mx.rounded(x), w.dense), "W4A4")
+    assert (room[0] == 7).all() and (room[1 + m * n :] == 7).all()
+
+
+def test_k_split_in_a_graph():
+    """Two captured graphs with scratch of their own, replayed in turn with eager work between them."""
+    n, k = 96, 8224
+    w = mx.Weight(n, k, seed=1)
+    xs = [mx.rows(m, k, torch.bfloat16, seed=m) for m in (40, 64)]
+    expected = [ops.gemm_mxfp4_w4a4_cuda(x, *w.packed, n) for x in xs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.gemm_mxfp4_w4a4_cuda(x, *w.packed, n))
+        graphs.append(g)
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        for g in graphs:
+            g.replay()
+        again = ops.gemm_mxfp4_w4a4_cuda(xs[0], *w.packed, n)
+        torch.cuda.synchronize()
+        for o, e in zip(outs, expected):
+            assert torch.equal(o, e)
+        assert torch.equal(again, expected[0])
 
 
 @pytest.mark.parametrize("m", [8, 40])
