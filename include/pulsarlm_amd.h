@@ -283,9 +283,10 @@ int plm_gemm_mxfp4(const void* x, plm_dtype x_dtype, const void* weight, const v
 
 /*
  * The same with x quantized by the rule of plm_quantize_mxfp4 (W4A4): both operands' codes and scales go to
- * the scaled matrix instruction. One token's x is quantized inside the product's kernel, longer ones' in a
- * launch of its own into the workspace (256-byte aligned; its contents need not be set and mean nothing
- * after the call).
+ * the scaled matrix instruction. A few tokens' x is quantized inside the product's kernel, more in a launch of
+ * their own into the workspace, which also holds the sums of a long K that is split over workgroups (256-byte
+ * aligned; its contents need not be set and mean nothing after the call). y of N % 4 == 0 that is not 8-byte
+ * aligned may be summed in another order.
  */
 int64_t plm_gemm_mxfp4_w4a4_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int plm_gemm_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* weight, const void* scale,

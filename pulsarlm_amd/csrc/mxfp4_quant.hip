@@ -1,5 +1,6 @@
 // MXFP4 quantizer, its inverse and the weights' repack. All stream: each value is read and written once,
-// so HBM bounds them (and a launch's latency, for one token).
+// so HBM bounds them (and a launch's latency, for one token). M = 4096, K 12288 in bf16: quantized in 23.4 us, 5.4 TB/s
+// (a copy of 2 GiB: 4.9-5.06); to the tile layout, M = 4096, K 4096, 9.8 us; one row of 4096 2.0 us.
 #include "mxfp4.hpp"
 
 namespace plm {

@@ -7,13 +7,15 @@
 // DW K tiles ahead in registers, nontemporal), so nothing is shared before the end and no barrier stands in
 // the K loop. K is not split over workgroups: 16-row strips alone give N / 16 of them, and with DW tiles in
 // flight per wavefront fewer than one workgroup to a CU already draw the memory's rate. x comes as:
-// * staged: all of x in LDS, where it is at most kStagedBytes (then two workgroups fit a CU). Rows past M
-//   are not stored, so their lanes read row M - 1 again. With 4-bit x the lane that holds a block's 32
+// * staged: all of x in LDS (`staged` says where). Rows past M are not stored, so their lanes read row M - 1 again. With 4-bit x the lane that holds a block's 32
 //   values quantizes them there: one launch, no scratch.
 // * a ring of two K tiles per wavefront, filled with loads to LDS.
 // * codes in the tile layout, straight to registers.
 // The weights are the matrix instruction's A operand and x its B operand, so that a lane ends with four
 // neighbouring columns of one row: 8-byte stores, and gate and up of a column in one lane.
+// One token, us (TB/s of weights), 16-bit x: N 6144, K 4096 5.6 (2.4; 4.9 of the kernel itself); N 4096, K 12288 8.0
+// (3.3); gate and up of 12288, K 4096 13.4 (4.0). A copy of 2 GiB makes 4.9-5.06 TB/s; the rest is the launch and the
+// first loads' latency, some 2.5 us.
 #include "mxfp4.hpp"
 
 namespace plm {
@@ -21,7 +23,6 @@ namespace plm {
 namespace {
 
 enum mx_x { kXStaged, kXStagedQuantize, kXRing, kXCodes };
-constexpr int64_t kStagedBytes = 64 * 1024;
 
 struct rows_args {
     const uint16_t* x;
@@ -248,7 +249,7 @@ template <int XM, bool BF16, int RB, int SG, mx_epilogue EPI> void launch(const 
     a.strips = static_cast<int>(d.strips);
     a.m_blocks = static_cast<int>(ceil_div(p.m, RB * 16));
     constexpr int NW = kWaves;
-    int64_t loop = 0;
+    int64_t loop = 0;  // bytes of LDS in the K loop
     if (XM == kXStaged || XM == kXStagedQuantize) loop = p.m * ceil_div(d.ktiles, 4) * 1024;
     if (XM == kXRing) loop = int64_t{NW} * 2 * RB * 4096;
     const int64_t lds = std::max<int64_t>(loop, int64_t{RB} * SG * NW * 1024);
@@ -276,14 +277,23 @@ template <int XM, bool BF16, int RB> void launch_sg(const mx_product& p, hipStre
     }
 }
 
-bool staged(const mx_product& p) { return p.m <= 16 && p.m * ceil_div(p.k, 512) * 1024 <= kStagedBytes; }
+int64_t all_strips(const mx_product& p) { return ceil_div(p.n, kTileN) * (p.epilogue == kMxPlain ? 1 : 2); }
+
+// x in LDS: up to 64 KiB, so that two workgroups fit a CU; up to 128 KiB where one does, if x is quantized there (a
+// launch less) or has at most 8 rows (the ring takes all 16). 128 / 64 KiB, us, quantized: M = 12, N 6144, K 4096
+// 7.6 / 8.5, N 2048 6.5 / 7.2, but M = 16, N 24576 17.7 / 16.7; 16-bit: M = 5, N 4096, K 12288 9.2 / 10.8, but M = 12,
+// N 2048, K 4096 5.3 / 4.9 and N 24576 16.4 / 14.5.
+bool staged(const mx_product& p, bool quantize_x) {
+    const bool more = all_strips(p) <= 2 * cu_count() && (quantize_x || p.m <= 8);
+    return p.m <= 16 && p.m * ceil_div(p.k, 512) * 1024 <= (more ? 128 : 64) * 1024;
+}
 
 template <bool BF16> void launch_typed(const mx_product& p, bool quantize_x, hipStream_t s) {
     if (quantize_x) return launch_sg<kXStagedQuantize, BF16, 1>(p, s);
     if (p.xq.codes != nullptr) {
         if (p.m <= 16) launch_sg<kXCodes, BF16, 1>(p, s);
         else launch_sg<kXCodes, BF16, 2>(p, s);
-    } else if (staged(p)) launch_sg<kXStaged, BF16, 1>(p, s);
+    } else if (staged(p, false)) launch_sg<kXStaged, BF16, 1>(p, s);
     else if (p.m <= 16) launch_sg<kXRing, BF16, 1>(p, s);
     else launch_sg<kXRing, BF16, 2>(p, s);
 }
@@ -295,10 +305,10 @@ template <bool BF16> void launch_typed(const mx_product& p, bool quantize_x, hip
 // x as codes, M = 32: 7.1, 7.6; 9.8, 10.7; 14.7, 19.0; 18.1, 16.2 (M = 16 16.5, 15.1); M = 64: 8.9, 8.3; 12.3, 11.7;
 // K 12288 18.6, 17.1 (the tiles' K split).
 bool launch_mx_rows(const mx_product& p, bool quantize_x, hipStream_t s) {
-    const int64_t strips = ceil_div(p.n, kTileN) * (p.epilogue == kMxPlain ? 1 : 2), cus = cu_count();
+    const int64_t strips = all_strips(p), cus = cu_count();
     const bool codes = p.xq.codes != nullptr;
     if (quantize_x) {
-        if (!staged(p)) return false;
+        if (!staged(p, true)) return false;
     } else if (strips > 4 * cus) {
         if (p.m > (codes ? 8 : 16)) return false;
     } else if (p.m > 32) {
