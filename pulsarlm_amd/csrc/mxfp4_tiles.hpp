@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(WM * WN * KG * 64) mx_tile_kernel(tile_args a)
     constexpr int STAGE = (XC + BS) * 1024 + (SL ? SCC * 256 : 0);
     constexpr int LOADS = (XC + BS) / NW + SCL;
     constexpr int SLICES = A4 ? 1 : 4;
-    static_assert((MT & (MT - 1)) == 0 && (NS & (NS - 1)) == 0 && (!A4 || WM % 2 == 0), "a wavefront's strips lie in whole groups, or in one");
+    static_assert((NS & (NS - 1)) == 0 && (!A4 || ((MT & (MT - 1)) == 0 && WM % 2 == 0)), "a wavefront's strips lie in whole groups, or in one");
     static_assert(XC % NW == 0 && BS % NW == 0, "every wavefront loads as many chunks");
     static_assert(EPI == kMxPlain || NS % 2 == 0, "gate and up in one wavefront");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S * KG * STAGE];
@@ -435,12 +435,14 @@ template <bool A4, bool BF16, mx_epilogue EPI, int WM, int WN, int MT, int NS, i
 
 // The tile shapes, and which of them takes a call: the least of rounds x K tiles x time of a K tile. The times (us)
 // were measured with one workgroup on the GPU and with every slot taken; between the two they grow with the
-// share of slots taken, as the workgroups share the L2s and the clock. {rows, columns, workgroups a CU, lone, full}
+// share of slots taken, as the workgroups share the L2s and the clock. 192 rows are there for what 128 and 256 waste:
+// M = 333, N 24576, K 4096 70 us with them and 87 without; gate and up of 4864, K 2080, M = 1001 45 and 54.
+// {rows, columns, workgroups a CU, lone, full}
 struct tile_cost {
     int rows, cols, per_cu;
     double lone, full;
 };
-constexpr tile_cost kTiles16[] = {{256, 256, 1, 2.35, 2.70}, {128, 256, 1, 1.10, 1.50}, {128, 128, 2, 1.20, 1.70}, {128, 128, 1, 0.69, 0.95},
+constexpr tile_cost kTiles16[] = {{256, 256, 1, 2.35, 2.70}, {192, 256, 1, 1.61, 2.03}, {128, 256, 1, 1.10, 1.50}, {128, 128, 2, 1.20, 1.70}, {128, 128, 1, 0.69, 0.95},
                                   {64, 128, 1, 0.36, 0.52},  {64, 64, 1, 0.29, 0.36},   {32, 64, 1, 0.18, 0.27},   {32, 64, 2, 0.20, 0.38}};
 constexpr tile_cost kTiles4[] = {{256, 256, 1, 0.60, 0.95}, {128, 256, 1, 0.40, 0.62}, {128, 128, 2, 0.33, 0.62},
                                  {64, 128, 2, 0.23, 0.38},  {64, 64, 2, 0.18, 0.24}};
@@ -479,7 +481,7 @@ template <bool A4, bool BF16, mx_epilogue EPI> void launch_shape(const mx_produc
     tile_choice c;
     if constexpr (A4 && EPI == kMxPlain) c = choose_w4a4(p.m, p.n, p.k, p.partial != nullptr && p.out.wide);
     else if constexpr (A4) c = choose_tile(kTiles4, 4, p.m, 2 * p.n, ceil_div(p.k, kTileK), 1);  // a block is in one wavefront: NS = 4
-    else c = choose_tile(kTiles16, 8, p.m, p.n * (EPI == kMxPlain ? 1 : 2), ceil_div(p.k, kTileK), 1);
+    else c = choose_tile(kTiles16, 9, p.m, p.n * (EPI == kMxPlain ? 1 : 2), ceil_div(p.k, kTileK), 1);
     const int shape = c.shape, splits = c.splits;
     if constexpr (A4) {
         switch (shape) {
@@ -495,12 +497,13 @@ template <bool A4, bool BF16, mx_epilogue EPI> void launch_shape(const mx_produc
         constexpr bool G = EPI == kMxGated;  // gate and up in one wavefront: an even number of strips
         switch (shape) {
             case 0: return launch<A4, BF16, EPI, 2, 4, 8, 4, 2, 1, false>(p, splits, s);
-            case 1: return launch<A4, BF16, EPI, 1, 8, 8, 2, 3>(p, splits, s);
-            case 2: return launch<A4, BF16, EPI, 1, 4, 8, 2, 2, 1, false>(p, splits, s);
-            case 3: return launch<A4, BF16, EPI, 2, 4, 4, 2, 3>(p, splits, s);
-            case 4: return launch<A4, BF16, EPI, 1, 4, 4, 2, 3, 2>(p, splits, s);
-            case 5: return launch<A4, BF16, EPI, 2, 2, 2, 2, 3, 2>(p, splits, s);
-            case 6: return launch<A4, BF16, EPI, 2, 2, 1, 2, 3, 4>(p, splits, s);
+            case 1: return launch<A4, BF16, EPI, 2, 4, 6, 4, 2>(p, splits, s);
+            case 2: return launch<A4, BF16, EPI, 1, 8, 8, 2, 3>(p, splits, s);
+            case 3: return launch<A4, BF16, EPI, 1, 4, 8, 2, 2, 1, false>(p, splits, s);
+            case 4: return launch<A4, BF16, EPI, 2, 4, 4, 2, 3>(p, splits, s);
+            case 5: return launch<A4, BF16, EPI, 1, 4, 4, 2, 3, 2>(p, splits, s);
+            case 6: return launch<A4, BF16, EPI, 2, 2, 2, 2, 3, 2>(p, splits, s);
+            case 7: return launch<A4, BF16, EPI, 2, 2, 1, 2, 3, 4>(p, splits, s);
             default: return launch<A4, BF16, EPI, G ? 2 : 1, G ? 2 : 4, G ? 1 : 2, G ? 2 : 1, 3, 2>(p, splits, s);
         }
     }

@@ -15,7 +15,7 @@ K = 1184  # ten K tiles, the last one a quarter full: turns of every stage count
 
 # Every tile shape with 16-bit x, once where whole rows leave and once where they cannot.
 TILES_W4A16 = [(33, 33), (33, 8), (4125, 65), (4125, 104), (4125, 200), (3288, 264), (3381, 200), (2668, 264), (3629, 513), (3629, 520),
-               (3598, 1034), (3598, 1032), (3598, 2050), (3598, 2056), (3846, 2050), (3846, 2056)]
+               (3598, 1034), (3598, 1032), (3598, 2050), (3598, 2056), (3846, 2050), (3846, 2056), (1924, 6100), (1924, 6104)]
 
 
 @BOTH
@@ -34,7 +34,8 @@ def test_tiles_w4a4(m, n, dtype):
 
 
 @BOTH
-@pytest.mark.parametrize("m,n", [(33, 8), (4125, 40), (3381, 104), (4125, 104), (3629, 264), (3598, 521), (3598, 1032), (3846, 1030)])
+@pytest.mark.parametrize("m,n", [(33, 8), (4125, 40), (3381, 104), (4125, 104), (3629, 264), (3598, 521), (3598, 1032), (3846, 1030),
+                                 (281, 12200), (405, 12202)])
 def test_tiles_gated(m, n, dtype):
     wg, wu, x = mx.Weight(n, K, seed=n), mx.Weight(n, K, seed=n + 1), mx.rows(m, K, mx.DT[dtype], seed=m)
     ref, err, _, _ = mx.gated(x.double(), wg.dense, wu.dense)
