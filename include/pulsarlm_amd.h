@@ -274,8 +274,9 @@ int plm_repack_mxfp4(const uint8_t* codes, const uint8_t* scale, int64_t n, int6
                      void* scale_out, void* stream);
 
 /*
- * y [M, N] = x [M, K] @ W^T in x_dtype (PLM_BF16 or PLM_FP16), W the repacked MXFP4 weight in x_dtype (exact
- * in bf16, rounded once to fp16), fp32 sums. M at most 2^24, M N and M K at most 2^36. M == 0 or N == 0 returns PLM_OK
+ * y [M, N] = x [M, K] @ W^T in x_dtype (PLM_BF16 or PLM_FP16), W the repacked MXFP4 weight in x_dtype (rounded
+ * once to fp16; exact in bf16 up to b = 252, the largest that finite values are quantized to, beyond which the
+ * largest codes overflow), fp32 sums. y may not overlap x. M at most 2^24, M N and M K at most 2^36. M == 0 or N == 0 returns PLM_OK
  * without touching y; K == 0 sets y to zero. No workspace.
  */
 int plm_gemm_mxfp4(const void* x, plm_dtype x_dtype, const void* weight, const void* scale,

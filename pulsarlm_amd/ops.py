@@ -488,7 +488,7 @@ def _mx_x(op: str, x: torch.Tensor):
 
 
 def gemm_mxfp4_cuda(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, n: int, out=None) -> torch.Tensor:
-    """y [M, N] = x [M, K] @ W^T with an MXFP4 weight (repack_mxfp4_cuda) and 16-bit x, fp32 sums."""
+    """y [M, N] = x [M, K] @ W^T with an MXFP4 weight (repack_mxfp4_cuda) and 16-bit x, fp32 sums. out may not overlap x."""
     op = "gemm_mxfp4"
     m, k = _mx_x(op, x)
     _mx_weight(op, x, weight, scale, n, k)

@@ -1,6 +1,7 @@
 """The MXFP4 products at sizes that take each of their kernels' shapes (on 256 CUs), unaligned outputs, operands
 that are not contiguous, work on two streams at once, and what the Python layer refuses."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -166,6 +167,21 @@ def test_plain_weights_need_not_be_contiguous():
         for a, b in zip(ops.repack_mxfp4_cuda(*views), w.packed):
             assert torch.equal(a, b)
         assert torch.equal(ops.dequantize_mxfp4_cuda(*views, torch.float32).double(), w.dense)
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+@pytest.mark.parametrize("lowest,power", [(0, 100), (249, -60)])
+def test_smallest_and_largest_scales(lowest, power, m):
+    """Weights that are subnormal in bf16, and ones at its upper end."""
+    n, k = 48, 288
+    w = mx.Weight(n, k, seed=1)
+    byte = np.random.default_rng(2).integers(lowest, lowest + 4, w.byte.shape, dtype=np.uint8)
+    dense = torch.from_numpy(mx.values(w.code, byte)).cuda()
+    packed = ops.repack_mxfp4_cuda(w.plain[0], torch.from_numpy(byte).cuda())
+    x, dy = (torch.ldexp(mx.rows(m, c, torch.bfloat16, seed=c).double(), torch.tensor(power)).to(torch.bfloat16) for c in (k, n))
+    mx.within(ops.gemm_mxfp4_cuda(x, *packed, n), *mx.product(x.double(), dense), "W4A16")
+    mx.within(ops.gemm_mxfp4_w4a4_cuda(x, *packed, n), *mx.product(mx.rounded(x), dense), "W4A4")
+    mx.within(ops.gemm_mxfp4_grad_cuda(dy, *packed, k), *mx.product(dy.double(), dense.t()), "dx")
 
 
 def test_two_streams_at_once():
