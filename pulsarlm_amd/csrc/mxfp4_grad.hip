@@ -34,6 +34,7 @@ struct grad_args {
     int m, k, ktiles, strips;
     int side_steps, steps, split_steps, splits;
     int m_blocks, n_blocks;
+    const float* row_scale;  // fp16 factors: what row m's sums are to be multiplied by; or null
 };
 
 typedef __attribute__((ext_vector_type(4))) short tr_t;
@@ -171,11 +172,15 @@ __global__ void __launch_bounds__(512) mx_grad_kernel(grad_args a) {
         const int r = (wm * MT + i) * 16 + col16;
         if (r >= rows) continue;
         const int64_t row = row0 + r;
+        float scale = 1.f;
+        if constexpr (!BF16)
+            if (a.row_scale != nullptr) scale = a.row_scale[row];
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
             const int col = nb * kGradCols + (wn * NS + j) * 16 + 4 * kq;  // K is a multiple of 32
             if (col >= a.k) continue;
-            const f32x4_t v = acc[i][j];
+            f32x4_t v = acc[i][j];
+            if constexpr (!BF16) v = f32x4_t{v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
             if (a.splits > 1) *reinterpret_cast<f32x4_t*>(a.partial + (static_cast<int64_t>(split) * a.m + row) * a.k + col) = v;
             else *reinterpret_cast<uint2*>(a.dx + row * a.k + col) = make_uint2(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]));
         }
@@ -193,9 +198,51 @@ __global__ void __launch_bounds__(256) mx_combine_kernel(const f32x4_t* __restri
     dx[i] = make_uint2(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]));
 }
 
+// Eight values of a row from column col on, zeros past n. WIDE: rows of whole 16-byte pieces.
+template <bool WIDE> __device__ __forceinline__ void row_load8(const uint16_t* p, int col, int n, uint32_t (&v)[8]) {
+    if (WIDE && col < n) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p + col);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = w[i] & 0xffffu, v[2 * i + 1] = w[i] >> 16;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = col + i < n ? p[col + i] : 0u;
+    }
+}
+template <bool WIDE> __device__ __forceinline__ void row_load8(const float* p, int col, int n, float (&v)[8]) {
+    if (WIDE && col < n) {
+        const f32x4_t a = reinterpret_cast<const f32x4_t*>(p + col)[0], b = reinterpret_cast<const f32x4_t*>(p + col)[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = col + i < n ? p[col + i] : 0.f;
+    }
+}
+__device__ __forceinline__ void row_store8(uint16_t* p, const uint32_t (&v)[8]) {
+    *reinterpret_cast<u32x4_t*>(p) = u32x4_t{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+}
+// Eight columns of one row's factors in fp32: with s = sigmoid(g), d gate = dh u s (1 + g (1 - s)), d up = dh g s.
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ void row_factors8(const uint16_t* dh, const float* gate_up, int col, int n, float (&dg)[8], float (&du)[8]) {
+    uint32_t d[8];
+    float g[8], u[8];
+    row_load8<WIDE>(dh, col, n, d);
+    row_load8<WIDE>(gate_up, col, n, g);
+    row_load8<WIDE>(gate_up + n, col, n, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = from_bits16<BF16>(d[i]), s = mx_sigmoid(g[i]);
+        dg[i] = f * u[i] * s * (1.f + g[i] * (1.f - s));
+        du[i] = f * g[i] * s;
+    }
+}
+
 // The gated block's [d gate | d up], each padded with zeros to a whole step, rounded to the matrix
-// instruction's 16 bits: with s = sigmoid(g), d gate = dh u s (1 + g (1 - s)), d up = dh g s.
-// !GATED: a copy of dy padded so. Eight values a thread; WIDE: rows of whole 16-byte pieces.
+// instruction's 16 bits. !GATED: a copy of dy padded so. Eight values a thread.
+// bf16 holds every factor that fp32 does, to 8 bits: dx is off by 2.3e-3 of its size against float64 with them and by 1.7e-3
+// with factors in fp32 (its own rounding). Two bf16 terms a factor would give that, but are the products of twice the
+// rows: N 9728, K 2080 57 us at M = 1001 and 96 at 2002; N 24576, K 4096 620 at M = 4096 and 1320 at 8192.
 template <bool BF16, bool GATED, bool WIDE>
 __global__ void __launch_bounds__(256) mx_grad_rows_kernel(const uint16_t* __restrict__ dy, const float* __restrict__ gate_up,
                                                            int64_t m, int n, int padded, uint16_t* __restrict__ out) {
@@ -204,47 +251,87 @@ __global__ void __launch_bounds__(256) mx_grad_rows_kernel(const uint16_t* __res
     for (int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; c < total; c += step) {
         const int64_t row = c / per_row;
         const int col = static_cast<int>(c % per_row) * 8;
-        auto load8 = [&](const uint16_t* p, uint32_t (&v)[8]) {
-            if (WIDE && col < n) {
-                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p + col);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[2 * i] = w[i] & 0xffffu, v[2 * i + 1] = w[i] >> 16;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = col + i < n ? p[col + i] : 0u;
-            }
-        };
-        auto store8 = [&](uint16_t* p, const uint32_t (&v)[8]) {
-            *reinterpret_cast<u32x4_t*>(p) = u32x4_t{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
-        };
         uint32_t d[8];
-        load8(dy + row * n, d);
         if constexpr (!GATED) {
-            store8(out + row * padded + col, d);
+            row_load8<WIDE>(dy + row * n, col, n, d);
+            row_store8(out + row * padded + col, d);
         } else {
-            auto load8f = [&](const float* p, float (&v)[8]) {
-                if (WIDE && col < n) {
-                    const f32x4_t a = reinterpret_cast<const f32x4_t*>(p + col)[0], b = reinterpret_cast<const f32x4_t*>(p + col)[1];
+            float dg[8], du[8];
+            row_factors8<BF16, WIDE>(dy + row * n, gate_up + row * 2 * n, col, n, dg, du);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-                } else {
+            for (int i = 0; i < 8; ++i) d[i] = to_bits16<BF16>(dg[i]);
+            row_store8(out + row * 2 * padded + col, d);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = col + i < n ? p[col + i] : 0.f;
-                }
-            };
-            float g[8], u[8];
-            uint32_t dg[8], du[8];
-            load8f(gate_up + row * 2 * n, g);
-            load8f(gate_up + row * 2 * n + n, u);
+            for (int i = 0; i < 8; ++i) d[i] = to_bits16<BF16>(du[i]);
+            row_store8(out + row * 2 * padded + padded + col, d);
+        }
+    }
+}
+
+// The factors in fp16. They pass its range at both ends where dx does not (dh of 100 by u of 1000; dh of 1e-5 by u of
+// 1e-3), so each row is brought by a power of two to a largest factor in [2^14, 2^15), and its sums are multiplied by
+// the inverse, row_scale, when they leave. Infinity and NaN do not count for that: they come through as such.
+// A workgroup a row. The first kHeld pieces of eight columns a thread wait in registers for the row's largest; what is
+// past them (N over 12288) is computed again, its reads mostly from the L2. M = 4096, N 12288: 127 us, the bf16 kernel 118.
+constexpr int kRowThreads = 512, kHeld = 3;
+template <bool WIDE>
+__global__ void __launch_bounds__(kRowThreads) mx_grad_rows_fp16_kernel(const uint16_t* __restrict__ dh, const float* __restrict__ gate_up,
+                                                                        int64_t m, int n, int padded, uint16_t* __restrict__ out,
+                                                                        float* __restrict__ row_scale) {
+    constexpr int kStep = kRowThreads * 8;
+    __shared__ uint32_t tops[kRowThreads / 64];
+    for (int64_t row = blockIdx.x; row < m; row += gridDim.x) {
+        const uint16_t* d = dh + row * n;
+        const float* gu = gate_up + row * 2 * n;
+        uint16_t* to = out + row * 2 * padded;
+        uint32_t top = 0;
+        auto count = [&](const float (&dg)[8], const float (&du)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float dh = from_bits16<BF16>(d[i]), gf = g[i], uf = u[i];
-                const float s = mx_sigmoid(gf);
-                dg[i] = to_bits16<BF16>(dh * uf * s * (1.f + gf * (1.f - s)));
-                du[i] = to_bits16<BF16>(dh * gf * s);
+                const uint32_t a = mx_magnitude(dg[i]), b = mx_magnitude(du[i]);
+                top = max(top, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
             }
-            store8(out + row * 2 * padded + col, dg);
-            store8(out + row * 2 * padded + padded + col, du);
+        };
+        const int first = threadIdx.x * 8;
+        float hg[kHeld][8], hu[kHeld][8];
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h)
+            if (first + h * kStep < padded) row_factors8<false, WIDE>(d, gu, first + h * kStep, n, hg[h], hu[h]);
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h)
+            if (first + h * kStep < padded) count(hg[h], hu[h]);
+        float dg[8], du[8];
+        for (int col = first + kHeld * kStep; col < n; col += kStep) {
+            row_factors8<false, WIDE>(d, gu, col, n, dg, du);
+            count(dg, du);
+        }
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), s)));
+        __syncthreads();  // the last row's are read
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kRowThreads / 64; ++w) top = max(top, tops[w]);
+        // 2^(141 - e) brings 2^(e - 127) to 2^14. Rows below 2^-86 (zeros among them) take that one's: |W| <= 65504 and N <=
+        // 2^19, so their dx is zero in fp16 whatever the factors are.
+        const uint32_t e = max(top >> 23, 41u);
+        const float up = __uint_as_float((127u + 141u - e) << 23);
+        if (threadIdx.x == 0) row_scale[row] = __uint_as_float((e - 14u) << 23);
+        auto store = [&](int col, const float (&dg)[8], const float (&du)[8]) {
+            uint32_t v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_bits16<false>(dg[i] * up);
+            row_store8(to + col, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_bits16<false>(du[i] * up);
+            row_store8(to + padded + col, v);
+        };
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h)
+            if (first + h * kStep < padded) store(first + h * kStep, hg[h], hu[h]);
+        for (int col = first + kHeld * kStep; col < padded; col += kStep) {
+            row_factors8<false, WIDE>(d, gu, col, n, dg, du);
+            store(col, dg, du);
         }
     }
 }
@@ -283,22 +370,30 @@ grad_plan make_grad_plan(int64_t m, int64_t k, int64_t steps) {
 int64_t padded_n(int64_t n) { return round_up(n, kGradStep); }
 bool copies_dy(const void* dy, int64_t n) { return n % kGradStep != 0 || !aligned(dy, 16); }
 
-// Workspace: [rows in 16 bits][fp32 partial sums].
+// Workspace: [rows in 16 bits][gated: a scale a row][fp32 partial sums].
 int64_t rows_bytes(int64_t m, int64_t n, int sides) { return round_up(m * sides * padded_n(n) * 2, 256); }
+int64_t row_scale_bytes(int64_t m, int sides) { return sides == 2 ? round_up(m * 4, 256) : 0; }
 int64_t grad_bytes(int64_t m, int64_t n, int64_t k, int sides) {
     const grad_plan p = make_grad_plan(m, k, sides * padded_n(n) / kGradStep);
-    return rows_bytes(m, n, sides) + (p.splits > 1 ? p.splits * m * k * 4 : 0);
+    return rows_bytes(m, n, sides) + row_scale_bytes(m, sides) + (p.splits > 1 ? p.splits * m * k * 4 : 0);
 }
 
 template <bool BF16, bool GATED>
-void launch_rows(const void* dy, const void* gate_up, int64_t m, int64_t n, uint16_t* out, hipStream_t s) {
-    const int64_t padded = padded_n(n);
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(m * padded / 8, 256), int64_t{64} * cu_count()));
+void launch_rows(const void* dy, const void* gate_up, int64_t m, int64_t n, uint16_t* out, float* row_scale, hipStream_t s) {
+    const int64_t padded = padded_n(n), most = int64_t{64} * cu_count();
+    const int nn = static_cast<int>(n), pn = static_cast<int>(padded);
     const auto* d = static_cast<const uint16_t*>(dy);
     const auto* g = static_cast<const float*>(gate_up);
-    if (n % 8 == 0 && aligned(dy, 16) && aligned(gate_up, 16))
-        mx_grad_rows_kernel<BF16, GATED, true><<<grid, 256, 0, s>>>(d, g, m, static_cast<int>(n), static_cast<int>(padded), out);
-    else mx_grad_rows_kernel<BF16, GATED, false><<<grid, 256, 0, s>>>(d, g, m, static_cast<int>(n), static_cast<int>(padded), out);
+    const bool wide = n % 8 == 0 && aligned(dy, 16) && aligned(gate_up, 16);
+    if constexpr (GATED && !BF16) {
+        const unsigned grid = static_cast<unsigned>(std::min(m, most));
+        if (wide) mx_grad_rows_fp16_kernel<true><<<grid, kRowThreads, 0, s>>>(d, g, m, nn, pn, out, row_scale);
+        else mx_grad_rows_fp16_kernel<false><<<grid, kRowThreads, 0, s>>>(d, g, m, nn, pn, out, row_scale);
+    } else {
+        const unsigned grid = static_cast<unsigned>(std::min(ceil_div(m * padded / 8, 256), most));
+        if (wide) mx_grad_rows_kernel<BF16, GATED, true><<<grid, 256, 0, s>>>(d, g, m, nn, pn, out);
+        else mx_grad_rows_kernel<BF16, GATED, false><<<grid, 256, 0, s>>>(d, g, m, nn, pn, out);
+    }
 }
 
 template <bool BF16>
@@ -311,8 +406,10 @@ int run(const char* op, bool gated, const void* dy, const void* gate_up, const m
     a.dy = static_cast<const uint16_t*>(dy);
     a.pitch = n;
     if (gated || copies_dy(dy, n)) {
-        if (gated) launch_rows<BF16, true>(dy, gate_up, m, n, rows, s);
-        else launch_rows<BF16, false>(dy, nullptr, m, n, rows, s);
+        auto* row_scale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + rows_bytes(m, n, sides));
+        if (gated) launch_rows<BF16, true>(dy, gate_up, m, n, rows, row_scale, s);
+        else launch_rows<BF16, false>(dy, nullptr, m, n, rows, nullptr, s);
+        if (gated && !BF16) a.row_scale = row_scale;
         PLM_HIP_LAUNCH_CHECK(op);
         a.dy = rows;
         a.pitch = sides * padded_n(n);
@@ -322,7 +419,7 @@ int run(const char* op, bool gated, const void* dy, const void* gate_up, const m
     a.w0 = w0;
     a.w1 = w1;
     a.dx = static_cast<uint16_t*>(dx);
-    a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + rows_bytes(m, n, sides));
+    a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + rows_bytes(m, n, sides) + row_scale_bytes(m, sides));
     a.m = static_cast<int>(m);
     a.k = static_cast<int>(k);
     a.ktiles = static_cast<int>(d.ktiles);

@@ -1,0 +1,77 @@
+"""The MXFP4 operators in training, where the 16-bit type's range or a term of the gradient could get lost."""
+
+import pytest
+import torch
+
+from pulsarlm_amd import ops
+from tests import _mxfp4 as mx
+
+pytestmark = pytest.mark.gpu
+
+
+def shifted(n, k, seed, power):
+    """A random weight times 2^power: (dense float64, packed)."""
+    w = mx.Weight(n, k, seed=seed)
+    return torch.ldexp(w.dense, torch.tensor(power)), ops.repack_mxfp4_cuda(w.plain[0], w.plain[1] + power)
+
+
+def fp16_gradient(dh, gate_up, wg, wu):
+    """(dx, bound) in float64. A factor is rounded to 11 bits of its own or, below 2^-14 of its row's largest in [2^14, 2^15),
+    to fp16's subnormal steps: half a step is 2^-25 there, 2^-39 of the row's largest. Its own arithmetic is off by a
+    few 2^-23 of the terms' magnitude (|1 + g (1 - s)| <= 1 + |g|)."""
+    n = dh.shape[1]
+    d, g, u = dh.double(), gate_up[:, :n].double(), gate_up[:, n:].double()
+    dg, du = mx.gated_factors(d, g, u)
+    top = torch.maximum(dg.abs().amax(dim=1), du.abs().amax(dim=1))[:, None]
+    own = [mx.half(torch.float16) * f.abs() + 2.0**-39 * top + 2.0**-19 * d.abs() * v * (1 + g.abs()) for f, v in ((dg, u.abs()), (du, 1.0))]
+    err = sum(e @ w.abs() + (2 * n + 8) * 2.0**-23 * ((f.abs() + e) @ w.abs()) for e, f, w in zip(own, (dg, du), (wg, wu)))
+    return dg @ wg + du @ wu, err, top
+
+
+# Rows of one and several tiles, unsplit and split sums, N of whole 16-byte pieces and not, and past what a workgroup holds.
+FACTORS = [(1, 96, 160), (3, 4096, 160), (70, 33, 96), (300, 520, 1056), (2100, 264, 288), (2, 12331, 96), (5, 16504, 96)]
+
+
+@pytest.mark.parametrize("m,n,k", FACTORS)
+def test_fp16_factors_beyond_the_type(m, n, k):
+    """dh u s (1 + g (1 - s)) passes 65504 where dx, through small weights, is an ordinary number."""
+    (dg, pg), (du, pu) = shifted(n, k, 1, -9), shifted(n, k, 2, -9)
+    r = torch.Generator("cuda").manual_seed(m)
+    dh = (64 * torch.randn(m, n, generator=r, device="cuda")).half()
+    gate_up = torch.randn(m, 2 * n, generator=r, device="cuda") * torch.tensor([3.0, 3000.0], device="cuda").repeat_interleave(n)
+    ref, err, top = fp16_gradient(dh, gate_up, dg, du)
+    assert (top > 65504).all() and (ref.abs() + err < 65504).all()
+    mx.within(ops.gated_mxfp4_grad_cuda(dh, gate_up, pg, pu, k), ref, err, "dx")
+
+
+@pytest.mark.parametrize("m,n,k", FACTORS)
+def test_fp16_factors_below_the_type(m, n, k):
+    """Factors among fp16's subnormals, whose dx through large weights is not."""
+    (dg, pg), (du, pu) = shifted(n, k, 1, 10), shifted(n, k, 2, 10)
+    r = torch.Generator("cuda").manual_seed(m)
+    dh = (2.0**-12 * torch.randn(m, n, generator=r, device="cuda")).half()
+    gate_up = 2.0**-8 * torch.randn(m, 2 * n, generator=r, device="cuda")
+    ref, err, top = fp16_gradient(dh, gate_up, dg, du)
+    assert (top < 2.0**-14).all()
+    mx.within(ops.gated_mxfp4_grad_cuda(dh, gate_up, pg, pu, k), ref, err, "dx")
+
+
+def test_fp16_factors_of_every_row_apart():
+    """Rows of very different size, of zeros, and with infinity and NaN, in one call: each as if it were alone."""
+    m, n, k = 40, 96, 160
+    (dg, pg), (du, pu) = shifted(n, k, 1, -9), shifted(n, k, 2, -9)
+    r = torch.Generator("cuda").manual_seed(3)
+    power = torch.arange(m, device="cuda") % 20 - 10.0
+    dh = (torch.randn(m, n, generator=r, device="cuda") * torch.exp2(power)[:, None]).half()
+    dh[7] = 0
+    gate_up = torch.randn(m, 2 * n, generator=r, device="cuda") * torch.exp2(power)[:, None]
+    dh[11, 5], gate_up[13, n + 3], gate_up[17, 2] = float("nan"), float("inf"), float("nan")
+    odd = torch.tensor([11, 13, 17], device="cuda")
+    dx = ops.gated_mxfp4_grad_cuda(dh, gate_up, pg, pu, k)
+    assert not dx[7].any() and not dx[odd].isfinite().any()
+    rest = torch.tensor([i for i in range(m) if i not in (11, 13, 17)], device="cuda")
+    ref, err, _ = fp16_gradient(dh[rest], gate_up[rest], dg, du)
+    mx.within(dx[rest], ref, err, "dx")
+    for i in range(m):
+        alone = ops.gated_mxfp4_grad_cuda(dh[i : i + 1], gate_up[i : i + 1], pg, pu, k)
+        assert torch.equal(alone.view(torch.int16), dx[i : i + 1].view(torch.int16)) or i in (11, 13, 17)
