@@ -287,7 +287,7 @@ int plm_gemm_mxfp4(const void* x, plm_dtype x_dtype, const void* weight, const v
  * the scaled matrix instruction. A few tokens' x is quantized inside the product's kernel, more in a launch of
  * their own into the workspace, which also holds the sums of a long K that is split over workgroups (256-byte
  * aligned; its contents need not be set and mean nothing after the call). y of N % 4 == 0 that is not 8-byte
- * aligned may be summed in another order.
+ * aligned may be summed in another order. The workspace queries give 0 for sizes that need none or are refused.
  */
 int64_t plm_gemm_mxfp4_w4a4_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int plm_gemm_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* weight, const void* scale,

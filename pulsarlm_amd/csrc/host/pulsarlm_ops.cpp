@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <string>
@@ -387,6 +388,7 @@ at::Tensor dequantize_mxfp4_cuda(const at::Tensor& codes, const at::Tensor& scal
 
 std::tuple<at::Tensor, at::Tensor> repack_mxfp4_cuda(const at::Tensor& codes, const at::Tensor& scale) {
     const auto [n, k] = mx_plain("repack_mxfp4", codes, scale);
+    TORCH_CHECK(std::max(n, k) <= int64_t{1} << 19, "repack_mxfp4: N and K must be at most 2^19");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
     const at::Tensor c = codes.contiguous(), s = scale.contiguous();
     at::Tensor weight = at::empty({plm_mxfp4_weight_bytes(n, k) / 4}, codes.options().dtype(at::kInt));

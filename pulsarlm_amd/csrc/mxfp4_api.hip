@@ -18,13 +18,17 @@ mx_matrix matrix(const void* codes, const void* scale) {
     return {static_cast<const uint8_t*>(codes), static_cast<const uint32_t*>(scale)};
 }
 
+// A grid of at most 2^32 work-items, and offsets of one workgroup below kOOB.
+bool takes_rows(int64_t m, int64_t n, int64_t k) { return m <= (int64_t{1} << 24) && m * std::max(n, k) <= (int64_t{1} << 36); }
+bool takes(int64_t m, int64_t n, int64_t k) { return n <= kMxMaxSize && k <= kMxMaxSize && takes_rows(m, n, k); }
+// What a workspace query counts: sizes that a call takes, and works on.
+bool counts(int64_t m, int64_t n, int64_t k) { return m > 0 && n > 0 && k > 0 && takes(m, n, k); }
 int check_sizes(const char* op, plm_dtype x_dtype, int64_t m, int64_t n, int64_t k) {
     PLM_CHECK_ARG(x_dtype == PLM_BF16 || x_dtype == PLM_FP16, op, "x must be fp16 or bf16");
     PLM_CHECK_ARG(m >= 0 && n >= 0 && k >= 0, op, "sizes must be non-negative");
     PLM_CHECK_ARG(k % kMxBlock == 0, op, "K must be a multiple of 32");
     PLM_CHECK_ARG(n <= kMxMaxSize && k <= kMxMaxSize, op, "N and K must be at most 2^19");
-    // A grid of at most 2^32 work-items, and offsets of one workgroup below kOOB.
-    PLM_CHECK_ARG(m <= (int64_t{1} << 24) && m * std::max(n, k) <= (int64_t{1} << 36), op, "M must be at most 2^24, M N and M K at most 2^36");
+    PLM_CHECK_ARG(takes_rows(m, n, k), op, "M must be at most 2^24, M N and M K at most 2^36");
     return PLM_OK;
 }
 int check_weight(const char* op, const void* weight, const void* scale) {
@@ -115,7 +119,7 @@ int plm_gemm_mxfp4(const void* x, plm_dtype x_dtype, const void* weight, const v
 }
 
 int64_t plm_gemm_mxfp4_w4a4_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return m <= 0 || n <= 0 || k <= 0 ? 0 : room(m, k).total + mx_tiles_w4a4_bytes(m, n, k);
+    return counts(m, n, k) ? room(m, k).total + mx_tiles_w4a4_bytes(m, n, k) : 0;
 }
 
 int plm_gemm_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* weight, const void* scale, int64_t m, int64_t n, int64_t k, void* y,
@@ -160,7 +164,7 @@ int plm_gated_mxfp4(const void* x, plm_dtype x_dtype, const void* gate_weight, c
 }
 
 int64_t plm_mlp_mxfp4_w4a4_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return m <= 0 || n <= 0 || k <= 0 ? 0 : room(m, k).total + room(m, n).total + mx_tiles_w4a4_bytes(m, k, n);
+    return counts(m, n, k) ? room(m, k).total + room(m, n).total + mx_tiles_w4a4_bytes(m, k, n) : 0;
 }
 
 int plm_mlp_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* gate_weight, const void* gate_scale, const void* up_weight,
@@ -196,10 +200,10 @@ int plm_mlp_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* gate_weight
 }
 
 int64_t plm_gemm_mxfp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return m <= 0 || n <= 0 || k <= 0 ? 0 : mx_grad_bytes(m, n, k, false);
+    return counts(m, n, k) ? mx_grad_bytes(m, n, k, false) : 0;
 }
 int64_t plm_gated_mxfp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return m <= 0 || n <= 0 || k <= 0 ? 0 : mx_grad_bytes(m, n, k, true);
+    return counts(m, n, k) ? mx_grad_bytes(m, n, k, true) : 0;
 }
 
 int plm_gemm_mxfp4_grad(const void* dy, plm_dtype dtype, const void* weight, const void* scale, int64_t m, int64_t n, int64_t k, void* dx,

@@ -137,6 +137,8 @@ unsigned stream_blocks(int64_t threads) {
     return static_cast<unsigned>(std::min<int64_t>(ceil_div(threads, kThreads), int64_t{64} * cu_count()));
 }
 
+bool repacks(int64_t n, int64_t k) { return n >= 0 && k >= 0 && n <= kMxMaxSize && k <= kMxMaxSize; }
+
 int check_blocks(const char* op, int64_t m, int64_t k) {
     PLM_CHECK_ARG(m >= 0 && k >= 0, op, "sizes must be non-negative");
     PLM_CHECK_ARG(k % kMxBlock == 0, op, "K must be a multiple of 32");
@@ -161,8 +163,8 @@ using namespace plm;
 
 extern "C" {
 
-int64_t plm_mxfp4_weight_bytes(int64_t n, int64_t k) { return n < 0 || k < 0 ? -1 : make_mx_dims(n, k).tile_bytes(); }
-int64_t plm_mxfp4_scale_bytes(int64_t n, int64_t k) { return n < 0 || k < 0 ? -1 : make_mx_dims(n, k).scale_bytes(); }
+int64_t plm_mxfp4_weight_bytes(int64_t n, int64_t k) { return repacks(n, k) ? make_mx_dims(n, k).tile_bytes() : -1; }
+int64_t plm_mxfp4_scale_bytes(int64_t n, int64_t k) { return repacks(n, k) ? make_mx_dims(n, k).scale_bytes() : -1; }
 
 int plm_quantize_mxfp4(const void* x, plm_dtype x_dtype, int64_t m, int64_t k, uint8_t* codes, uint8_t* scale, void* stream) {
     const char* op = "quantize_mxfp4";

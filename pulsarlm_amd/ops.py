@@ -445,6 +445,7 @@ def repack_mxfp4_cuda(codes: torch.Tensor, scale: torch.Tensor):
     scale int32 [groups, K tiles, 64]), opaque, the plm tile layout of the format."""
     op = "repack_mxfp4"
     n, k = _mx_plain(op, codes, scale)
+    _require(max(n, k) <= 1 << 19, op, "N and K must be at most 2^19")
     weight = torch.empty((_lib.mxfp4_bytes("mxfp4_weight_bytes", n, k) // 4,), dtype=torch.int32, device=codes.device)
     packed = torch.empty(_mx_scale_shape(n, k), dtype=torch.int32, device=codes.device)
     codes, scale = codes.contiguous(), scale.contiguous()

@@ -156,3 +156,25 @@ def test_python_and_library_agree_on_the_scales():
         for k in (0, 32, 128, 160, 544, 4128):
             g, t, lanes = ops._mx_scale_shape(n, k)
             assert 4 * g * t * lanes == lib.plm_mxfp4_scale_bytes(n, k)
+
+
+QUERIES = ["plm_gemm_mxfp4_w4a4_workspace_bytes", "plm_mlp_mxfp4_w4a4_workspace_bytes", "plm_gemm_mxfp4_grad_workspace_bytes",
+           "plm_gated_mxfp4_grad_workspace_bytes"]
+
+
+@pytest.mark.parametrize("name", QUERIES)
+def test_workspace_queries_take_any_sizes(name):
+    """Sizes that the call refuses need no workspace; the sizes are multiplied only once they are known to be small."""
+    query = getattr(_lib.load(), name)
+    for huge in (1 << 25, 1 << 32, 1 << 40, (1 << 63) - 1):
+        for sizes in ((huge, 64, 64), (64, huge, 64), (64, 64, huge), (huge, huge, 64), (huge, 64, huge), (64, huge, huge), (huge, huge, huge)):
+            assert query(*sizes) == 0, sizes
+    assert query(1 << 24, 64, 64) > 0  # the largest M
+    assert query(1 << 17, 1 << 19, 1 << 19) > 0
+
+
+def test_layout_queries_take_any_sizes():
+    lib = _lib.load()
+    for n, k in ((1 << 62, 1 << 62), ((1 << 19) + 1, 32), (16, (1 << 19) + 32), ((1 << 63) - 1, 1)):
+        assert lib.plm_mxfp4_weight_bytes(n, k) == lib.plm_mxfp4_scale_bytes(n, k) == -1
+    assert lib.plm_mxfp4_weight_bytes(1 << 19, 1 << 19) == 1 << 37
