@@ -75,3 +75,50 @@ def test_fp16_factors_of_every_row_apart():
     for i in range(m):
         alone = ops.gated_mxfp4_grad_cuda(dh[i : i + 1], gate_up[i : i + 1], pg, pu, k)
         assert torch.equal(alone.view(torch.int16), dx[i : i + 1].view(torch.int16)) or i in (11, 13, 17)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,n,k", [(20, 96, 160), (70, 520, 288)])
+def test_gated_gradient_is_the_slope(m, n, k, dtype):
+    """<dx, v> against the central difference of sum(dh h(x + t v)), h in float64 and differentiated by nothing but
+    that, along a v in which every term of the gradient counts: a dx without one is told apart."""
+    dt = mx.DT[dtype]
+    wg, wu = mx.Weight(n, k, seed=1), mx.Weight(n, k, seed=2)
+    x, dh = mx.rows(m, k, dt, seed=3) * 0.25, mx.rows(m, n, dt, seed=5)
+    _, gate_up = ops.gated_mxfp4_cuda(x, wg.packed, wu.packed, n, keep_gate_up=True)
+    dx = ops.gated_mxfp4_grad_cuda(dh, gate_up, wg.packed, wu.packed, k)
+    check = Slope(x, dh, wg.dense, wu.dense, dt)
+    assert check.accepts(dx.double())
+    for without in check.incomplete():
+        assert not check.accepts(without)
+
+
+class Slope:
+    def __init__(self, x, dh, wg, wu, dt):
+        x, d = x.double(), dh.double()
+        g, u = x @ wg.t(), x @ wu.t()
+        s = torch.sigmoid(g)
+        dg, du = mx.gated_factors(d, g, u)
+        self.ref = dg @ wg + du @ wu
+        # dx without its up term, its gate term, the factor 1 + g (1 - s), and the part g (1 - s) of it.
+        self.others = [dg @ wg, du @ wu, (d * u) @ wg + du @ wu, (d * u * s) @ wg + du @ wu]
+        self.v = self.ref / self.ref.abs().max()
+
+        def loss(t):
+            gt, ut = (x + t * self.v) @ wg.t(), (x + t * self.v) @ wu.t()
+            return (d * gt / (1 + torch.exp(-gt)) * ut).sum().item()
+
+        # t^2 / 6 of the third derivative and 2^-53 of the losses' terms over t: 1e-5 of the slope leaves room for both.
+        t = 1e-4
+        self.slope = (loss(t) - loss(-t)) / (2 * t)
+        # A factor is rounded by at most half a step of its size and meets v through its weight row, dx likewise. g, u and dx
+        # are sums in 32 bits, off by less than 600 2^-23 of magnitudes some 10 times their own: 2^-10 of the terms.
+        rounding = (dg * (self.v @ wg.t())).abs().sum() + (du * (self.v @ wu.t())).abs().sum() + (self.ref * self.v).abs().sum()
+        terms = ((dg.abs() @ wg.abs() + du.abs() @ wu.abs()) * self.v.abs()).sum()
+        self.bound = (mx.half(dt) * rounding + 2.0**-10 * terms).item() + 1e-5 * abs(self.slope)
+
+    def accepts(self, dx):
+        return abs((dx * self.v).sum().item() - self.slope) <= self.bound
+
+    def incomplete(self):
+        return [torch.zeros_like(self.ref), *self.others]
