@@ -295,8 +295,10 @@ int plm_gemm_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* weight, co
                         void* stream);
 
 /* The input's gradient of plm_gemm_mxfp4: dx [M, K] = dy [M, N] @ W in `dtype`, dx 8-byte aligned.
- * (The weights are codes and have none.) N == 0 sets dx to zero. Workspace as above. */
+ * (The weights are codes and have none.) N == 0 sets dx to zero. Workspace as above; ..._aligned_workspace_bytes is
+ * what a dy that is 16-byte aligned needs: with N a multiple of 64 it is read in place, else copied there first. */
 int64_t plm_gemm_mxfp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int64_t plm_gemm_mxfp4_grad_aligned_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int plm_gemm_mxfp4_grad(const void* dy, plm_dtype dtype, const void* weight, const void* scale,
                         int64_t m, int64_t n, int64_t k, void* dx, void* workspace, size_t workspace_bytes,
                         void* stream);

@@ -51,6 +51,7 @@ SIGNATURES = {
     "plm_gemm_mxfp4_w4a4_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "plm_gemm_mxfp4_w4a4": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
     "plm_gemm_mxfp4_grad_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "plm_gemm_mxfp4_grad_aligned_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "plm_gemm_mxfp4_grad": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
     "plm_gated_mxfp4": (_INT, [_P, _INT, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P]),
     "plm_gated_mxfp4_grad_workspace_bytes": (_I64, [_I64, _I64, _I64]),

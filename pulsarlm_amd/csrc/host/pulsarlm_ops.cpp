@@ -427,7 +427,9 @@ at::Tensor gemm_mxfp4_grad_cuda(const at::Tensor& dy, const at::Tensor& weight, 
     mx_weight(op, dy, weight, scale, dy.size(1), k);
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
     at::Tensor dx = at::empty({dy.size(0), k}, dy.options());
-    const at::Tensor ws = mx_scratch(dy, plm_gemm_mxfp4_grad_workspace_bytes(dy.size(0), dy.size(1), k));
+    const auto bytes = reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0 ? plm_gemm_mxfp4_grad_aligned_workspace_bytes
+                                                                            : plm_gemm_mxfp4_grad_workspace_bytes;
+    const at::Tensor ws = mx_scratch(dy, bytes(dy.size(0), dy.size(1), k));
     check_rc(plm_gemm_mxfp4_grad(dy.data_ptr(), dtype_of(op, dy.scalar_type()), weight.data_ptr(), scale.data_ptr(), dy.size(0),
                                  dy.size(1), k, dx.data_ptr(), ptr(ws), mx_bytes(ws), stream_of(dy)));
     return dx;

@@ -8,7 +8,7 @@ int zero_output(const char* op, void* y, int64_t m, int64_t n, hipStream_t s);
 void launch_mx_tiles_w4a16(const mx_product& p, hipStream_t s);
 void launch_mx_tiles_w4a4(const mx_product& p, hipStream_t s);
 int64_t mx_tiles_w4a4_bytes(int64_t m, int64_t n, int64_t k);
-int64_t mx_grad_bytes(int64_t m, int64_t n, int64_t k, bool gated);
+int64_t mx_grad_bytes(int64_t m, int64_t n, int64_t k, bool gated, bool dy_aligned);
 int launch_mx_grad(const char* op, bool gated, bool bf16, const void* dy, const void* gate_up, const mx_matrix& w0, const mx_matrix& w1,
                    int64_t m, int64_t n, int64_t k, void* dx, void* workspace, hipStream_t s);
 
@@ -200,10 +200,13 @@ int plm_mlp_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* gate_weight
 }
 
 int64_t plm_gemm_mxfp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return counts(m, n, k) ? mx_grad_bytes(m, n, k, false) : 0;
+    return counts(m, n, k) ? mx_grad_bytes(m, n, k, false, false) : 0;
+}
+int64_t plm_gemm_mxfp4_grad_aligned_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    return counts(m, n, k) ? mx_grad_bytes(m, n, k, false, true) : 0;
 }
 int64_t plm_gated_mxfp4_grad_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return counts(m, n, k) ? mx_grad_bytes(m, n, k, true) : 0;
+    return counts(m, n, k) ? mx_grad_bytes(m, n, k, true, true) : 0;
 }
 
 int plm_gemm_mxfp4_grad(const void* dy, plm_dtype dtype, const void* weight, const void* scale, int64_t m, int64_t n, int64_t k, void* dx,
@@ -217,7 +220,7 @@ int plm_gemm_mxfp4_grad(const void* dy, plm_dtype dtype, const void* weight, con
     if (n == 0) return zero_output(op, dx, m, k, s);
     PLM_CHECK_ARG(dy && aligned(dy, 2), op, "dy must be 2-byte aligned");
     if (int rc = check_weight(op, weight, scale)) return rc;
-    if (int rc = check_workspace(op, workspace, workspace_bytes, plm_gemm_mxfp4_grad_workspace_bytes(m, n, k))) return rc;
+    if (int rc = check_workspace(op, workspace, workspace_bytes, mx_grad_bytes(m, n, k, false, aligned(dy, 16)))) return rc;
     return launch_mx_grad(op, false, dtype == PLM_BF16, dy, nullptr, matrix(weight, scale), matrix(weight, scale), m, n, k, dx, workspace, s);
 }
 

@@ -368,14 +368,14 @@ grad_plan make_grad_plan(int64_t m, int64_t k, int64_t steps) {
 }
 
 int64_t padded_n(int64_t n) { return round_up(n, kGradStep); }
-bool copies_dy(const void* dy, int64_t n) { return n % kGradStep != 0 || !aligned(dy, 16); }
+bool copies_dy(int64_t n, bool dy_aligned) { return n % kGradStep != 0 || !dy_aligned; }
 
-// Workspace: [rows in 16 bits][gated: a scale a row][fp32 partial sums].
+// Workspace: [rows in 16 bits, where dy is not read in place][gated: a scale a row][fp32 partial sums].
 int64_t rows_bytes(int64_t m, int64_t n, int sides) { return round_up(m * sides * padded_n(n) * 2, 256); }
 int64_t row_scale_bytes(int64_t m, int sides) { return sides == 2 ? round_up(m * 4, 256) : 0; }
-int64_t grad_bytes(int64_t m, int64_t n, int64_t k, int sides) {
+int64_t grad_bytes(int64_t m, int64_t n, int64_t k, int sides, bool rows) {
     const grad_plan p = make_grad_plan(m, k, sides * padded_n(n) / kGradStep);
-    return rows_bytes(m, n, sides) + row_scale_bytes(m, sides) + (p.splits > 1 ? p.splits * m * k * 4 : 0);
+    return (rows ? rows_bytes(m, n, sides) + row_scale_bytes(m, sides) : 0) + (p.splits > 1 ? p.splits * m * k * 4 : 0);
 }
 
 template <bool BF16, bool GATED>
@@ -405,7 +405,8 @@ int run(const char* op, bool gated, const void* dy, const void* gate_up, const m
     auto* rows = static_cast<uint16_t*>(workspace);
     a.dy = static_cast<const uint16_t*>(dy);
     a.pitch = n;
-    if (gated || copies_dy(dy, n)) {
+    auto* sums = static_cast<uint8_t*>(workspace);
+    if (gated || copies_dy(n, aligned(dy, 16))) {
         auto* row_scale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + rows_bytes(m, n, sides));
         if (gated) launch_rows<BF16, true>(dy, gate_up, m, n, rows, row_scale, s);
         else launch_rows<BF16, false>(dy, nullptr, m, n, rows, nullptr, s);
@@ -413,13 +414,14 @@ int run(const char* op, bool gated, const void* dy, const void* gate_up, const m
         PLM_HIP_LAUNCH_CHECK(op);
         a.dy = rows;
         a.pitch = sides * padded_n(n);
+        sums += rows_bytes(m, n, sides) + row_scale_bytes(m, sides);
     }
     a.side_steps = static_cast<int>(padded_n(n) / kGradStep);
     const grad_plan p = make_grad_plan(m, k, int64_t{sides} * a.side_steps);
     a.w0 = w0;
     a.w1 = w1;
     a.dx = static_cast<uint16_t*>(dx);
-    a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + rows_bytes(m, n, sides) + row_scale_bytes(m, sides));
+    a.partial = reinterpret_cast<float*>(sums);
     a.m = static_cast<int>(m);
     a.k = static_cast<int>(k);
     a.ktiles = static_cast<int>(d.ktiles);
@@ -452,7 +454,9 @@ void launch_mx_combine(bool bf16, const float* partial, int64_t count, int split
     else mx_combine_kernel<false><<<grid, 256, 0, s>>>(p, quads, splits, o);
 }
 
-int64_t mx_grad_bytes(int64_t m, int64_t n, int64_t k, bool gated) { return grad_bytes(m, n, k, gated ? 2 : 1); }
+int64_t mx_grad_bytes(int64_t m, int64_t n, int64_t k, bool gated, bool dy_aligned) {
+    return grad_bytes(m, n, k, gated ? 2 : 1, gated || copies_dy(n, dy_aligned));
+}
 
 int launch_mx_grad(const char* op, bool gated, bool bf16, const void* dy, const void* gate_up, const mx_matrix& w0, const mx_matrix& w1,
                    int64_t m, int64_t n, int64_t k, void* dx, void* workspace, hipStream_t s) {

@@ -520,7 +520,7 @@ def gemm_mxfp4_grad_cuda(dy: torch.Tensor, weight: torch.Tensor, scale: torch.Te
     m, n = dy.shape
     _mx_weight(op, dy, weight, scale, n, k)
     dx = _mx_out(op, dy, (m, k), out)
-    ws = _mx_scratch(op, dy, m, n, k)
+    ws = _mx_scratch(op if dy.data_ptr() % 16 else "gemm_mxfp4_grad_aligned", dy, m, n, k)
     with _on(dy.device):
         _call("plm_gemm_mxfp4_grad", _ptr(dy), _DTYPES[dy.dtype], _ptr(weight), _ptr(scale), m, n, k, _ptr(dx), _ptr(ws),
               0 if ws is None else ws.numel(), _stream(dy.device))

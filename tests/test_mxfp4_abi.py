@@ -178,3 +178,17 @@ def test_layout_queries_take_any_sizes():
     for n, k in ((1 << 62, 1 << 62), ((1 << 19) + 1, 32), (16, (1 << 19) + 32), ((1 << 63) - 1, 1)):
         assert lib.plm_mxfp4_weight_bytes(n, k) == lib.plm_mxfp4_scale_bytes(n, k) == -1
     assert lib.plm_mxfp4_weight_bytes(1 << 19, 1 << 19) == 1 << 37
+
+
+def test_gradient_needs_no_room_for_a_dy_that_it_reads_in_place():
+    lib = _lib.load()
+    for m, n, k in ((4096, 24576, 4096), (1, 64, 32), (2000, 4096, 4096), (333, 5000, 4128), (8200, 4300, 96)):
+        every, aligned = lib.plm_gemm_mxfp4_grad_workspace_bytes(m, n, k), lib.plm_gemm_mxfp4_grad_aligned_workspace_bytes(m, n, k)
+        copy = -(-m * -(-n // 64) * 64 * 2 // 256) * 256
+        assert every - aligned == (copy if n % 64 == 0 else 0) and every >= copy
+    assert lib.plm_gemm_mxfp4_grad_aligned_workspace_bytes(4096, 24576, 4096) == 0  # one round of tiles, unsplit
+    assert lib.plm_gemm_mxfp4_grad_aligned_workspace_bytes(0, 64, 64) == lib.plm_gemm_mxfp4_grad_aligned_workspace_bytes(1 << 40, 64, 1 << 40) == 0
+    # What is missing is said for the dy at hand: an aligned one asks for less.
+    need = lib.plm_gemm_mxfp4_grad_workspace_bytes(1, 64, 32)
+    rc, said = grad(dy=ctypes.c_void_p(4098), m=1, n=64, k=32, ws=None, size=0)
+    assert rc == _lib.PLM_ERR_WORKSPACE and f"workspace of {need} bytes" in said

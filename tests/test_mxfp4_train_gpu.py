@@ -122,3 +122,37 @@ class Slope:
 
     def incomplete(self):
         return [torch.zeros_like(self.ref), *self.others]
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 64, 96), (333, 4096, 4128), (300, 256, 1056), (70, 33, 96)])
+def test_linear_gradient_in_the_workspace_it_asks_for(m, n, k):
+    """Exactly the bytes of either query, with a guard behind them; the same dx from an aligned dy and one that is copied."""
+    from pulsarlm_amd import _lib
+
+    lib, w, dy = _lib.load(), mx.Weight(n, k, seed=1), mx.rows(m, n, torch.bfloat16, seed=2)
+    room = torch.empty(m * n + 8, dtype=torch.bfloat16, device="cuda")
+    apart = room[1 : 1 + m * n].view(m, n).copy_(dy)
+    results = []
+    for rows, need in ((dy, lib.plm_gemm_mxfp4_grad_aligned_workspace_bytes(m, n, k)), (dy, lib.plm_gemm_mxfp4_grad_workspace_bytes(m, n, k)),
+                       (apart, lib.plm_gemm_mxfp4_grad_workspace_bytes(m, n, k))):
+        ws = torch.full((need + 256,), 77, dtype=torch.uint8, device="cuda")
+        dx = torch.full((m, k), float("nan"), dtype=torch.bfloat16, device="cuda")
+        _lib.check(lib.plm_gemm_mxfp4_grad(rows.data_ptr(), _lib.PLM_BF16, w.packed[0].data_ptr(), w.packed[1].data_ptr(), m, n, k,
+                                           dx.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+        assert (ws[need:] == 77).all()
+        results.append(dx)
+    mx.within(results[0], *mx.product(dy.double(), w.dense.t()), "dx")
+    assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+    assert torch.equal(results[0], ops.gemm_mxfp4_grad_cuda(dy, *w.packed, k)) and torch.equal(results[0], ops.gemm_mxfp4_grad_cuda(apart, *w.packed, k))
+
+
+def test_linear_gradient_takes_no_scratch_for_rows_in_place():
+    """What a call takes from the allocator, over its output."""
+    m, n, k = 8192, 4096, 4096
+    w, dy = mx.Weight(n, k, seed=1), torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    dx = torch.empty(m, k, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.gemm_mxfp4_grad_cuda(dy, *w.packed, k, out=dx)
+    assert torch.cuda.max_memory_allocated() - before < 2 * m * n
