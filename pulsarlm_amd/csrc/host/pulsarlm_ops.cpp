@@ -8,7 +8,10 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <torch/csrc/autograd/custom_function.h>
+
 #include <algorithm>
+#include <functional>
 #include <map>
 #include <mutex>
 #include <string>
@@ -361,6 +364,52 @@ at::Tensor mx_scratch(const at::Tensor& x, int64_t bytes) {
 }
 size_t mx_bytes(const at::Tensor& t) { return t.defined() ? static_cast<size_t>(t.numel()) : 0; }
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool mx_records(const at::Tensor& x) { return x.requires_grad() && at::GradMode::is_enabled(); }
+
+struct mx_linear : torch::autograd::Function<mx_linear> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, int64_t n) {
+        at::Tensor y = gemm_mxfp4_cuda(x, weight, scale, n);
+        ctx->save_for_backward({weight, scale});
+        ctx->saved_data["k"] = x.size(1);
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list dy) {
+        const variable_list w = ctx->get_saved_variables();
+        return {gemm_mxfp4_grad_cuda(dy[0].contiguous(), w[0], w[1], ctx->saved_data["k"].toInt()), {}, {}, {}};
+    }
+};
+
+struct mx_gated : torch::autograd::Function<mx_gated> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate_weight, const at::Tensor& gate_scale,
+                                 const at::Tensor& up_weight, const at::Tensor& up_scale, int64_t intermediate) {
+        auto [h, gate_up] = gated_mxfp4_cuda(x, gate_weight, gate_scale, up_weight, up_scale, intermediate, true);
+        ctx->mark_non_differentiable({gate_up});
+        ctx->set_materialize_grads(false);  // no zeros for gate_up's
+        ctx->save_for_backward({gate_up, gate_weight, gate_scale, up_weight, up_scale});
+        ctx->saved_data["k"] = x.size(1);
+        return {h, gate_up};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list dh) {
+        const variable_list w = ctx->get_saved_variables();
+        return {gated_mxfp4_grad_cuda(dh[0].contiguous(), w[0], w[1], w[2], w[3], w[4], ctx->saved_data["k"].toInt()), {}, {}, {}, {}, {}};
+    }
+};
+
+// call(): an output in the graph of its two inputs (or one, twice) whose gradient is asked for in vain, and says so then.
+struct mx_no_gradient : torch::autograd::Function<mx_no_gradient> {
+    static at::Tensor forward(AutogradContext* ctx, const char* op, const std::function<at::Tensor()>& call, const at::Tensor&,
+                              const at::Tensor&) {
+        ctx->saved_data["op"] = std::string(op);
+        return call();
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list&) {
+        TORCH_CHECK(false, ctx->saved_data["op"].toStringRef(), ": has no gradient");
+    }
+};
+
 }  // namespace
 
 std::tuple<at::Tensor, at::Tensor> quantize_mxfp4_cuda(const at::Tensor& x) {
@@ -400,6 +449,7 @@ std::tuple<at::Tensor, at::Tensor> repack_mxfp4_cuda(const at::Tensor& codes, co
 
 at::Tensor gemm_mxfp4_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, int64_t n) {
     const char* op = "gemm_mxfp4";
+    if (mx_records(x)) return mx_linear::apply(x, weight, scale, n);
     mx_rows(op, "x", x);
     mx_weight(op, x, weight, scale, n, x.size(1));
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
@@ -411,6 +461,7 @@ at::Tensor gemm_mxfp4_cuda(const at::Tensor& x, const at::Tensor& weight, const 
 
 at::Tensor gemm_mxfp4_w4a4_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, int64_t n) {
     const char* op = "gemm_mxfp4_w4a4";
+    if (mx_records(x)) return mx_no_gradient::apply(op, [&] { return gemm_mxfp4_w4a4_cuda(x, weight, scale, n); }, x, x);
     mx_rows(op, "x", x);
     mx_weight(op, x, weight, scale, n, x.size(1));
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
@@ -423,6 +474,7 @@ at::Tensor gemm_mxfp4_w4a4_cuda(const at::Tensor& x, const at::Tensor& weight, c
 
 at::Tensor gemm_mxfp4_grad_cuda(const at::Tensor& dy, const at::Tensor& weight, const at::Tensor& scale, int64_t k) {
     const char* op = "gemm_mxfp4_grad";
+    if (mx_records(dy)) return mx_no_gradient::apply(op, [&] { return gemm_mxfp4_grad_cuda(dy, weight, scale, k); }, dy, dy);
     mx_rows(op, "dy", dy);
     mx_weight(op, dy, weight, scale, dy.size(1), k);
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
@@ -439,6 +491,10 @@ std::tuple<at::Tensor, at::Tensor> gated_mxfp4_cuda(const at::Tensor& x, const a
                                                     const at::Tensor& up_weight, const at::Tensor& up_scale,
                                                     int64_t intermediate, bool keep_gate_up) {
     const char* op = "gated_mxfp4";
+    if (mx_records(x)) {
+        const variable_list out = mx_gated::apply(x, gate_weight, gate_scale, up_weight, up_scale, intermediate);
+        return {out[0], keep_gate_up ? out[1] : at::Tensor()};
+    }
     mx_rows(op, "x", x);
     mx_weight(op, x, gate_weight, gate_scale, intermediate, x.size(1));
     mx_weight(op, x, up_weight, up_scale, intermediate, x.size(1));
@@ -455,6 +511,9 @@ at::Tensor gated_mxfp4_grad_cuda(const at::Tensor& dh, const at::Tensor& gate_up
                                  const at::Tensor& gate_scale, const at::Tensor& up_weight, const at::Tensor& up_scale,
                                  int64_t hidden) {
     const char* op = "gated_mxfp4_grad";
+    if (mx_records(dh) || mx_records(gate_up))
+        return mx_no_gradient::apply(
+            op, [&] { return gated_mxfp4_grad_cuda(dh, gate_up, gate_weight, gate_scale, up_weight, up_scale, hidden); }, dh, gate_up);
     mx_rows(op, "dh", dh);
     const int64_t m = dh.size(0), n = dh.size(1);
     TORCH_CHECK(gate_up.scalar_type() == at::kFloat && gate_up.device() == dh.device() && gate_up.dim() == 2 && gate_up.size(0) == m &&
@@ -475,6 +534,11 @@ at::Tensor mlp_mxfp4_w4a4_cuda(const at::Tensor& x, const at::Tensor& gate_weigh
                                const at::Tensor& up_weight, const at::Tensor& up_scale, const at::Tensor& down_weight,
                                const at::Tensor& down_scale, int64_t intermediate) {
     const char* op = "mlp_mxfp4_w4a4";
+    if (mx_records(x))
+        return mx_no_gradient::apply(
+            op,
+            [&] { return mlp_mxfp4_w4a4_cuda(x, gate_weight, gate_scale, up_weight, up_scale, down_weight, down_scale, intermediate); }, x,
+            x);
     mx_rows(op, "x", x);
     const int64_t m = x.size(0), k = x.size(1);
     mx_weight(op, x, gate_weight, gate_scale, intermediate, k);

@@ -89,7 +89,8 @@ at::Tensor gemm_int4_split_cuda(const at::Tensor& x, const at::Tensor& weight_pa
                                 const at::Tensor& weight_scale, int64_t group_size, int64_t num_splits);
 
 // ---- MXFP4: microscaled 4-bit floating point (no counterpart in ops.hpp). 32 consecutive K values share a
-// scale 2^(b - 127) and are e2m1 codes; include/pulsarlm_amd.h has the rules. ----
+// scale 2^(b - 127) and are e2m1 codes; include/pulsarlm_amd.h has the rules. gemm_mxfp4_cuda and gated_mxfp4_cuda record
+// their x's gradient for autograd; a backward pass that reaches another of these raises. ----
 
 // x [M, K] fp32, fp16 or bf16 -> (codes uint8 [M, K/2], scale uint8 [M, K/32]), and back.
 std::tuple<at::Tensor, at::Tensor> quantize_mxfp4_cuda(const at::Tensor& x);

@@ -482,6 +482,54 @@ def _mx_out(op: str, x: torch.Tensor, shape, out: torch.Tensor | None) -> torch.
     return out
 
 
+class _MxLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, scale, n):
+        y = gemm_mxfp4_cuda(x, weight, scale, n)
+        ctx.save_for_backward(weight, scale)
+        ctx.k = x.shape[1]
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return gemm_mxfp4_grad_cuda(dy.contiguous(), *ctx.saved_tensors, ctx.k), None, None, None
+
+
+class _MxGated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, gate_scale, up, up_scale, intermediate):
+        h, gate_up = gated_mxfp4_cuda(x, (gate, gate_scale), (up, up_scale), intermediate, keep_gate_up=True)
+        ctx.mark_non_differentiable(gate_up)
+        ctx.set_materialize_grads(False)  # no zeros for gate_up's
+        ctx.save_for_backward(gate_up, gate, gate_scale, up, up_scale)
+        ctx.k = x.shape[1]
+        return h, gate_up
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, _):
+        gate_up, gate, gate_scale, up, up_scale = ctx.saved_tensors
+        return gated_mxfp4_grad_cuda(dh.contiguous(), gate_up, (gate, gate_scale), (up, up_scale), ctx.k), *(None,) * 5
+
+
+class _MxNoGradient(torch.autograd.Function):
+    """call(): an output in x's graph whose gradient is asked for in vain, and says so then."""
+
+    @staticmethod
+    def forward(ctx, op, call, *inputs):
+        ctx.op = op
+        return call()
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.op}: has no gradient")
+
+
+def _mx_records(x: torch.Tensor) -> bool:
+    return x.requires_grad and torch.is_grad_enabled()
+
+
 def _mx_x(op: str, x: torch.Tensor):
     _mx_contiguous(op, "x", x, _HALF)
     _require(x.shape[1] % 32 == 0, op, "K must be a multiple of 32")
@@ -489,8 +537,12 @@ def _mx_x(op: str, x: torch.Tensor):
 
 
 def gemm_mxfp4_cuda(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, n: int, out=None) -> torch.Tensor:
-    """y [M, N] = x [M, K] @ W^T with an MXFP4 weight (repack_mxfp4_cuda) and 16-bit x, fp32 sums. out may not overlap x."""
+    """y [M, N] = x [M, K] @ W^T with an MXFP4 weight (repack_mxfp4_cuda) and 16-bit x, fp32 sums. out may not overlap x.
+    Differentiable in x, without out, by gemm_mxfp4_grad_cuda."""
     op = "gemm_mxfp4"
+    if _mx_records(x):
+        _require(out is None, op, "out records no gradient")
+        return _MxLinear.apply(x, weight, scale, n)
     m, k = _mx_x(op, x)
     _mx_weight(op, x, weight, scale, n, k)
     y = _mx_out(op, x, (m, n), out)
@@ -500,8 +552,12 @@ def gemm_mxfp4_cuda(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, 
 
 
 def gemm_mxfp4_w4a4_cuda(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, n: int, out=None) -> torch.Tensor:
-    """W4A4: the same with x quantized as by quantize_mxfp4_cuda, on the fp4 matrix instruction."""
+    """W4A4: the same with x quantized as by quantize_mxfp4_cuda, on the fp4 matrix instruction. Has no gradient: a
+    backward pass that reaches it raises."""
     op = "gemm_mxfp4_w4a4"
+    if _mx_records(x):
+        _require(out is None, op, "out records no gradient")
+        return _MxNoGradient.apply(op, lambda: gemm_mxfp4_w4a4_cuda(x, weight, scale, n), x)
     m, k = _mx_x(op, x)
     _mx_weight(op, x, weight, scale, n, k)
     y = _mx_out(op, x, (m, n), out)
@@ -513,8 +569,11 @@ def gemm_mxfp4_w4a4_cuda(x: torch.Tensor, weight: torch.Tensor, scale: torch.Ten
 
 
 def gemm_mxfp4_grad_cuda(dy: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, k: int, out=None) -> torch.Tensor:
-    """The gradient of gemm_mxfp4_cuda's x: dx [M, K] = dy [M, N] @ W."""
+    """The gradient of gemm_mxfp4_cuda's x: dx [M, K] = dy [M, N] @ W. Has none of its own."""
     op = "gemm_mxfp4_grad"
+    if _mx_records(dy):
+        _require(out is None, op, "out records no gradient")
+        return _MxNoGradient.apply(op, lambda: gemm_mxfp4_grad_cuda(dy, weight, scale, k), dy)
     _mx_contiguous(op, "dy", dy, _HALF)
     _require(k % 32 == 0, op, "K must be a multiple of 32")
     m, n = dy.shape
@@ -529,8 +588,12 @@ def gemm_mxfp4_grad_cuda(dy: torch.Tensor, weight: torch.Tensor, scale: torch.Te
 
 def gated_mxfp4_cuda(x: torch.Tensor, gate: tuple, up: tuple, intermediate: int, keep_gate_up: bool = False):
     """h [M, I] = silu(x @ Wgate^T) * (x @ Wup^T) in one kernel, from fp32 sums; gate and up are (weight, scale) pairs
-    of repack_mxfp4_cuda. keep_gate_up: (h, gate_up fp32 [M, 2 I]), what gated_mxfp4_grad_cuda takes."""
+    of repack_mxfp4_cuda. keep_gate_up: (h, gate_up fp32 [M, 2 I]), what gated_mxfp4_grad_cuda takes. h is differentiable
+    in x by that (gate_up is kept then in either case), gate_up is not."""
     op = "gated_mxfp4"
+    if _mx_records(x):
+        h, gate_up = _MxGated.apply(x, *gate, *up, intermediate)
+        return (h, gate_up) if keep_gate_up else h
     m, k = _mx_x(op, x)
     for w in (gate, up):
         _mx_weight(op, x, w[0], w[1], intermediate, k)
@@ -543,8 +606,10 @@ def gated_mxfp4_cuda(x: torch.Tensor, gate: tuple, up: tuple, intermediate: int,
 
 
 def gated_mxfp4_grad_cuda(dh: torch.Tensor, gate_up: torch.Tensor, gate: tuple, up: tuple, hidden: int) -> torch.Tensor:
-    """The gradient of gated_mxfp4_cuda's x [M, hidden] from dh [M, I] and the gate_up that it kept."""
+    """The gradient of gated_mxfp4_cuda's x [M, hidden] from dh [M, I] and the gate_up that it kept. Has none of its own."""
     op = "gated_mxfp4_grad"
+    if _mx_records(dh) or _mx_records(gate_up):
+        return _MxNoGradient.apply(op, lambda: gated_mxfp4_grad_cuda(dh, gate_up, gate, up, hidden), dh, gate_up)
     _mx_contiguous(op, "dh", dh, _HALF)
     _require(hidden % 32 == 0, op, "K must be a multiple of 32")
     m, n = dh.shape
@@ -562,8 +627,11 @@ def gated_mxfp4_grad_cuda(dh: torch.Tensor, gate_up: torch.Tensor, gate: tuple, 
 
 def mlp_mxfp4_w4a4_cuda(x: torch.Tensor, gate: tuple, up: tuple, down: tuple, intermediate: int) -> torch.Tensor:
     """The feed-forward block with 4-bit activations: y [M, K] = Q(h) @ Wdown^T, h = silu(g) u of Q(x), Q as
-    quantize_mxfp4_cuda; h is quantized from its fp32 values. Wgate, Wup [I, K], Wdown [K, I]; I a multiple of 32."""
+    quantize_mxfp4_cuda; h is quantized from its fp32 values. Wgate, Wup [I, K], Wdown [K, I]; I a multiple of 32. Has no
+    gradient: a backward pass that reaches it raises."""
     op = "mlp_mxfp4_w4a4"
+    if _mx_records(x):
+        return _MxNoGradient.apply(op, lambda: mlp_mxfp4_w4a4_cuda(x, gate, up, down, intermediate), x)
     m, k = _mx_x(op, x)
     _require(intermediate % 32 == 0, op, "the intermediate size must be a multiple of 32")
     for w in (gate, up):
