@@ -1,7 +1,7 @@
 // MXFP4 products for few rows (one token to short prompts): y[M, N] = x[M, K] @ W^T, the gated block's
 // two products with its activation, and the same with 4-bit x.
 //
-// A workgroup owns RB blocks of 16 rows by SG strips of 16 weight rows over all of K; its wavefronts take
+// A workgroup owns the rows (RB blocks of 16, one or two) by SG strips of 16 weight rows over all of K; its wavefronts take
 // the K tiles round-robin, each holding all RB x SG accumulators of its own tiles, and their sums are added
 // through LDS in wavefront order. The weight bytes bound it (they are read once, by one wavefront each,
 // DW K tiles ahead in registers, nontemporal), so nothing is shared before the end and no barrier stands in
@@ -28,7 +28,7 @@ struct rows_args {
     const uint16_t* x;
     mx_matrix xq, w0, w1;
     mx_output out;
-    int m, k, ktiles, strips, m_blocks;
+    int m, k, ktiles, strips;
 };
 
 constexpr int kWaves = 8;
@@ -49,8 +49,7 @@ __global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
     const int lane = threadIdx.x & 63;
     const int wave = uniform(threadIdx.x >> 6);
     const int col16 = lane & 15, kq = lane >> 4;
-    const int strip0 = blockIdx.x / a.m_blocks * P, row0 = (blockIdx.x % a.m_blocks) * RB * 16;
-    const int rows = min(RB * 16, a.m - row0);
+    const int strip0 = blockIdx.x * P;
     const int mine = min(P, a.strips - strip0);  // strips past N read zeros
 
     const int64_t w_at = static_cast<int64_t>(strip0) * a.ktiles * kSubTileBytes, s_at = static_cast<int64_t>(strip0 >> 2) * a.ktiles * 64;
@@ -63,12 +62,9 @@ __global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
     }
     const int x_pitch = STAGED ? (a.ktiles + 3) / 4 * 1024 : 0;
     const __amdgpu_buffer_rsrc_t xr =
-        XM == kXCodes ? make_rsrc(a.xq.codes + static_cast<int64_t>(row0 / 16) * a.ktiles * kSubTileBytes,
-                                  static_cast<uint32_t>((rows + 15) / 16) * a.ktiles * kSubTileBytes)
-                      : make_rsrc(a.x + static_cast<int64_t>(row0) * a.k, static_cast<uint32_t>(rows) * a.k * 2);
-    const __amdgpu_buffer_rsrc_t xsr =
-        XM == kXCodes ? make_rsrc(a.xq.scale + static_cast<int64_t>(row0 / 64) * a.ktiles * 64, static_cast<uint32_t>(a.ktiles) * 256)
-                      : xr;
+        XM == kXCodes ? make_rsrc(a.xq.codes, static_cast<uint32_t>((a.m + 15) / 16) * a.ktiles * kSubTileBytes)
+                      : make_rsrc(a.x, static_cast<uint32_t>(a.m) * a.k * 2);
+    const __amdgpu_buffer_rsrc_t xsr = XM == kXCodes ? make_rsrc(a.xq.scale, static_cast<uint32_t>(a.ktiles) * 256) : xr;
 
     struct batch {
         u32x4_t w[SG], x[XM == kXCodes ? RB : 1];
@@ -86,7 +82,7 @@ __global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
                 b.x[i] = buffer_load16(xr, lane * 16, in ? (i * a.ktiles + kt) * kSubTileBytes : kOOB);
-                b.xs[i] = __builtin_amdgcn_raw_buffer_load_b8(xsr, lane * 4, in ? kt * 256 + ((row0 / 16 + i) & 3) : kOOB, 0);
+                b.xs[i] = __builtin_amdgcn_raw_buffer_load_b8(xsr, lane * 4, in ? kt * 256 + i : kOOB, 0);
             }
         }
     };
@@ -99,7 +95,7 @@ __global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
 #pragma unroll
             for (int i = 0; i < XL; ++i) {
                 const int r = 4 * i + (lane >> 4), c = (lane & 15) ^ (r & 15);
-                const bool ok = in && kt * kTileK + 8 * c < a.k;  // rows past `rows` are past the buffer's end
+                const bool ok = in && kt * kTileK + 8 * c < a.k;  // rows past M are past the buffer's end
                 buffer_load_lds16(xr, ring + slot * SLOT + i * 1024, ok ? r * a.k * 2 + c * 16 : kOOB, in ? kt * 256 : 0);
             }
         }
@@ -116,7 +112,7 @@ __global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
         const uint8_t* xt[RB];
         int swz = 0;
         if constexpr (STAGED) {
-            const int r = min(col16, rows - 1);
+            const int r = min(col16, a.m - 1);
             xt[0] = mx_lds + r * x_pitch + kt * 256;
             swz = r & 15;
         } else if constexpr (XM == kXRing) {
@@ -168,7 +164,7 @@ __global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
     if constexpr (STAGED) {
         // Row r's K group q (512 values, 1 KiB), swizzled within each K tile.
         const int groups = x_pitch / 1024;
-        for (int i = wave; i < rows * groups; i += NW) {
+        for (int i = wave; i < a.m * groups; i += NW) {
             const int r = i / groups, q = i % groups;
             const int c = (lane & 48) | ((lane & 15) ^ (r & 15)), at = q * 512 + c * 8;
             buffer_load_lds16(xr, mx_lds + i * 1024, at < a.k ? (r * a.k + at) * 2 : kOOB, 0);
@@ -218,23 +214,24 @@ __global__ void __launch_bounds__(kWaves * 64) mx_rows_kernel(rows_args a) {
         if constexpr (EPI == kMxGatedCodes) {
             static_assert(P == 2 || EPI != kMxGatedCodes, "a block is two strips");
             const f32x4_t g[2] = {total(i, 0, ln), total(i, 1, ln)}, h[2] = {total(i, P, ln), total(i, P + 1, ln)};
-            if (16 * i < rows) mx_store_codes(a.out, row0 / 16 + i, strip0 >> 1, g, h);  // wave-uniform
+            if (16 * i < a.m) mx_store_codes(a.out, i, strip0 >> 1, g, h);  // wave-uniform
         } else {
             const int col = (strip0 + p) * kTileN + 4 * (ln >> 4);
             const f32x4_t v = total(i, p, ln);
             if constexpr (EPI == kMxPlain) {
-                if (r < rows) mx_store_plain<BF16>(a.out, row0 + r, col, v);
+                if (r < a.m) mx_store_plain<BF16>(a.out, r, col, v);
             } else {
                 const f32x4_t up = total(i, P + p, ln);
-                if (r < rows) {
-                    mx_store_plain<BF16>(a.out, row0 + r, col, mx_gated4(v, up));
-                    mx_store_gate_up(a.out, row0 + r, col, v, up);
+                if (r < a.m) {
+                    mx_store_plain<BF16>(a.out, r, col, mx_gated4(v, up));
+                    mx_store_gate_up(a.out, r, col, v, up);
                 }
             }
         }
     }
 }
 
+// M <= 16 RB.
 template <int XM, bool BF16, int RB, int SG, mx_epilogue EPI> void launch(const mx_product& p, hipStream_t s) {
     const mx_dims d = make_mx_dims(p.n, p.k);
     rows_args a{};
@@ -247,14 +244,13 @@ template <int XM, bool BF16, int RB, int SG, mx_epilogue EPI> void launch(const 
     a.k = static_cast<int>(p.k);
     a.ktiles = static_cast<int>(d.ktiles);
     a.strips = static_cast<int>(d.strips);
-    a.m_blocks = static_cast<int>(ceil_div(p.m, RB * 16));
     constexpr int NW = kWaves;
     int64_t loop = 0;  // bytes of LDS in the K loop
     if (XM == kXStaged || XM == kXStagedQuantize) loop = p.m * ceil_div(d.ktiles, 4) * 1024;
     if (XM == kXRing) loop = int64_t{NW} * 2 * RB * 4096;
     const int64_t lds = std::max<int64_t>(loop, int64_t{RB} * SG * NW * 1024);
     constexpr int P = EPI == kMxPlain ? SG : SG / 2;
-    const int64_t grid = ceil_div(d.strips, P) * a.m_blocks;
+    const int64_t grid = ceil_div(d.strips, P);
     mx_rows_kernel<XM, BF16, RB, SG, EPI><<<static_cast<unsigned>(grid), NW * 64, static_cast<size_t>(lds), s>>>(a);
 }
 

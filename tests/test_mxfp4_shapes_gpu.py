@@ -67,6 +67,13 @@ def test_rows_strips(m, n, k):
     mx.within(ops.gemm_mxfp4_w4a4_cuda(x, *w.packed, n), *mx.product(mx.rounded(x), w.dense), "W4A4")
 
 
+# x as codes in one row block (K too long to be quantized in the kernel), two and four strips, and in a whole second block.
+@pytest.mark.parametrize("m,n,k", [(16, 4200, 8224), (16, 8300, 4128), (9, 4200, 12320), (32, 4200, 8224), (17, 8300, 160)])
+def test_rows_codes_blocks(m, n, k):
+    w, x = mx.Weight(n, k, seed=n), mx.rows(m, k, torch.bfloat16, seed=m)
+    mx.within(ops.gemm_mxfp4_w4a4_cuda(x, *w.packed, n), *mx.product(mx.rounded(x), w.dense), "W4A4")
+
+
 @pytest.mark.parametrize("m", [1, 20])
 def test_rows_gated_strips(m):
     n, k = 4200, 544
