@@ -89,7 +89,7 @@ __device__ __forceinline__ f32x4_t mx_mfma(u32x4_t a, uint32_t sa, u32x4_t b, ui
 }
 
 // silu(g) u from the 32-bit sums. 1 / (1 + e^-g) by the hardware's exp2 and reciprocal, each within an ulp
-// or two of 32 bits: the caller rounds to 16 bits or to e2m1 codes.
+// or two of 32 bits (and zero below 2^-126, g < -87.3): the caller rounds to 16 bits or to e2m1 codes.
 __device__ __forceinline__ float mx_sigmoid(float g) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f));
 }

@@ -13,7 +13,8 @@
 //   (mxfp4_tiles.hpp): their operands are in registers, and the next step's first half is read meanwhile.
 // * Few tiles: the steps are split over workgroups, whose fp32 sums a second kernel adds in split order.
 // * What bounds it: the way of W through LDS. At M = 2000, N = K = 4096 the matrix units are busy 42% of the cycles and LDS
-//   48% (60% and 45% with tiles of 256 rows); without W's writes a pass takes 51 us of 70, without dy's 60. M = 4096,
+//   48% (60% and 45% with tiles of 256 rows); without W's decoding and writes, its loads kept, a call takes 61 us of 73,
+//   without dy's writes 66. M = 4096,
 //   N 24576, K 4096: 627 us, 1314 TFLOP/s; M = 2000 70 us, 960; the gated block's M = 4096, intermediate 12288: 740 us,
 //   150 of them the factors' kernel, which moves 704 MB at 4.6 TB/s.
 #include "mxfp4.hpp"

@@ -13,8 +13,9 @@
 //   W4A16 four of 32 K values.
 // * The weights are the A operand and x the B operand: a lane ends with four neighbouring columns of a row.
 // * What bounds it (M = 4096, N 24576, K 4096): W4A16 546 us, 1511 TFLOP/s, what the library's 16-bit product makes
-//   (1410-1455); W4A4 214 us, 3850 TFLOP/s, with the matrix units busy 55% of the cycles (70% at K 24576) at 1.7-1.9
-//   GHz. The same FLOPs at N 4096, K 24576, with a sixth of the stores, take 216 us: the clock gives way to the load.
+//   (1410-1455); W4A4 214 us with the quantizer's 10, of which the product takes 195, 4200 TFLOP/s, with the matrix units
+//   busy 55% of the cycles at 1.83-1.95 GHz, and wavefronts waiting 27%. The same FLOPs at N 4096, K 24576, with a
+//   sixth of the stores and as long a run a tile, take 167 us, 70% and 1.89-1.91 GHz.
 // * Gated: local strips 2 p and 2 p + 1 are gate and up of one 16-column slice, so that both halves of an
 //   output are in one lane.
 #pragma once
