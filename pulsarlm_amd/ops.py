@@ -606,7 +606,8 @@ def gated_mxfp4_cuda(x: torch.Tensor, gate: tuple, up: tuple, intermediate: int,
 
 
 def gated_mxfp4_grad_cuda(dh: torch.Tensor, gate_up: torch.Tensor, gate: tuple, up: tuple, hidden: int) -> torch.Tensor:
-    """The gradient of gated_mxfp4_cuda's x [M, hidden] from dh [M, I] and the gate_up that it kept. Has none of its own."""
+    """The gradient of gated_mxfp4_cuda's x [M, hidden] from dh [M, I] and the gate_up that it kept, d gate and d up rounded
+    to dh's type for the products (in fp16 after a power of two a row that keeps them in range). Has none of its own."""
     op = "gated_mxfp4_grad"
     if _mx_records(dh) or _mx_records(gate_up):
         return _MxNoGradient.apply(op, lambda: gated_mxfp4_grad_cuda(dh, gate_up, gate, up, hidden), dh, gate_up)

@@ -28,8 +28,9 @@ def fp16_gradient(dh, gate_up, wg, wu):
     return dg @ wg + du @ wu, err, top
 
 
-# Rows of one and several tiles, unsplit and split sums, N of whole 16-byte pieces and not, and past what a workgroup holds.
-FACTORS = [(1, 96, 160), (3, 4096, 160), (70, 33, 96), (300, 520, 1056), (2100, 264, 288), (2, 12331, 96), (5, 16504, 96)]
+# Rows of one and several tiles, unsplit and split sums, N of whole 16-byte pieces and not, past what a workgroup
+# holds, and more rows than workgroups.
+FACTORS = [(1, 96, 160), (3, 4096, 160), (70, 33, 96), (300, 520, 1056), (2100, 264, 288), (2, 12331, 96), (5, 16504, 96), (20000, 88, 32)]
 
 
 @pytest.mark.parametrize("m,n,k", FACTORS)
