@@ -393,6 +393,7 @@ struct mx_gated : torch::autograd::Function<mx_gated> {
         return {h, gate_up};
     }
     static variable_list backward(AutogradContext* ctx, variable_list dh) {
+        if (!dh[0].defined()) return variable_list(6);
         const variable_list w = ctx->get_saved_variables();
         return {gated_mxfp4_grad_cuda(dh[0].contiguous(), w[0], w[1], w[2], w[3], w[4], ctx->saved_data["k"].toInt()), {}, {}, {}, {}, {}};
     }

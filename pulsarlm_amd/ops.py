@@ -509,6 +509,8 @@ class _MxGated(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, _):
+        if dh is None:
+            return (None,) * 6
         gate_up, gate, gate_scale, up, up_scale = ctx.saved_tensors
         return gated_mxfp4_grad_cuda(dh.contiguous(), gate_up, (gate, gate_scale), (up, up_scale), ctx.k), *(None,) * 5
 

@@ -71,6 +71,28 @@ def test_feed_forward_block_through_autograd(layer):
     assert torch.equal(at.grad, dy + gated_grad(linear_grad(dy, *wd, n), gate_up, wg, wu, k))
 
 
+class Stop(torch.autograd.Function):
+    """A user's own function that hands no gradient back."""
+
+    @staticmethod
+    def forward(ctx, y):
+        return y.clone()
+
+    @staticmethod
+    def backward(ctx, dy):
+        return None
+
+
+@LAYERS
+def test_no_gradient_from_above_is_none_below(layer):
+    linear, _, gated, _, _, _ = layer
+    x, dy, wg, wu, _ = parts(20)
+    for f in (lambda x: linear(x, *wg, 96), lambda x: gated(x, wg, wu, 96)):
+        at = leaf(x)
+        Stop.apply(f(at)).backward(dy)
+        assert at.grad is None or not at.grad.any()
+
+
 @LAYERS
 def test_nothing_is_recorded_unasked(layer):
     linear, _, gated, _, w4a4, mlp = layer
