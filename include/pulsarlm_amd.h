@@ -334,6 +334,61 @@ int plm_mlp_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* gate_weight
                        int64_t m, int64_t n, int64_t k, void* y, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/*
+ * 8-bit integers with a scale for each row: tokens' activations, or a weight's output channels. x_scale[m] =
+ * max(amax(x[m, :]), 1e-12) / 127 in fp32, codes[m, k] the integer nearest to x[m, k] / x_scale[m] (the exact quotient),
+ * ties to even, so within [-127, 127]. A row with an infinity or NaN gets scale NaN and codes 0. x fp32, fp16 or bf16,
+ * K at most 2^28, any alignment; M below 2^24. plm_dequantize_rows_int8 is the inverse: codes times scale in fp32, rounded to
+ * out_dtype. The reference has no counterpart of these and the following entry points' formats.
+ */
+int plm_quantize_rows_int8(const void* x, plm_dtype x_dtype, int64_t m, int64_t k, int8_t* codes, float* x_scale, void* stream);
+int plm_dequantize_rows_int8(const int8_t* codes, const float* x_scale, int64_t m, int64_t k, void* out, plm_dtype out_dtype,
+                             void* stream);
+
+/*
+ * y [M, N] = x_scale[m] scale[n] sum_k codes[m, k] weight[n, k], rounded once to y_dtype (PLM_BF16 or PLM_FP16); the sum
+ * is exact. weight int8 [N, K] row-major, read in place, its scale fp32 [N]; any codes, -128 too. K a multiple of 16, at
+ * most 131056; N at most 2^19, M below 2^24, M N and M K at most 2^36. codes and weight 16-byte aligned, y at any
+ * element. M == 0 or N == 0 returns PLM_OK without touching y; K == 0 sets y to zero.
+ */
+int plm_gemm_int8(const int8_t* codes, const float* x_scale, const int8_t* weight, const float* scale, int64_t m, int64_t n,
+                  int64_t k, void* y, plm_dtype y_dtype, void* stream);
+
+/* W8A8: the same with 16-bit x [M, K], quantized on the way by the rule of plm_quantize_rows_int8. y has x's
+ * type. The workspace is 256-byte aligned; its contents need not be set and mean nothing after the call. */
+int64_t plm_gemm_int8_w8a8_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int plm_gemm_int8_w8a8(const void* x, plm_dtype x_dtype, const int8_t* weight, const float* scale, int64_t m, int64_t n,
+                       int64_t k, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The W8A8 product grouped by expert: rows [offsets[e-1], offsets[e]) of x (offsets int32 [n_experts] on the device,
+ * inclusive ends, as plm_grouped_gemm takes) times expert e's weight; weight int8 [n_experts, N, K], scale fp32
+ * [n_experts, N]. Offsets are taken within [0, rows], and one that is less than an earlier one as that one, so the experts'
+ * rows never overlap. Rows past the last expert's are set to zero where zero_rest is not 0, else not written.
+ * n_experts at most 4096, n_experts N K at most 2^38, n_experts N and n_experts K at most 2^28. Otherwise as plm_gemm_int8_w8a8.
+ */
+int64_t plm_grouped_gemm_int8_workspace_bytes(int64_t rows, int64_t n, int64_t k);
+int plm_grouped_gemm_int8(const void* x, plm_dtype x_dtype, const int8_t* weight, const float* scale, const int32_t* offsets,
+                          int64_t n_experts, int64_t rows, int64_t n, int64_t k, void* y, int zero_rest, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
+ * 16-bit experts, as the reference's at::_grouped_mm takes (pulsarlm-core/src/engine/model/paged_forward.cpp:124-125):
+ * rows [offsets[e-1], offsets[e]) of x [rows, K] times expert e's W^T, weight [n_experts, N, K] row-major in x's type,
+ * fp32 sums, rounded once. Offsets and the rows past the last expert's as plm_grouped_gemm_int8. K a multiple of 8; x and
+ * weight 16-byte aligned, y at any element; sizes as plm_grouped_gemm_int8. No workspace.
+ */
+int plm_grouped_gemm_16(const void* x, plm_dtype dtype, const void* weight, const int32_t* offsets, int64_t n_experts,
+                        int64_t rows, int64_t n, int64_t k, void* y, int zero_rest, void* stream);
+
+/* Its gradients from dy [rows, N]: dx [rows, K] = dy W_e, and dw [n_experts, N, K], expert e's the sum over its rows of
+ * dy[r, n] x[r, k], zero for an expert without rows; rows past the last expert's add to none. N and K multiples of 8, dy,
+ * x and weight 16-byte aligned, dx and dw at any element. Sums in fp32 in an order that does not depend on timing. */
+int plm_grouped_gemm_grad_x(const void* dy, plm_dtype dtype, const void* weight, const int32_t* offsets, int64_t n_experts,
+                            int64_t rows, int64_t n, int64_t k, void* dx, int zero_rest, void* stream);
+int plm_grouped_gemm_grad_w(const void* dy, const void* x, plm_dtype dtype, const int32_t* offsets, int64_t n_experts,
+                            int64_t rows, int64_t n, int64_t k, void* dw, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -58,6 +58,16 @@ SIGNATURES = {
     "plm_gated_mxfp4_grad": (_INT, [_P, _P, _INT, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
     "plm_mlp_mxfp4_w4a4_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "plm_mlp_mxfp4_w4a4": (_INT, [_P, _INT, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
+    "plm_quantize_rows_int8": (_INT, [_P, _INT, _I64, _I64, _P, _P, _P]),
+    "plm_dequantize_rows_int8": (_INT, [_P, _P, _I64, _I64, _P, _INT, _P]),
+    "plm_gemm_int8": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _INT, _P]),
+    "plm_gemm_int8_w8a8_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "plm_gemm_int8_w8a8": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
+    "plm_grouped_gemm_int8_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "plm_grouped_gemm_int8": (_INT, [_P, _INT, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _INT, _P, _SZ, _P]),
+    "plm_grouped_gemm_16": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _I64, _P, _INT, _P]),
+    "plm_grouped_gemm_grad_x": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _I64, _P, _INT, _P]),
+    "plm_grouped_gemm_grad_w": (_INT, [_P, _P, _INT, _P, _I64, _I64, _I64, _I64, _P, _P]),
     "plm_moe": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _INT, _I64, _P, _P, _P, _SZ,
                        _P]),
 }

@@ -1,0 +1,115 @@
+// The kernel of the products on unpacked weights (dense_gemm.hpp) for few rows, where the weights' bytes are what
+// counts: they go from memory to registers once, as the matrix instruction's A operand, and x's few rows, which the
+// caches hold, as its B operand.
+//
+// * A workgroup owns 16 MT rows by 16 NS columns. Its NW wavefronts take chunks of 64 U bytes of K in turn, each with the
+//   next chunk's loads in flight, and their sums meet in LDS in wavefront order: results do not depend on timing.
+#pragma once
+
+#include <algorithm>
+
+#include "dense_gemm.hpp"
+
+namespace plm {
+
+namespace {
+
+template <dense_type T, dense_mode MODE, int MT, int NS, int U, int NW>
+__global__ void __launch_bounds__(NW * 64) dense_rows_kernel(dense_args a) {
+    using acc_t = dense_acc<T>;
+    constexpr int SIZE = T == kInt8 ? 1 : 2, CHUNK = 64 * U, BM = 16 * MT;
+    constexpr int SHIFT = MT == 1 ? 4 : MT == 2 ? 5 : 6;
+    static_assert(1 << SHIFT == BM, "row blocks are powers of two");
+    __shared__ acc_t sums[NW][MT * NS][64];
+
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const int col16 = lane & 15, kq = lane >> 4;
+    const int nb = blockIdx.x % a.n_blocks, mb = blockIdx.x / a.n_blocks;
+    int row0 = mb * BM, rows = min(BM, a.rows - row0), expert = 0, depth = a.depth;
+    bool rest = false;  // rows of no expert: zeros, whatever scales they have
+    if constexpr (MODE == kByRows) {
+        if (mb >= count_blocks(a.offsets, a.experts, a.rows, a.zero_rest, SHIFT)) return;
+        const expert_range r = find_block(a.offsets, a.experts, a.rows, a.zero_rest, SHIFT, mb);
+        expert = r.expert, row0 = r.lo, rows = r.hi - r.lo;
+        if (expert == a.experts) rest = true, expert = 0, depth = 0;
+    }
+    const int col0 = nb * (16 * NS);
+    const int bytes = depth * SIZE, chunks = (bytes + CHUNK - 1) / CHUNK;
+
+    const uint8_t* q_base = a.q + (MODE == kByRows ? expert * a.q_expert : 0) + static_cast<int64_t>(col0) * a.pitch_q;
+    const __amdgpu_buffer_rsrc_t qr = make_rsrc(q_base, static_cast<uint32_t>(min(16 * NS, a.cols - col0)) * a.pitch_q);
+    const __amdgpu_buffer_rsrc_t pr = make_rsrc(a.p + static_cast<int64_t>(row0) * a.pitch_p, static_cast<uint32_t>(rows) * a.pitch_p);
+    const int q_at = col16 * a.pitch_q + kq * 16, p_at = col16 * a.pitch_p + kq * 16;
+
+    struct chunk {
+        u32x4_t q[NS][U], p[MT][U];
+    };
+    auto load = [&](chunk& c, int at) {  // chunk `at`; past the end zeros
+        const int from = at < chunks ? at * CHUNK : 0, left = bytes - at * CHUNK;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int past = u * 64 + kq * 16 < left ? u * 64 : kOOB;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) c.q[j][u] = buffer_load16_stream(qr, q_at + past, from + j * 16 * a.pitch_q);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) c.p[i][u] = buffer_load16(pr, p_at + past, from + i * 16 * a.pitch_p);
+        }
+    };
+    acc_t acc[MT][NS];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+    auto multiply = [&](const chunk& c) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) acc[i][j] = dense_mfma<T>(c.q[j][u], c.p[i][u], acc[i][j]);
+    };
+    chunk even, odd;
+    load(even, wave);
+    for (int c = wave; c < chunks; c += 2 * NW) {
+        load(odd, c + NW);
+        multiply(even);
+        load(even, c + 2 * NW);
+        multiply(odd);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) sums[wave][i * NS + j][lane] = acc[i][j];
+    __syncthreads();
+
+    auto finish = [&](auto bf16) {
+        constexpr bool BF16 = decltype(bf16)::value;
+        for (int s = wave; s < MT * NS; s += NW) {
+            const int i = s / NS, j = s % NS, r = i * 16 + col16, col = col0 + j * 16 + 4 * kq;
+            acc_t v = sums[0][s][lane];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) v = v + sums[w][s][lane];
+            if (r >= rows) continue;
+            f32x4_t f;
+            if constexpr (T == kInt8) f = dense_scaled(v, dense_channels(a.q_scale + static_cast<int64_t>(expert) * a.cols, col, a.cols), a.p_scale[row0 + r]);
+            else f = v;
+            if (T == kInt8 && rest) f = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            dense_store4<BF16>(a.y + (static_cast<int64_t>(row0) + r) * a.cols, col, a.cols, a.wide, f);
+        }
+    };
+    if constexpr (T == kBf16) finish(std::true_type{});
+    else if constexpr (T == kFp16) finish(std::false_type{});
+    else if (a.bf16) finish(std::true_type{});
+    else finish(std::false_type{});
+}
+
+template <dense_type T, dense_mode MODE, int MT, int NS, int U, int NW> void launch_rows(const dense_product& p, hipStream_t s) {
+    dense_args a = make_dense_args(p, false, false);
+    a.n_blocks = static_cast<int>(ceil_div(p.cols, 16 * NS));
+    a.m_blocks = static_cast<int>(dense_row_blocks(p, MODE, 16 * MT));
+    dense_rows_kernel<T, MODE, MT, NS, U, NW><<<static_cast<unsigned>(a.n_blocks) * a.m_blocks, NW * 64, 0, s>>>(a);
+}
+
+}  // namespace
+
+}  // namespace plm

@@ -1,0 +1,383 @@
+// The tile kernel of the products on unpacked weights (dense_gemm.hpp): a workgroup owns a tile of (WM MT 16) rows by
+// (WN NT 16) columns, its WM x WN wavefronts MT x NT products of 16 x 16 each.
+//
+// * A stage is 128 bytes of K (64 values in 16 bits, 128 in 8), two slices of the matrix instruction's. P's and Q's
+//   parts of it go from memory straight into LDS, into rings of S + PX and S. Where an operand lies along the sum, its
+//   rows are there with their 16-byte pieces XOR-swizzled by row; where it lies across (gradients), 64 rows of the sum's
+//   index, 32-byte pieces swizzled, and the fragments are read with the transposing LDS read.
+// * One barrier a stage, before its second slice's matrix instructions, whose operands are in registers by then: past it
+//   the stage's room is free for loads, and stage kt + 1 has landed and is read while they run.
+// * Q is the A operand and P the B operand: a lane ends with four neighbouring columns of a row.
+#pragma once
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+#include <utility>
+
+#include "dense_gemm.hpp"
+
+namespace plm {
+
+namespace {
+
+// 16 bytes a lane from memory straight to LDS, as buffer_load_lds16, but written out: the compiler would wait for every
+// such load in flight before a transposing LDS read, as it cannot tell their addresses apart. No register is written;
+// the kernel counts these loads itself. `lds` and `soffset` are wave-uniform.
+__device__ __forceinline__ void dma16(i32x4_t buffer, uint32_t lds, int lds_more, int voffset, int soffset) {
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds" ::"s"(lds), "i"(lds_more), "v"(voffset), "s"(buffer), "s"(soffset) : "memory", "scc");
+}
+// make_rsrc's four words: a raw buffer of `bytes` from a wave-uniform address.
+__device__ __forceinline__ i32x4_t buffer_words(const uint8_t* base, uint32_t bytes) {
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    return i32x4_t{static_cast<int>(at), static_cast<int>(at >> 32) & 0xffff, static_cast<int>(bytes), 0x00020000};
+}
+
+typedef __attribute__((ext_vector_type(4))) short tr16_t;
+
+// f(integral_constant<int, 0>) .. f(integral_constant<int, N - 1>).
+template <typename F, int... I> __device__ __forceinline__ void unrolled_(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F> __device__ __forceinline__ void unrolled(F f) {
+    unrolled_(f, std::make_integer_sequence<int, N>{});
+}
+
+
+// One operand: BLOCK rows or columns of the tile.
+template <bool CROSS, int BLOCK, int NW> struct dense_operand {
+    static constexpr int kBytes = BLOCK * 128;          // of a stage
+    static constexpr int kLoads = kBytes / 1024 / NW;   // of a wavefront
+    static_assert(kBytes % (1024 * NW) == 0, "every wavefront loads as much");
+    // Along: 8 rows a load. Across: rows of the sum's index, BLOCK values each.
+    static constexpr int kPitch = CROSS ? BLOCK * 2 : 128;
+    static constexpr int kRowsLoad = 1024 / kPitch;
+    static_assert(!CROSS || (NW * kRowsLoad) % 8 == 0, "the swizzle repeats");
+};
+
+// Across: piece (32 bytes) c of the sum's row k lies at piece c ^ f(k), so that the rows and pieces that 32 lanes of a
+// transposing read touch fall on different banks.
+__device__ __forceinline__ constexpr int cross_swizzle(int k, int pieces) {
+    return pieces >= 8 ? (k & 3) << 1 | (((k >> 2) ^ (k >> 3)) & 1) : (k & 2) | ((k >> 3) & 1);
+}
+
+template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX>
+__global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) {
+    constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
+    using P = dense_operand<PC, BM, NW>;
+    using Q = dense_operand<QC, BN, NW>;
+    using acc_t = dense_acc<T>;
+    constexpr int P_RING = (S + PX) * P::kBytes, LDS = P_RING + S * Q::kBytes;
+    constexpr int SIZE = T == kInt8 ? 1 : 2;
+    constexpr int DEPTH = 128 / SIZE;  // of the sum, a stage
+    static_assert(T != kInt8 || (!PC && !QC), "8-bit operands lie along the sum");
+    static_assert(LDS <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
+
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN, col16 = lane & 15, kq = lane >> 4;
+
+    // The workgroup's tile. Workgroups go round the 8 XCDs by id: each takes one run of the tiles, which are ordered in
+    // bands of `band` row blocks, row block fastest, so that an XCD's L2 holds what its tiles share.
+    constexpr int SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : BM == 64 ? 6 : 5;
+    static_assert(1 << SHIFT == BM, "row blocks are powers of two");
+    int m_blocks = a.m_blocks;
+    if constexpr (MODE == kByRows) m_blocks = count_blocks(a.offsets, a.experts, a.rows, a.zero_rest, SHIFT);
+    const int per_expert = m_blocks * a.n_blocks, tiles = MODE == kByRanges ? per_expert * a.experts : per_expert;
+    const int id = blockIdx.x;
+    if (id >= tiles) return;
+    const int xcd = id & 7;
+    int lin = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (id >> 3);
+    int expert = 0;
+    if constexpr (MODE == kByRanges) expert = lin / per_expert, lin -= expert * per_expert;
+    const int band0 = lin / (a.band * a.n_blocks) * a.band;
+    const int band_rows = min(a.band, m_blocks - band0), in_band = lin - band0 * a.n_blocks;
+    const int nb = in_band / band_rows, mb = band0 + in_band % band_rows;
+    int row0 = mb * BM, rows = min(BM, a.rows - row0), first = 0, depth = a.depth;
+    bool rest = false;  // rows of no expert: zeros, whatever scales they have
+    if constexpr (MODE == kByRows) {
+        const expert_range r = find_block(a.offsets, a.experts, a.rows, a.zero_rest, SHIFT, mb);
+        expert = r.expert, row0 = r.lo, rows = r.hi - r.lo;
+        if (expert == a.experts) rest = true, expert = 0, depth = 0;
+    } else if constexpr (MODE == kByRanges) {
+        const expert_range r = find_expert(a.offsets, expert, a.depth);
+        first = r.lo, depth = r.hi - r.lo;
+    }
+    const int col0 = nb * BN;
+    const int stages = (depth + DEPTH - 1) / DEPTH;
+
+    // Operands. Along: the tile's rows from the first on, the range check ends past the last. Across: the sum's rows
+    // from the first on; a stage's base moves with it, as all of them can pass 2 GiB.
+    const uint8_t* p_base = a.p + (PC ? static_cast<int64_t>(first) * a.pitch_p + row0 * 2 : static_cast<int64_t>(row0) * a.pitch_p);
+    const uint8_t* q_base = a.q + (MODE == kByRows ? expert * a.q_expert : 0) +
+                            (QC ? static_cast<int64_t>(first) * a.pitch_q + col0 * 2 : static_cast<int64_t>(col0) * a.pitch_q);
+    const int q_rows = min(BN, a.cols - col0);
+    // Along: the lane's row and 16-byte piece of a load, swizzled.
+    const int along_row = lane >> 3, along_piece = (lane & 7) ^ along_row;
+    // Across: its row of the sum and where its 16 bytes lie in it; the swizzle of loads an odd number apart differs by 4
+    // where a turn of the wavefronts is 8 rows.
+    auto across = [&](auto operand, int parity, int limit) {
+        using O = decltype(operand);
+        const int r = lane * 16 / O::kPitch, at = lane * 16 % O::kPitch;
+        const int k = (parity * NW + wave) * O::kRowsLoad + r;
+        const int bytes = (((at >> 5) ^ cross_swizzle(k, O::kPitch / 32)) << 5) + (at & 16);
+        return bytes < limit * 2 ? bytes : kOOB;
+    };
+    int p_cross[2], q_cross[2];
+    if constexpr (PC) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) p_cross[i] = across(P{}, i, rows) + lane * 16 / P::kPitch * a.pitch_p;
+    }
+    if constexpr (QC) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) q_cross[i] = across(Q{}, i, q_rows) + lane * 16 / Q::kPitch * a.pitch_q;
+    }
+
+    // What a stage's loads of an operand have in common: its buffer, from the stage's part of the sum on, and the lanes'
+    // offsets. A load's range check covers both its offsets: past the end of the sum, or of the operand, zeros are written.
+    struct source {
+        i32x4_t buffer;
+        int v[2];  // of even and odd loads
+    };
+    auto along = [&](int kt, const uint8_t* base, int block_rows, int pitch) {
+        const int left = depth * SIZE - kt * 128;  // bytes of the sum
+        const int v = along_piece * 16 < left ? along_row * pitch + along_piece * 16 : kOOB;
+        return source{buffer_words(base + kt * 128, left > 0 ? static_cast<uint32_t>(block_rows) * pitch - kt * 128 : 0u), {v, v}};
+    };
+    auto cross = [&](int kt, const uint8_t* base, int pitch, int column, const int (&v)[2]) {
+        const int left = min(depth - kt * DEPTH, DEPTH);
+        return source{buffer_words(base + static_cast<int64_t>(kt) * DEPTH * pitch, left > 0 ? static_cast<uint32_t>(left) * pitch - column * 2 : 0u), {v[0], v[1]}};
+    };
+    auto source_p = [&](int kt) {
+        if constexpr (PC) return cross(kt, p_base, a.pitch_p, row0, p_cross);
+        else return along(kt, p_base, rows, a.pitch_p);
+    };
+    auto source_q = [&](int kt) {
+        if constexpr (QC) return cross(kt, q_base, a.pitch_q, col0, q_cross);
+        else return along(kt, q_base, q_rows, a.pitch_q);
+    };
+    // Load l of the wavefront's.
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds)) + wave * 1024;
+    auto issue_p = [&](const source& s, auto l, int slot) {
+        constexpr int n = decltype(l)::value;
+        dma16(s.buffer, lds0 + slot * P::kBytes, n * NW * 1024, s.v[n & 1], (n * NW + wave) * P::kRowsLoad * a.pitch_p);
+    };
+    auto issue_q = [&](const source& s, auto l, int slot) {
+        constexpr int n = decltype(l)::value;
+        dma16(s.buffer, lds0 + slot * Q::kBytes, P_RING + n * NW * 1024, s.v[n & 1], (n * NW + wave) * Q::kRowsLoad * a.pitch_q);
+    };
+
+    // Fragment f of slice t.
+    auto read_along = [&](const uint8_t* base, int f, int t) {
+        return *reinterpret_cast<const u32x4_t*>(base + (f * 16 + col16) * 128 + (((4 * t + kq) ^ (col16 & 7)) << 4));
+    };
+    auto read_across = [&](const uint8_t* base, int f, int t, auto operand) {
+        using O = decltype(operand);
+        const int k = 32 * t + 8 * kq + (col16 >> 2);
+        const uint8_t* at = base + k * O::kPitch + (col16 & 3) * 8;
+        const int s = cross_swizzle(k, O::kPitch / 32), s4 = cross_swizzle(k + 4, O::kPitch / 32);
+        const tr16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr16_t*)(at + ((f ^ s) << 5)));
+        const tr16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr16_t*)(at + 4 * O::kPitch + ((f ^ s4) << 5)));
+        const u32x2_t l = __builtin_bit_cast(u32x2_t, lo), h = __builtin_bit_cast(u32x2_t, hi);
+        return u32x4_t{l[0], l[1], h[0], h[1]};
+    };
+    auto read_p = [&](int f, int slot, int t) {
+        const uint8_t* base = lds + slot * P::kBytes;
+        if constexpr (PC) return read_across(base, wm * MT + f, t, P{});
+        else return read_along(base, wm * MT + f, t);
+    };
+    auto read_q = [&](int f, int slot, int t) {
+        const uint8_t* base = lds + P_RING + slot * Q::kBytes;
+        if constexpr (QC) return read_across(base, wn * NT + f, t, Q{});
+        else return read_along(base, wn * NT + f, t);
+    };
+
+    acc_t acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+
+    // Q's loads of stage kt + S follow the barrier of stage kt, among the matrix instructions of its second slice: the
+    // memory pipeline takes a load in 16 cycles, one pipeline a CU, and a wavefront that waits for it leaves its matrix
+    // unit idle. With PX, P's loads of stage kt + S + 1 stand in the next stage's first slice: both slices' time is the
+    // pipeline's then, and they have a slice more to land.
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const source from_p = source_p(s), from_q = source_q(s);
+        unrolled<P::kLoads>([&](auto l) { issue_p(from_p, l, s); });
+        unrolled<Q::kLoads>([&](auto l) { issue_q(from_q, l, s); });
+    }
+    // Stage 0 has landed; later, at stage kt's barrier, stage kt + 1, when only these are left:
+    constexpr int LEFT = (S - 2) * (P::kLoads + Q::kLoads) + PX * P::kLoads, LEFT0 = (S - 1) * (P::kLoads + Q::kLoads);
+    static_assert(S >= 2 && LEFT0 <= 63 && LEFT <= 63, "the counter's range");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LEFT0) : "memory");
+    u32x4_t p[2][MT], q[2][NT];
+#pragma unroll
+    for (int f = 0; f < MT; ++f) p[0][f] = read_p(f, 0, 0);
+#pragma unroll
+    for (int f = 0; f < NT; ++f) q[0][f] = read_q(f, 0, 0);
+    int ps = 0, qs = 0, p_to = S;  // the stage's slots, and with PX where P's next loads go
+    // One slice of stage kt. Among its matrix instructions, one behind each, stand the reads of the next slice's
+    // fragments, over the first three quarters, so that they are there when it begins, and the loads: a wavefront issues
+    // in order, and two such in a row would take longer than a matrix instruction and leave its unit idle.
+    constexpr int STEPS = MT * NT, READS = MT + NT, EARLY = STEPS * 3 / 4;
+    auto slice = [&](auto second, int kt) {
+        constexpr int t = decltype(second)::value;
+        constexpr int PL = PX != t ? P::kLoads : 0, QL = t ? Q::kLoads : 0, LOADS = PL + QL;
+        const int pn = t ? (ps + 1 == S + PX ? 0 : ps + 1) : ps, qn = t ? (qs + 1 == S ? 0 : qs + 1) : qs;
+        source from_p, from_q;
+        if constexpr (PL > 0) from_p = source_p(kt + S);
+        if constexpr (QL > 0) from_q = source_q(kt + S);
+        if constexpr (t) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+        unrolled<STEPS>([&](auto step) {
+            constexpr int s = decltype(step)::value, i = s / NT, j = s % NT;
+            acc[i][j] = dense_mfma<T>(q[t][j], p[t][i], acc[i][j]);
+            unrolled<READS>([&](auto read) {
+                constexpr int f = decltype(read)::value;
+                if constexpr (f * EARLY / READS == s) {
+                    if constexpr (f < NT) q[t ^ 1][f] = read_q(f, qn, t ^ 1);
+                    else p[t ^ 1][f - NT] = read_p(f - NT, pn, t ^ 1);
+                }
+            });
+            unrolled<LOADS>([&](auto load) {
+                constexpr int l = decltype(load)::value;
+                if constexpr (std::min(l * STEPS / LOADS + 1, STEPS - 1) == s) {
+                    if constexpr (l < PL) issue_p(from_p, load, PX ? p_to : ps);
+                    else issue_q(from_q, std::integral_constant<int, l - PL>{}, qs);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (t) {
+            p_to = ps;
+            ps = pn, qs = qn;
+        }
+    };
+    for (int kt = 0; kt < stages; ++kt) {
+        slice(std::integral_constant<int, 0>{}, kt);
+        slice(std::integral_constant<int, 1>{}, kt);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // requests past the end; LDS is free
+
+    // A lane has four columns of one row, a quarter of a 32-byte piece. RB row blocks at a time go through the
+    // wavefront's own part of LDS (pitch padded by 16 bytes) and leave as 16 bytes a lane, whole rows of its tile.
+    auto finish = [&](auto bf16) {
+        constexpr bool BF16 = decltype(bf16)::value;
+        constexpr int COLS = NT * 16, PITCH = COLS * 2 + 16, CH = COLS / 8;
+        constexpr int FIT = LDS / (NW * 16 * PITCH), RB = FIT >= MT ? MT : (FIT >= 4 ? 4 : (FIT >= 2 ? 2 : 1));
+        static_assert(FIT >= 1 && MT % RB == 0, "the rows fit");
+        uint8_t* mine = lds + wave * RB * 16 * PITCH;
+        const int c0 = col0 + wn * COLS;
+        uint16_t* y = a.y + (MODE == kByRanges ? expert * static_cast<int64_t>(a.rows) * a.cols : 0);
+        f32x4_t channel[NT];
+        if constexpr (T == kInt8)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) channel[j] = dense_channels(a.q_scale + static_cast<int64_t>(expert) * a.cols, c0 + j * 16 + 4 * kq, a.cols);
+        auto token = [&](int i) {
+            const int r = (wm * MT + i) * 16 + col16;
+            return T == kInt8 && r < rows ? a.p_scale[row0 + r] : 0.f;
+        };
+        auto value = [&](int i, int j, float tok) {
+            if constexpr (T == kInt8) return rest ? f32x4_t{0.f, 0.f, 0.f, 0.f} : dense_scaled(acc[i][j], channel[j], tok);
+            else return acc[i][j];
+        };
+        if (!a.lines) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int r = (wm * MT + i) * 16 + col16;
+                const float tok = token(i);
+                if (r < rows)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        dense_store4<BF16>(y + (static_cast<int64_t>(row0) + r) * a.cols, c0 + j * 16 + 4 * kq, a.cols, a.wide, value(i, j, tok));
+            }
+            return;
+        }
+#pragma unroll
+        for (int i0 = 0; i0 < MT; i0 += RB) {
+            const int r0 = (wm * MT + i0) * 16;
+            if (r0 >= rows) break;
+#pragma unroll
+            for (int i = i0; i < i0 + RB; ++i) {
+                const float tok = token(i);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    *reinterpret_cast<uint2*>(mine + ((i - i0) * 16 + col16) * PITCH + (j * 16 + 4 * kq) * 2) = dense_pack<BF16>(value(i, j, tok));
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int s = 0; s < RB * 16 * CH; s += 64) {
+                const int c = s + lane, r = c / CH, col = c0 + c % CH * 8;
+                if (c < RB * 16 * CH && r0 + r < rows && col < a.cols)
+                    *reinterpret_cast<u32x4_t*>(y + (static_cast<int64_t>(row0) + r0 + r) * a.cols + col) =
+                        *reinterpret_cast<const u32x4_t*>(mine + r * PITCH + c % CH * 16);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    };
+    if constexpr (T == kBf16) finish(std::true_type{});
+    else if constexpr (T == kFp16) finish(std::false_type{});
+    else if (a.bf16) finish(std::true_type{});
+    else finish(std::false_type{});
+}
+
+template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX>
+void launch_tile(const dense_product& p, hipStream_t s) {
+    constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
+    dense_args a = make_dense_args(p, PC, QC);
+    a.band = 8;
+    a.n_blocks = static_cast<int>(ceil_div(p.cols, BN));
+    a.m_blocks = static_cast<int>(dense_row_blocks(p, MODE, BM));
+    const int64_t tiles = int64_t{1} * a.m_blocks * a.n_blocks * (MODE == kByRanges ? p.experts : 1);
+    dense_tile_kernel<T, MODE, PC, QC, WM, WN, MT, NT, S, PX><<<static_cast<unsigned>(tiles), WM * WN * 64, 0, s>>>(a);
+}
+
+// The tile shapes, and which of them takes a call: the least of rounds x stages x time of a stage. The times (us) were
+// measured with one workgroup on the GPU and with every slot taken; between the two they grow with the share of slots
+// taken, as the workgroups share the L2s and the clock.
+// {rows, columns, threads, workgroups a CU, lone, full}
+struct dense_cost {
+    int rows, cols, threads, per_cu;
+    double lone, full;
+};
+constexpr dense_cost kDenseTiles[] = {
+    {256, 256, 512, 1, 1.0, 1.6}, {128, 256, 512, 1, 0.6, 0.9}, {128, 128, 256, 2, 0.45, 0.9}, {64, 128, 256, 2, 0.3, 0.5}, {64, 64, 256, 2, 0.25, 0.35}};
+
+// By rows, how many blocks there are is known on the device only: with parts of unknown sizes, half a block of each
+// expert is taken to be empty.
+inline int choose_dense_tile(const dense_product& p, dense_mode mode) {
+    const int64_t depth = mode == kByRanges ? ceil_div(p.depth, p.experts) : p.depth;
+    const int64_t stages = std::max<int64_t>(1, ceil_div(depth * (p.type == kInt8 ? 1 : 2), 128));
+    int best = 0;
+    double least = 1e300;
+    const int forced = knobs().dense_tile;
+    for (int i = 0; i < 5; ++i) {
+        const dense_cost& c = kDenseTiles[i];
+        const int64_t cols = ceil_div(p.cols, c.cols), experts = mode == kByRanges ? p.experts : 1;
+        if (forced >= 0 && i != forced && i > 0) continue;
+        if (i > 0 && !dense_grid_fits(dense_row_blocks(p, mode, c.rows) * cols * experts, c.threads)) continue;
+        const double blocks = mode == kByRows ? static_cast<double>(p.rows) / c.rows + 0.5 * std::min(p.rows, p.experts)
+                                              : static_cast<double>(ceil_div(p.rows, c.rows) * experts);
+        const double tiles = blocks * cols, slots = static_cast<double>(c.per_cu) * cu_count();
+        const double fill = std::min(1.0, tiles / slots);
+        const double rounds = mode == kDense ? std::ceil(tiles / slots) : std::max(1.0, tiles / slots);
+        const double t = rounds * (stages + 4) * (c.lone + (c.full - c.lone) * fill);
+        if (t < least || i == forced) least = t, best = i;
+    }
+    return best;
+}
+
+template <dense_type T, dense_mode MODE, bool PC, bool QC> void launch_shape(const dense_product& p, hipStream_t s) {
+    switch (choose_dense_tile(p, MODE)) {
+        case 0: return launch_tile<T, MODE, PC, QC, 2, 4, 8, 4, 2, 1>(p, s);
+        case 1: return launch_tile<T, MODE, PC, QC, 2, 4, 4, 4, 3, 0>(p, s);
+        case 2: return launch_tile<T, MODE, PC, QC, 2, 2, 4, 4, 2, 0>(p, s);
+        case 3: return launch_tile<T, MODE, PC, QC, 2, 2, 2, 4, 3, 0>(p, s);
+        default: return launch_tile<T, MODE, PC, QC, 2, 2, 2, 2, 4, 0>(p, s);
+    }
+}
+
+}  // namespace
+
+}  // namespace plm

@@ -82,6 +82,11 @@ tuning parse_tuning() {
     if (const char* e = env("PLM_MOE_SMALL_SORT")) t.moe_small_sort_off = e[0] == '0';
     t.moe_unfused = env("PLM_MOE_UNFUSED") != nullptr;
     if (const char* e = env("PLM_MOE_PERSIST")) t.moe_persist = e[0] == '1';
+    if (const char* e = env("PLM_DENSE")) {
+        const int v = e[0] != 0 ? atoi(e + 1) : -1;
+        if (e[0] == 't' && v >= 0 && v < 5) t.dense_tile = v, t.dense_rows = 0;
+        if (e[0] == 'r' && (v == 0 || v == 16 || v == 32 || v == 64)) t.dense_rows = v;
+    }
     return t;
 }
 std::mutex g_tuning_mutex;

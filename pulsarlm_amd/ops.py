@@ -532,6 +532,10 @@ def _mx_records(x: torch.Tensor) -> bool:
     return x.requires_grad and torch.is_grad_enabled()
 
 
+def _records(*inputs: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in inputs)
+
+
 def _mx_x(op: str, x: torch.Tensor):
     _mx_contiguous(op, "x", x, _HALF)
     _require(x.shape[1] % 32 == 0, op, "K must be a multiple of 32")
@@ -647,3 +651,202 @@ def mlp_mxfp4_w4a4_cuda(x: torch.Tensor, gate: tuple, up: tuple, down: tuple, in
               _ptr(down[0]), _ptr(down[1]), m, intermediate, k, _ptr(y), _ptr(ws), 0 if ws is None else ws.numel(),
               _stream(x.device))
     return y
+
+
+# ---------------------------------------------------------------------------
+# 8-bit integers with a scale for each token and channel, and experts in 8 and 16 bits (formats that the reference has no
+# kernels of its own for). Weights are row-major and read in place: int8 [N, K] with scale fp32 [N], or 16-bit; by expert
+# [E, N, K]. A grouped call's rows are sorted by expert, offsets int32 [E] their inclusive ends, as in grouped_gemm_int4_cuda.
+# ---------------------------------------------------------------------------
+
+
+def quantize_rows_int8_cuda(x: torch.Tensor):
+    """x [M, K] (fp32, fp16 or bf16; tokens, or a weight's output channels) -> (codes int8 [M, K], scale fp32 [M]): scale
+    max(amax, 1e-12) / 127, codes the integers nearest to x / scale, ties to even. A row with an infinity or NaN gets scale
+    NaN and codes 0. Has no gradient: a backward pass that reaches it raises."""
+    op = "quantize_rows_int8"
+    if _mx_records(x):
+        return _MxNoGradient.apply(op, lambda: quantize_rows_int8_cuda(x), x)
+    _mx_contiguous(op, "x", x, _DTYPES)
+    m, k = x.shape
+    codes = torch.empty((m, k), dtype=torch.int8, device=x.device)
+    scale = torch.empty((m,), dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        _call("plm_quantize_rows_int8", _ptr(x), _DTYPES[x.dtype], m, k, _ptr(codes), _ptr(scale), _stream(x.device))
+    return codes, scale
+
+
+def _int8_codes(op: str, name: str, codes: torch.Tensor, scale: torch.Tensor, dim: int) -> None:
+    if not (codes.is_cuda and codes.dtype is torch.int8 and codes.dim() == dim and codes.is_contiguous()):
+        _require(False, op, f"{name} must be a contiguous CUDA int8 tensor of {dim} dimensions")
+    if not (scale.dtype is torch.float32 and scale.get_device() == codes.get_device() and scale.shape == codes.shape[:-1] and scale.is_contiguous()):
+        _require(False, op, f"{name}'s scale must be contiguous fp32, one for each row, on its device")
+
+
+def dequantize_rows_int8_cuda(codes: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values [M, K] that codes and scale stand for: their product in fp32, rounded to dtype. Has no gradient."""
+    op = "dequantize_rows_int8"
+    if _mx_records(scale):
+        return _MxNoGradient.apply(op, lambda: dequantize_rows_int8_cuda(codes, scale, dtype), scale)
+    _int8_codes(op, "codes", codes, scale, 2)
+    _require(dtype in _DTYPES, op, "dtype must be fp32, fp16 or bf16")
+    m, k = codes.shape
+    out = torch.empty((m, k), dtype=dtype, device=codes.device)
+    with _on(codes.device):
+        _call("plm_dequantize_rows_int8", _ptr(codes), _ptr(scale), m, k, _ptr(out), _DTYPES[dtype], _stream(codes.device))
+    return out
+
+
+def _int8_out(op: str, like: torch.Tensor, dtype, shape, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    _require(out.dtype == dtype and out.device == like.device and tuple(out.shape) == shape and out.is_contiguous(), op,
+             f"out must be contiguous {list(shape)} of type {dtype} on the inputs' device")
+    return out
+
+
+def gemm_int8_cuda(codes: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16,
+                   out=None) -> torch.Tensor:
+    """y [M, N] = x_scale[m] scale[n] sum_k codes[m, k] weight[n, k] in dtype (fp16 or bf16), the sums exact: int8 codes
+    [M, K] and x_scale fp32 [M] as quantize_rows_int8_cuda makes them, weight int8 [N, K] and scale fp32 [N]. K a multiple of
+    16. Has no gradient."""
+    op = "gemm_int8"
+    if _records(x_scale, scale):
+        _require(out is None, op, "out records no gradient")
+        return _MxNoGradient.apply(op, lambda: gemm_int8_cuda(codes, x_scale, weight, scale, dtype), x_scale, scale)
+    _int8_codes(op, "codes", codes, x_scale, 2)
+    _int8_codes(op, "weight", weight, scale, 2)
+    m, k = codes.shape
+    n = weight.shape[0]
+    _require(weight.shape[1] == k and weight.get_device() == codes.get_device(), op, "weight must be [N, K] for codes [M, K], on their device")
+    _require(dtype in _HALF, op, "dtype must be fp16 or bf16")
+    y = _int8_out(op, codes, dtype, (m, n), out)
+    with _on(codes.device):
+        _call("plm_gemm_int8", _ptr(codes), _ptr(x_scale), _ptr(weight), _ptr(scale), m, n, k, _ptr(y), _DTYPES[dtype], _stream(codes.device))
+    return y
+
+
+def gemm_int8_w8a8_cuda(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, out=None) -> torch.Tensor:
+    """W8A8: gemm_int8_cuda with 16-bit x [M, K], quantized on the way as by quantize_rows_int8_cuda; y in x's type. out may
+    not overlap x. Has no gradient: a backward pass that reaches it raises."""
+    op = "gemm_int8_w8a8"
+    if _records(x, scale):
+        _require(out is None, op, "out records no gradient")
+        return _MxNoGradient.apply(op, lambda: gemm_int8_w8a8_cuda(x, weight, scale), x, scale)
+    _mx_contiguous(op, "x", x, _HALF)
+    _int8_codes(op, "weight", weight, scale, 2)
+    m, k = x.shape
+    n = weight.shape[0]
+    _require(weight.shape[1] == k and weight.get_device() == x.get_device(), op, "weight must be [N, K] for x [M, K], on its device")
+    y = _mx_out(op, x, (m, n), out)
+    ws = _mx_scratch(op, x, m, n, k)
+    with _on(x.device):
+        _call("plm_gemm_int8_w8a8", _ptr(x), _DTYPES[x.dtype], _ptr(weight), _ptr(scale), m, n, k, _ptr(y), _ptr(ws),
+              0 if ws is None else ws.numel(), _stream(x.device))
+    return y
+
+
+def _expert_offsets(op: str, x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> None:
+    _require(weight.get_device() == x.get_device() and offsets.get_device() == x.get_device(), op, "x, weight and offsets must be on one device")
+    if not (offsets.dtype is torch.int32 and offsets.shape == weight.shape[:1] and offsets.is_contiguous()):
+        _require(False, op, "offsets must be contiguous int32 [E]")
+
+
+def grouped_gemm_int8_cuda(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, offsets: torch.Tensor, out=None) -> torch.Tensor:
+    """Rows [offsets[e-1], offsets[e]) of x times expert e's W^T, W8A8 as gemm_int8_w8a8_cuda: weight int8 [E, N, K], scale
+    fp32 [E, N]. Rows past the last expert's are left as they were in out, and zero in a new tensor. Has no gradient: a
+    backward pass that reaches it raises."""
+    op = "grouped_gemm_int8"
+    if _records(x, scale):
+        _require(out is None, op, "out records no gradient")
+        return _MxNoGradient.apply(op, lambda: grouped_gemm_int8_cuda(x, weight, scale, offsets), x, scale)
+    _mx_contiguous(op, "x", x, _HALF)
+    _int8_codes(op, "weight", weight, scale, 3)
+    _expert_offsets(op, x, weight, offsets)
+    rows, k = x.shape
+    e, n = scale.shape
+    _require(weight.shape[2] == k, op, "weight must be [E, N, K] for x [rows, K]")
+    y = _mx_out(op, x, (rows, n), out)
+    ws = _mx_scratch(op, x, rows, n, k)
+    with _on(x.device):
+        _call("plm_grouped_gemm_int8", _ptr(x), _DTYPES[x.dtype], _ptr(weight), _ptr(scale), _ptr(offsets), e, rows, n, k, _ptr(y),
+              int(out is None), _ptr(ws), 0 if ws is None else ws.numel(), _stream(x.device))
+    return y
+
+
+class _Grouped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets):
+        ctx.save_for_backward(x, weight, offsets)
+        return grouped_gemm_cuda(x, weight, offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, offsets = ctx.saved_tensors
+        dy = dy.contiguous()
+        dx = grouped_gemm_grad_x_cuda(dy, weight, offsets) if ctx.needs_input_grad[0] else None
+        dw = grouped_gemm_grad_w_cuda(dy, x, offsets) if ctx.needs_input_grad[1] else None
+        return dx, dw, None
+
+
+def _expert_weight(op: str, x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> None:
+    if not (weight.dim() == 3 and weight.dtype == x.dtype and weight.is_contiguous()):
+        _require(False, op, "weight must be contiguous [E, N, K] of the rows' type")
+    _expert_offsets(op, x, weight, offsets)
+
+
+def grouped_gemm_cuda(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, out=None) -> torch.Tensor:
+    """Rows [offsets[e-1], offsets[e]) of x [rows, K] times expert e's W^T, 16-bit weight [E, N, K] of x's type (one
+    at::_grouped_mm of paged_forward.cpp:124-125), fp32 sums. Rows past the last expert's are left as they were in out, and
+    zero in a new tensor. K a multiple of 8, for the gradients N, too. Differentiable in x and weight, without out."""
+    op = "grouped_gemm"
+    if _records(x, weight):
+        _require(out is None, op, "out records no gradient")
+        _require(weight.dim() != 3 or weight.shape[1] % 8 == 0, op, "N must be a multiple of 8 for the gradients")
+        return _Grouped.apply(x, weight, offsets)
+    _mx_contiguous(op, "x", x, _HALF)
+    _expert_weight(op, x, weight, offsets)
+    rows, k = x.shape
+    e, n = weight.shape[:2]
+    _require(weight.shape[2] == k, op, "weight must be [E, N, K] for x [rows, K]")
+    y = _mx_out(op, x, (rows, n), out)
+    with _on(x.device):
+        _call("plm_grouped_gemm_16", _ptr(x), _DTYPES[x.dtype], _ptr(weight), _ptr(offsets), e, rows, n, k, _ptr(y), int(out is None), _stream(x.device))
+    return y
+
+
+def grouped_gemm_grad_x_cuda(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """The gradient of grouped_gemm_cuda's x: dx [rows, K] = dy [rows, N] W_e, zero past the last expert's rows. N and K
+    multiples of 8. Has none of its own."""
+    op = "grouped_gemm_grad_x"
+    if _records(dy, weight):
+        return _MxNoGradient.apply(op, lambda: grouped_gemm_grad_x_cuda(dy, weight, offsets), dy, weight)
+    _mx_contiguous(op, "dy", dy, _HALF)
+    _expert_weight(op, dy, weight, offsets)
+    rows, n = dy.shape
+    e, k = weight.shape[0], weight.shape[2]
+    _require(weight.shape[1] == n, op, "weight must be [E, N, K] for dy [rows, N]")
+    dx = dy.new_empty((rows, k))
+    with _on(dy.device):
+        _call("plm_grouped_gemm_grad_x", _ptr(dy), _DTYPES[dy.dtype], _ptr(weight), _ptr(offsets), e, rows, n, k, _ptr(dx), 1, _stream(dy.device))
+    return dx
+
+
+def grouped_gemm_grad_w_cuda(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """The gradient of grouped_gemm_cuda's weight: dw [E, N, K], expert e's the sum over its rows of dy[r, n] x[r, k], zero
+    for an expert without rows. N and K multiples of 8. Has none of its own."""
+    op = "grouped_gemm_grad_w"
+    if _records(dy, x):
+        return _MxNoGradient.apply(op, lambda: grouped_gemm_grad_w_cuda(dy, x, offsets), dy, x)
+    _mx_contiguous(op, "dy", dy, _HALF)
+    _mx_contiguous(op, "x", x, _HALF)
+    _require(x.dtype == dy.dtype and x.shape[0] == dy.shape[0], op, "dy and x must have one type and as many rows")
+    _require(offsets.dim() == 1, op, "offsets must be contiguous int32 [E]")
+    e, (rows, n), k = offsets.shape[0], dy.shape, x.shape[1]
+    dw = dy.new_empty((e, n, k))
+    _expert_offsets(op, dy, dw, offsets)
+    _require(x.get_device() == dy.get_device(), op, "dy, x and offsets must be on one device")
+    with _on(dy.device):
+        _call("plm_grouped_gemm_grad_w", _ptr(dy), _ptr(x), _DTYPES[dy.dtype], _ptr(offsets), e, rows, n, k, _ptr(dw), _stream(dy.device))
+    return dw
