@@ -349,13 +349,16 @@ int plm_dequantize_rows_int8(const int8_t* codes, const float* x_scale, int64_t 
  * y [M, N] = x_scale[m] scale[n] sum_k codes[m, k] weight[n, k], rounded once to y_dtype (PLM_BF16 or PLM_FP16); the sum
  * is exact. weight int8 [N, K] row-major, read in place, its scale fp32 [N]; any codes, -128 too. K a multiple of 16, at
  * most 131056; N at most 2^19, M below 2^24, M N and M K at most 2^36. codes and weight 16-byte aligned, y at any
- * element. M == 0 or N == 0 returns PLM_OK without touching y; K == 0 sets y to zero.
+ * element. M == 0 or N == 0 returns PLM_OK without touching y; K == 0 sets y to zero. The workspace, where the query
+ * names one, holds the parts of a sum that is split over workgroups (256-byte aligned; its contents need not be set and
+ * mean nothing after the call).
  */
+int64_t plm_gemm_int8_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int plm_gemm_int8(const int8_t* codes, const float* x_scale, const int8_t* weight, const float* scale, int64_t m, int64_t n,
-                  int64_t k, void* y, plm_dtype y_dtype, void* stream);
+                  int64_t k, void* y, plm_dtype y_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* W8A8: the same with 16-bit x [M, K], quantized on the way by the rule of plm_quantize_rows_int8. y has x's
- * type. The workspace is 256-byte aligned; its contents need not be set and mean nothing after the call. */
+ * type. The workspace holds the tokens' codes and scales, too. */
 int64_t plm_gemm_int8_w8a8_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int plm_gemm_int8_w8a8(const void* x, plm_dtype x_dtype, const int8_t* weight, const float* scale, int64_t m, int64_t n,
                        int64_t k, void* y, void* workspace, size_t workspace_bytes, void* stream);

@@ -60,7 +60,8 @@ SIGNATURES = {
     "plm_mlp_mxfp4_w4a4": (_INT, [_P, _INT, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
     "plm_quantize_rows_int8": (_INT, [_P, _INT, _I64, _I64, _P, _P, _P]),
     "plm_dequantize_rows_int8": (_INT, [_P, _P, _I64, _I64, _P, _INT, _P]),
-    "plm_gemm_int8": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _INT, _P]),
+    "plm_gemm_int8_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "plm_gemm_int8": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _INT, _P, _SZ, _P]),
     "plm_gemm_int8_w8a8_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "plm_gemm_int8_w8a8": (_INT, [_P, _INT, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
     "plm_grouped_gemm_int8_workspace_bytes": (_I64, [_I64, _I64, _I64]),
@@ -125,6 +126,7 @@ def reload_tuning() -> None:
     fn()
     gemm_workspace_bytes.cache_clear()  # the plans follow the knobs
     gemm_w8a8_workspace_bytes.cache_clear()
+    mxfp4_bytes.cache_clear()
 
 
 def check(rc: int) -> None:

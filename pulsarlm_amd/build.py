@@ -25,7 +25,7 @@ LIB = PKG / "libpulsarlm_amd.so"
 SOURCES = ["repack.hip", "gemm_decode.hip", "gemm_mfma.hip", "gemm_mfma_int4.hip", "gemm_mfma_fp8.hip", "gemm_mfma_a8.hip",
            "gemm_mfma_grouped.hip", "gemm_rows_int4.hip", "gemm_rows_fp8.hip", "quant.hip", "moe.hip", "routing.hip", "gemm_plain.hip", "capi.hip",
            "mxfp4_quant.hip", "mxfp4_rows.hip", "mxfp4_tiles_w4a16.hip", "mxfp4_tiles_w4a4.hip", "mxfp4_grad.hip", "mxfp4_api.hip",
-           "int8_quant.hip", "dense_rows.hip", "dense_tiles_int8.hip", "dense_tiles_16.hip", "dense_tiles_grad_x.hip", "dense_tiles_grad_w.hip", "dense_api.hip"]
+           "int8_quant.hip", "dense_rows.hip", "dense_tiles_int8.hip", "dense_tiles_16.hip", "dense_tiles_grad_x.hip", "dense_tiles_grad_w.hip", "dense_plan.hip", "dense_api.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

@@ -21,6 +21,8 @@ int check_sizes(const char* op, const char* m, int64_t rows, int64_t n, int64_t 
     PLM_CHECK_ARG(takes_rows(rows, n, k), op, "%s must be below 2^24, %s N and %s K at most 2^36", m, m, m);
     return PLM_OK;
 }
+// What a workspace query counts: sizes that a call takes, and works on.
+bool counts(int64_t m, int64_t n, int64_t k) { return m > 0 && n > 0 && k > 0 && k <= kInt8MaxK && n <= kDenseMaxSize && takes_rows(m, n, k); }
 int check_int8(const char* op, int64_t k) {
     PLM_CHECK_ARG(k % 16 == 0, op, "K must be a multiple of 16");
     PLM_CHECK_ARG(k <= kInt8MaxK, op, "K must be at most 131056");
@@ -52,13 +54,25 @@ dense_product product(dense_type type, const void* p, const void* q, void* y, bo
     d.experts = 1;
     return d;
 }
-void run_int8(const dense_product& p, dense_mode mode, hipStream_t s) {
-    if (!launch_dense_rows(p, mode, s)) launch_tiles_int8(p, mode, s);
+// The dense 8-bit product, and the workspace of a split sum's parts.
+int64_t partial_bytes(int64_t m, int64_t n, int64_t k) {
+    const dense_product p = product(kInt8, nullptr, nullptr, nullptr, true, m, n, k);
+    return dense_partial_bytes(plan_dense(p, kDense, true, true), m, n);
 }
+void run_int8(dense_product p, void* partial, hipStream_t s) {
+    p.plan = plan_dense(p, kDense, true, true);
+    if (p.plan.rows_block > 0) return launch_dense_rows(p, kDense, s);
+    p.partial = static_cast<i32x4_t*>(partial);
+    launch_tiles_int8(p, kDense, s);
+    if (p.plan.splits > 1) launch_combine_int8(p, s);
+}
+
 // 16-bit experts, forward.
 int run_experts(const char* op, dense_product p, const int32_t* offsets, int64_t experts, int zero_rest, hipStream_t s) {
     p.offsets = offsets, p.experts = experts, p.zero_rest = zero_rest != 0;
-    if (!launch_dense_rows(p, kByRows, s)) launch_tiles_16(p, s);
+    p.plan = plan_dense(p, kByRows, true, false);
+    if (p.plan.rows_block > 0) launch_dense_rows(p, kByRows, s);
+    else launch_tiles_16(p, s);
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;
 }
@@ -111,8 +125,10 @@ int plm_dequantize_rows_int8(const int8_t* codes, const float* x_scale, int64_t 
     return PLM_OK;
 }
 
+int64_t plm_gemm_int8_workspace_bytes(int64_t m, int64_t n, int64_t k) { return counts(m, n, k) ? partial_bytes(m, n, k) : 0; }
+
 int plm_gemm_int8(const int8_t* codes, const float* x_scale, const int8_t* weight, const float* scale, int64_t m, int64_t n, int64_t k,
-                  void* y, plm_dtype y_dtype, void* stream) {
+                  void* y, plm_dtype y_dtype, void* workspace, size_t workspace_bytes, void* stream) {
     const char* op = "gemm_int8";
     clear_error();
     PLM_CHECK_ARG(sixteen(y_dtype), op, "y must be fp16 or bf16");
@@ -126,15 +142,16 @@ int plm_gemm_int8(const int8_t* codes, const float* x_scale, const int8_t* weigh
     if (int rc = check_pointer(op, "weight", weight, 16)) return rc;
     if (int rc = check_pointer(op, "x_scale", x_scale, 4)) return rc;
     if (int rc = check_pointer(op, "scale", scale, 4)) return rc;
+    if (int rc = check_workspace(op, workspace, workspace_bytes, partial_bytes(m, n, k))) return rc;
     dense_product p = product(kInt8, codes, weight, y, y_dtype == PLM_BF16, m, n, k);
     p.p_scale = x_scale, p.q_scale = scale;
-    run_int8(p, kDense, s);
+    run_int8(p, workspace, s);
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;
 }
 
 int64_t plm_gemm_int8_w8a8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return m > 0 && n > 0 && k > 0 && k <= kInt8MaxK && n <= kDenseMaxSize && takes_rows(m, n, k) ? tokens_bytes(m, k) : 0;
+    return counts(m, n, k) ? tokens_bytes(m, k) + partial_bytes(m, n, k) : 0;
 }
 
 int plm_gemm_int8_w8a8(const void* x, plm_dtype x_dtype, const int8_t* weight, const float* scale, int64_t m, int64_t n, int64_t k, void* y,
@@ -151,18 +168,18 @@ int plm_gemm_int8_w8a8(const void* x, plm_dtype x_dtype, const int8_t* weight, c
     if (int rc = check_pointer(op, "x", x, 2)) return rc;
     if (int rc = check_pointer(op, "weight", weight, 16)) return rc;
     if (int rc = check_pointer(op, "scale", scale, 4)) return rc;
-    if (int rc = check_workspace(op, workspace, workspace_bytes, tokens_bytes(m, k))) return rc;
+    if (int rc = check_workspace(op, workspace, workspace_bytes, tokens_bytes(m, k) + partial_bytes(m, n, k))) return rc;
     auto* codes = static_cast<int8_t*>(workspace);
     auto* x_scale = reinterpret_cast<float*>(codes + codes_bytes(m, k));
     launch_quantize_int8(x, x_dtype, m, k, codes, x_scale, s);
     dense_product p = product(kInt8, codes, weight, y, x_dtype == PLM_BF16, m, n, k);
     p.p_scale = x_scale, p.q_scale = scale;
-    run_int8(p, kDense, s);
+    run_int8(p, codes + tokens_bytes(m, k), s);
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;
 }
 
-int64_t plm_grouped_gemm_int8_workspace_bytes(int64_t rows, int64_t n, int64_t k) { return plm_gemm_int8_w8a8_workspace_bytes(rows, n, k); }
+int64_t plm_grouped_gemm_int8_workspace_bytes(int64_t rows, int64_t n, int64_t k) { return counts(rows, n, k) ? tokens_bytes(rows, k) : 0; }
 
 int plm_grouped_gemm_int8(const void* x, plm_dtype x_dtype, const int8_t* weight, const float* scale, const int32_t* offsets,
                           int64_t n_experts, int64_t rows, int64_t n, int64_t k, void* y, int zero_rest, void* workspace,
@@ -188,7 +205,9 @@ int plm_grouped_gemm_int8(const void* x, plm_dtype x_dtype, const int8_t* weight
     dense_product p = product(kInt8, codes, weight, y, x_dtype == PLM_BF16, rows, n, k);
     p.p_scale = x_scale, p.q_scale = scale;
     p.offsets = offsets, p.experts = n_experts, p.zero_rest = zero_rest != 0;
-    run_int8(p, kByRows, s);
+    p.plan = plan_dense(p, kByRows, true, false);
+    if (p.plan.rows_block > 0) launch_dense_rows(p, kByRows, s);
+    else launch_tiles_int8(p, kByRows, s);
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;
 }
@@ -225,6 +244,7 @@ int plm_grouped_gemm_grad_x(const void* dy, plm_dtype dtype, const void* weight,
     if (int rc = check_offsets(op, offsets)) return rc;
     dense_product p = product(dtype == PLM_BF16 ? kBf16 : kFp16, dy, weight, dx, dtype == PLM_BF16, rows, k, n);
     p.offsets = offsets, p.experts = n_experts, p.zero_rest = zero_rest != 0;
+    p.plan = plan_dense(p, kByRows, false, false);
     launch_tiles_grad_x(p, as_stream(stream));
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;
@@ -245,6 +265,7 @@ int plm_grouped_gemm_grad_w(const void* dy, const void* x, plm_dtype dtype, cons
     if (int rc = check_offsets(op, offsets)) return rc;
     dense_product p = product(dtype == PLM_BF16 ? kBf16 : kFp16, dy, x, dw, dtype == PLM_BF16, n, k, rows);
     p.offsets = offsets, p.experts = n_experts;
+    p.plan = plan_dense(p, kByRanges, false, false);
     launch_tiles_grad_w(p, as_stream(stream));
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;

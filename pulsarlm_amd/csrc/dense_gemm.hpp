@@ -28,6 +28,8 @@ constexpr int64_t kDenseMaxRows = (int64_t{1} << 24) - 1;
 constexpr int64_t kInt8MaxK = 131056;  // 128 * 128 * K fits 31 bits
 constexpr int64_t kMaxExperts = 4096;
 
+typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+
 struct dense_args {
     const uint8_t *p, *q;  // rows pitch_p and pitch_q bytes apart
     uint16_t* y;           // [rows][cols], an expert's product `rows * cols` after the one before (kByRanges)
@@ -41,6 +43,8 @@ struct dense_args {
     bool zero_rest;             // kByRows: rows past the last expert's are set to zero, else not written
     bool lines, wide;           // stores of 16 bytes (cols % 8 == 0, y 16-byte aligned), of 8
     bool bf16;                  // the output's type
+    i32x4_t* partial;           // dense 8-bit: sums of split_stages stages each, [splits][rows][quads of columns], or null
+    int split_stages, quads;
 };
 
 // The rows of the experts: offsets are their inclusive ends, each taken within [0, rows] and no less than the ones before
@@ -121,7 +125,6 @@ __device__ __forceinline__ expert_range find_block(const int32_t* offsets, int n
 
 // Sums, int32 or fp32, of the matrix instruction on 16 x 16 rows and columns and 64 bytes of K: a lane's operand is 16
 // bytes, row lane % 16, K bytes 16 (lane / 16) on; its sums are P's row lane % 16 and Q's rows 4 (lane / 16) + 0..3.
-typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 template <dense_type T> using dense_acc = std::conditional_t<T == kInt8, i32x4_t, f32x4_t>;
 
 template <dense_type T> __device__ __forceinline__ dense_acc<T> dense_mfma(u32x4_t q, u32x4_t p, dense_acc<T> c) {
@@ -158,6 +161,11 @@ template <bool BF16> __device__ __forceinline__ void dense_store4(uint16_t* row,
         if (col + i < cols) row[col + i] = static_cast<uint16_t>(to_bits16<BF16>(f[i]));
 }
 
+// Which kernel takes a call: for few rows, in blocks of rows_block, or where that is 0 a tile shape, with the sum split
+// into parts.
+struct dense_plan {
+    int shape = 0, splits = 1, rows_block = 0;
+};
 // One call's product. type: the operands'.
 struct dense_product {
     const void *p, *q;
@@ -168,6 +176,8 @@ struct dense_product {
     int64_t experts;
     dense_type type;
     bool bf16, zero_rest;
+    dense_plan plan;
+    i32x4_t* partial;
 };
 
 // Row blocks of `rows` that a call can have: by rows, each expert's last one can be a part.
@@ -198,15 +208,24 @@ inline dense_args make_dense_args(const dense_product& p, bool p_across, bool q_
     a.bf16 = p.bf16;
     a.lines = p.cols % 8 == 0 && aligned(p.y, 16);
     a.wide = p.cols % 4 == 0 && aligned(p.y, 8);
+    a.quads = static_cast<int>(ceil_div(p.cols, 4));
     return a;
 }
 
+dense_plan plan_dense(const dense_product& p, dense_mode mode, bool rows_kernel, bool may_split);
+// Strips of 16 columns of a workgroup of the kernel for few rows: two where that leaves work for every CU.
+inline int64_t dense_rows_strips(int64_t blocks, int64_t cols) { return ceil_div(cols, 16) * blocks > cu_count() ? 2 : 1; }
+// Workspace of a plan's parts.
+inline int64_t dense_partial_bytes(const dense_plan& plan, int64_t rows, int64_t cols) {
+    return plan.splits > 1 ? plan.splits * rows * ceil_div(cols, 4) * 16 : 0;
+}
 void launch_tiles_int8(const dense_product& p, dense_mode mode, hipStream_t s);
 void launch_tiles_16(const dense_product& p, hipStream_t s);         // forward, by rows
 void launch_tiles_grad_x(const dense_product& p, hipStream_t s);
 void launch_tiles_grad_w(const dense_product& p, hipStream_t s);
-// The kernel for few rows, forward: true where it has launched.
-bool launch_dense_rows(const dense_product& p, dense_mode mode, hipStream_t s);
+void launch_combine_int8(const dense_product& p, hipStream_t s);
+// The kernel for few rows, forward.
+void launch_dense_rows(const dense_product& p, dense_mode mode, hipStream_t s);
 
 // Rows of codes and their scales.
 void launch_quantize_int8(const void* x, plm_dtype dtype, int64_t m, int64_t k, int8_t* codes, float* scale, hipStream_t s);

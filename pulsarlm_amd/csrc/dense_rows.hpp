@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(NW * 64) dense_rows_kernel(dense_args a) {
         for (int u = 0; u < U; ++u) {
             const int past = u * 64 + kq * 16 < left ? u * 64 : kOOB;
 #pragma unroll
-            for (int j = 0; j < NS; ++j) c.q[j][u] = buffer_load16_stream(qr, q_at + past, from + j * 16 * a.pitch_q);
+            for (int j = 0; j < NS; ++j) c.q[j][u] = buffer_load16(qr, q_at + past, from + j * 16 * a.pitch_q);
 #pragma unroll
             for (int i = 0; i < MT; ++i) c.p[i][u] = buffer_load16(pr, p_at + past, from + i * 16 * a.pitch_p);
         }

@@ -11,7 +11,6 @@
 #pragma once
 
 #include <algorithm>
-#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -58,11 +57,12 @@ template <bool CROSS, int BLOCK, int NW> struct dense_operand {
 // Across: piece (32 bytes) c of the sum's row k lies at piece c ^ f(k), so that the rows and pieces that 32 lanes of a
 // transposing read touch fall on different banks.
 __device__ __forceinline__ constexpr int cross_swizzle(int k, int pieces) {
-    return pieces >= 8 ? (k & 3) << 1 | (((k >> 2) ^ (k >> 3)) & 1) : (k & 2) | ((k >> 3) & 1);
+    return pieces >= 8 ? (k & 3) << 1 | (((k >> 2) ^ (k >> 3)) & 1) : pieces == 4 ? (k & 2) | ((k >> 3) & 1) : (k >> 3) & 1;
 }
 
-template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX>
-__global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) {
+// KG: groups of WM x WN wavefronts that take the stages in turn, each with rings of its own; their sums meet in LDS.
+template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX, int KG>
+__global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_args a) {
     constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
     using P = dense_operand<PC, BM, NW>;
     using Q = dense_operand<QC, BN, NW>;
@@ -70,11 +70,14 @@ __global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) 
     constexpr int P_RING = (S + PX) * P::kBytes, LDS = P_RING + S * Q::kBytes;
     constexpr int SIZE = T == kInt8 ? 1 : 2;
     constexpr int DEPTH = 128 / SIZE;  // of the sum, a stage
+    constexpr bool SPLITS = T == kInt8 && MODE == kDense && KG == 1;
     static_assert(T != kInt8 || (!PC && !QC), "8-bit operands lie along the sum");
-    static_assert(LDS <= 160 * 1024, "LDS");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
+    static_assert(KG * LDS <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t all_lds[KG * LDS];
 
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int group = KG == 1 ? 0 : uniform(threadIdx.x >> 6) / NW, wave = uniform(threadIdx.x >> 6) % NW;
+    uint8_t* lds = all_lds + group * LDS;
     const int wm = wave / WN, wn = wave % WN, col16 = lane & 15, kq = lane >> 4;
 
     // The workgroup's tile. Workgroups go round the 8 XCDs by id: each takes one run of the tiles, which are ordered in
@@ -104,7 +107,10 @@ __global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) 
         first = r.lo, depth = r.hi - r.lo;
     }
     const int col0 = nb * BN;
-    const int stages = (depth + DEPTH - 1) / DEPTH;
+    // The workgroup's part of the sum: from stage `skipped` on, `depth` to its end.
+    int skipped = 0;
+    if constexpr (SPLITS) skipped = static_cast<int>(blockIdx.y) * a.split_stages, depth = min(depth, (skipped + a.split_stages) * DEPTH);
+    const int stages = (depth + DEPTH - 1) / DEPTH - skipped;
 
     // Operands. Along: the tile's rows from the first on, the range check ends past the last. Across: the sum's rows
     // from the first on; a stage's base moves with it, as all of them can pass 2 GiB.
@@ -148,16 +154,18 @@ __global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) 
         const int left = min(depth - kt * DEPTH, DEPTH);
         return source{buffer_words(base + static_cast<int64_t>(kt) * DEPTH * pitch, left > 0 ? static_cast<uint32_t>(left) * pitch - column * 2 : 0u), {v[0], v[1]}};
     };
-    auto source_p = [&](int kt) {
+    auto source_p = [&](int turn) {
+        const int kt = skipped + turn * KG + group;
         if constexpr (PC) return cross(kt, p_base, a.pitch_p, row0, p_cross);
         else return along(kt, p_base, rows, a.pitch_p);
     };
-    auto source_q = [&](int kt) {
+    auto source_q = [&](int turn) {
+        const int kt = skipped + turn * KG + group;
         if constexpr (QC) return cross(kt, q_base, a.pitch_q, col0, q_cross);
         else return along(kt, q_base, q_rows, a.pitch_q);
     };
     // Load l of the wavefront's.
-    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds)) + wave * 1024;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)all_lds)) + group * LDS + wave * 1024;
     auto issue_p = [&](const source& s, auto l, int slot) {
         constexpr int n = decltype(l)::value;
         dma16(s.buffer, lds0 + slot * P::kBytes, n * NW * 1024, s.v[n & 1], (n * NW + wave) * P::kRowsLoad * a.pitch_p);
@@ -218,17 +226,17 @@ __global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) 
 #pragma unroll
     for (int f = 0; f < NT; ++f) q[0][f] = read_q(f, 0, 0);
     int ps = 0, qs = 0, p_to = S;  // the stage's slots, and with PX where P's next loads go
-    // One slice of stage kt. Among its matrix instructions, one behind each, stand the reads of the next slice's
+    // One slice of a turn's stage. Among its matrix instructions, one behind each, stand the reads of the next slice's
     // fragments, over the first three quarters, so that they are there when it begins, and the loads: a wavefront issues
     // in order, and two such in a row would take longer than a matrix instruction and leave its unit idle.
     constexpr int STEPS = MT * NT, READS = MT + NT, EARLY = STEPS * 3 / 4;
-    auto slice = [&](auto second, int kt) {
+    auto slice = [&](auto second, int turn) {
         constexpr int t = decltype(second)::value;
         constexpr int PL = PX != t ? P::kLoads : 0, QL = t ? Q::kLoads : 0, LOADS = PL + QL;
         const int pn = t ? (ps + 1 == S + PX ? 0 : ps + 1) : ps, qn = t ? (qs + 1 == S ? 0 : qs + 1) : qs;
         source from_p, from_q;
-        if constexpr (PL > 0) from_p = source_p(kt + S);
-        if constexpr (QL > 0) from_q = source_q(kt + S);
+        if constexpr (PL > 0) from_p = source_p(turn + S);
+        if constexpr (QL > 0) from_q = source_q(turn + S);
         if constexpr (t) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
         unrolled<STEPS>([&](auto step) {
             constexpr int s = decltype(step)::value, i = s / NT, j = s % NT;
@@ -254,20 +262,59 @@ __global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) 
             ps = pn, qs = qn;
         }
     };
-    for (int kt = 0; kt < stages; ++kt) {
-        slice(std::integral_constant<int, 0>{}, kt);
-        slice(std::integral_constant<int, 1>{}, kt);
+    const int turns = (stages + KG - 1) / KG;  // past the last stage of zeros
+    for (int turn = 0; turn < turns; ++turn) {
+        slice(std::integral_constant<int, 0>{}, turn);
+        slice(std::integral_constant<int, 1>{}, turn);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // requests past the end; LDS is free
+
+    if constexpr (KG > 1) {
+        // In group order, so that the result does not depend on which is done first.
+        static_assert((KG - 1) * NW * MT * NT * 1024 <= KG * LDS, "the sums fit");
+        acc_t* sums = reinterpret_cast<acc_t*>(all_lds);
+        if (group > 0)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) sums[(((group - 1) * NW + wave) * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
+        __syncthreads();
+        if (group == 0)
+#pragma unroll
+            for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = acc[i][j] + sums[((g * NW + wave) * MT * NT + i * NT + j) * 64 + lane];
+        __syncthreads();
+        if (group > 0) return;
+    }
+
+    if constexpr (SPLITS) {
+        if (a.partial != nullptr) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int r = (wm * MT + i) * 16 + col16;
+                i32x4_t* to = a.partial + ((static_cast<int64_t>(blockIdx.y) * a.rows + row0 + r) * a.quads + (col0 >> 2));
+                if (r < rows)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const int quad = (wn * NT + j) * 4 + kq;
+                        if ((col0 >> 2) + quad < a.quads) to[quad] = acc[i][j];
+                    }
+            }
+            return;
+        }
+    }
 
     // A lane has four columns of one row, a quarter of a 32-byte piece. RB row blocks at a time go through the
     // wavefront's own part of LDS (pitch padded by 16 bytes) and leave as 16 bytes a lane, whole rows of its tile.
     auto finish = [&](auto bf16) {
         constexpr bool BF16 = decltype(bf16)::value;
         constexpr int COLS = NT * 16, PITCH = COLS * 2 + 16, CH = COLS / 8;
-        constexpr int FIT = LDS / (NW * 16 * PITCH), RB = FIT >= MT ? MT : (FIT >= 4 ? 4 : (FIT >= 2 ? 2 : 1));
+        constexpr int FIT = KG * LDS / (NW * 16 * PITCH), RB = FIT >= MT ? MT : (FIT >= 4 ? 4 : (FIT >= 2 ? 2 : 1));
         static_assert(FIT >= 1 && MT % RB == 0, "the rows fit");
-        uint8_t* mine = lds + wave * RB * 16 * PITCH;
+        uint8_t* mine = all_lds + wave * RB * 16 * PITCH;
         const int c0 = col0 + wn * COLS;
         uint16_t* y = a.y + (MODE == kByRanges ? expert * static_cast<int64_t>(a.rows) * a.cols : 0);
         f32x4_t channel[NT];
@@ -322,7 +369,7 @@ __global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) 
     else finish(std::false_type{});
 }
 
-template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX>
+template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX, int KG = 1>
 void launch_tile(const dense_product& p, hipStream_t s) {
     constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
     dense_args a = make_dense_args(p, PC, QC);
@@ -330,50 +377,24 @@ void launch_tile(const dense_product& p, hipStream_t s) {
     a.n_blocks = static_cast<int>(ceil_div(p.cols, BN));
     a.m_blocks = static_cast<int>(dense_row_blocks(p, MODE, BM));
     const int64_t tiles = int64_t{1} * a.m_blocks * a.n_blocks * (MODE == kByRanges ? p.experts : 1);
-    dense_tile_kernel<T, MODE, PC, QC, WM, WN, MT, NT, S, PX><<<static_cast<unsigned>(tiles), WM * WN * 64, 0, s>>>(a);
-}
-
-// The tile shapes, and which of them takes a call: the least of rounds x stages x time of a stage. The times (us) were
-// measured with one workgroup on the GPU and with every slot taken; between the two they grow with the share of slots
-// taken, as the workgroups share the L2s and the clock.
-// {rows, columns, threads, workgroups a CU, lone, full}
-struct dense_cost {
-    int rows, cols, threads, per_cu;
-    double lone, full;
-};
-constexpr dense_cost kDenseTiles[] = {
-    {256, 256, 512, 1, 1.0, 1.6}, {128, 256, 512, 1, 0.6, 0.9}, {128, 128, 256, 2, 0.45, 0.9}, {64, 128, 256, 2, 0.3, 0.5}, {64, 64, 256, 2, 0.25, 0.35}};
-
-// By rows, how many blocks there are is known on the device only: with parts of unknown sizes, half a block of each
-// expert is taken to be empty.
-inline int choose_dense_tile(const dense_product& p, dense_mode mode) {
-    const int64_t depth = mode == kByRanges ? ceil_div(p.depth, p.experts) : p.depth;
-    const int64_t stages = std::max<int64_t>(1, ceil_div(depth * (p.type == kInt8 ? 1 : 2), 128));
-    int best = 0;
-    double least = 1e300;
-    const int forced = knobs().dense_tile;
-    for (int i = 0; i < 5; ++i) {
-        const dense_cost& c = kDenseTiles[i];
-        const int64_t cols = ceil_div(p.cols, c.cols), experts = mode == kByRanges ? p.experts : 1;
-        if (forced >= 0 && i != forced && i > 0) continue;
-        if (i > 0 && !dense_grid_fits(dense_row_blocks(p, mode, c.rows) * cols * experts, c.threads)) continue;
-        const double blocks = mode == kByRows ? static_cast<double>(p.rows) / c.rows + 0.5 * std::min(p.rows, p.experts)
-                                              : static_cast<double>(ceil_div(p.rows, c.rows) * experts);
-        const double tiles = blocks * cols, slots = static_cast<double>(c.per_cu) * cu_count();
-        const double fill = std::min(1.0, tiles / slots);
-        const double rounds = mode == kDense ? std::ceil(tiles / slots) : std::max(1.0, tiles / slots);
-        const double t = rounds * (stages + 4) * (c.lone + (c.full - c.lone) * fill);
-        if (t < least || i == forced) least = t, best = i;
+    dim3 grid(static_cast<unsigned>(tiles));
+    if (T == kInt8 && MODE == kDense && p.plan.splits > 1) {
+        grid.y = static_cast<unsigned>(p.plan.splits);
+        a.split_stages = static_cast<int>(ceil_div(ceil_div(p.depth, 128), p.plan.splits));
+        a.partial = p.partial;
+    } else {
+        a.split_stages = 1 << 20;
     }
-    return best;
+    dense_tile_kernel<T, MODE, PC, QC, WM, WN, MT, NT, S, PX, KG><<<grid, WM * WN * 64 * KG, 0, s>>>(a);
 }
 
 template <dense_type T, dense_mode MODE, bool PC, bool QC> void launch_shape(const dense_product& p, hipStream_t s) {
-    switch (choose_dense_tile(p, MODE)) {
+    switch (p.plan.shape) {
         case 0: return launch_tile<T, MODE, PC, QC, 2, 4, 8, 4, 2, 1>(p, s);
         case 1: return launch_tile<T, MODE, PC, QC, 2, 4, 4, 4, 3, 0>(p, s);
-        case 2: return launch_tile<T, MODE, PC, QC, 2, 2, 4, 4, 2, 0>(p, s);
-        case 3: return launch_tile<T, MODE, PC, QC, 2, 2, 2, 4, 3, 0>(p, s);
+        case 2: return launch_tile<T, MODE, PC, QC, 2, 2, 4, 4, 5, 0>(p, s);
+        case 3: return launch_tile<T, MODE, PC, QC, 2, 2, 4, 4, 2, 0>(p, s);
+        case 4: return launch_tile<T, MODE, PC, QC, 2, 2, 2, 4, 3, 0>(p, s);
         default: return launch_tile<T, MODE, PC, QC, 2, 2, 2, 2, 4, 0>(p, s);
     }
 }

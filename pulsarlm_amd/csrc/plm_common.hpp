@@ -462,7 +462,8 @@ struct tuning {
     bool moe_small_sort_off = false;   // PLM_MOE_SMALL_SORT=0
     bool moe_unfused = false;          // PLM_MOE_UNFUSED
     bool moe_persist = false;          // PLM_MOE_PERSIST=1: persistent grouped launches
-    int dense_tile = -1;               // PLM_DENSE=t<index>: one tile shape of the products on unpacked weights
+    int dense_tile = -1;               // PLM_DENSE=t<index>[,splits]: one tile shape of the products on unpacked weights
+    int dense_splits = 1;
     int dense_rows = -1;               // PLM_DENSE=r<rows>: their kernel for few rows, 16, 32 or 64 a block; r0: not at all
     unsigned epoch = 0;                // one more with each re-parse
 };

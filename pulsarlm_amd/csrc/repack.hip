@@ -83,9 +83,10 @@ tuning parse_tuning() {
     t.moe_unfused = env("PLM_MOE_UNFUSED") != nullptr;
     if (const char* e = env("PLM_MOE_PERSIST")) t.moe_persist = e[0] == '1';
     if (const char* e = env("PLM_DENSE")) {
-        const int v = e[0] != 0 ? atoi(e + 1) : -1;
-        if (e[0] == 't' && v >= 0 && v < 5) t.dense_tile = v, t.dense_rows = 0;
-        if (e[0] == 'r' && (v == 0 || v == 16 || v == 32 || v == 64)) t.dense_rows = v;
+        int v = -1, splits = 1;
+        const int got = e[0] != 0 ? sscanf(e + 1, "%d,%d", &v, &splits) : 0;
+        if (got >= 1 && e[0] == 't' && v >= 0 && v < 6) t.dense_tile = v, t.dense_rows = 0, t.dense_splits = std::max(1, splits);
+        if (got >= 1 && e[0] == 'r' && (v == 0 || v == 16 || v == 32 || v == 64)) t.dense_rows = v;
     }
     return t;
 }

@@ -721,8 +721,10 @@ def gemm_int8_cuda(codes: torch.Tensor, x_scale: torch.Tensor, weight: torch.Ten
     _require(weight.shape[1] == k and weight.get_device() == codes.get_device(), op, "weight must be [N, K] for codes [M, K], on their device")
     _require(dtype in _HALF, op, "dtype must be fp16 or bf16")
     y = _int8_out(op, codes, dtype, (m, n), out)
+    ws = _mx_scratch(op, codes, m, n, k)
     with _on(codes.device):
-        _call("plm_gemm_int8", _ptr(codes), _ptr(x_scale), _ptr(weight), _ptr(scale), m, n, k, _ptr(y), _DTYPES[dtype], _stream(codes.device))
+        _call("plm_gemm_int8", _ptr(codes), _ptr(x_scale), _ptr(weight), _ptr(scale), m, n, k, _ptr(y), _DTYPES[dtype], _ptr(ws),
+              0 if ws is None else ws.numel(), _stream(codes.device))
     return y
 
 

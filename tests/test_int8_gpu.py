@@ -11,7 +11,7 @@ from tests import _dense as dense
 pytestmark = pytest.mark.gpu
 
 # The kernels that a call can run on: by the rule, each block of the kernel for few rows, each tile shape.
-KERNELS = [None, "r16", "r32", "r64", "t0", "t1", "t2", "t3", "t4"]
+KERNELS = [None, "r16", "r32", "r64", *(f"t{i}" for i in range(6)), "t0,3", "t2,2", "t3,5", "t4,16", "t5,4"]
 
 
 def check_quantizer(x):
