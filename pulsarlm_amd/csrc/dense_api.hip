@@ -169,11 +169,18 @@ int plm_gemm_int8_w8a8(const void* x, plm_dtype x_dtype, const int8_t* weight, c
     if (int rc = check_pointer(op, "weight", weight, 16)) return rc;
     if (int rc = check_pointer(op, "scale", scale, 4)) return rc;
     if (int rc = check_workspace(op, workspace, workspace_bytes, tokens_bytes(m, k) + partial_bytes(m, n, k))) return rc;
+    dense_product p = product(kInt8, x, weight, y, x_dtype == PLM_BF16, m, n, k);
+    p.q_scale = scale;
+    p.plan = plan_dense(p, kDense, true, true);
+    if (dense_rows_quantizes(p)) {
+        launch_dense_rows_quantize(p, s);
+        PLM_HIP_LAUNCH_CHECK(op);
+        return PLM_OK;
+    }
     auto* codes = static_cast<int8_t*>(workspace);
     auto* x_scale = reinterpret_cast<float*>(codes + codes_bytes(m, k));
     launch_quantize_int8(x, x_dtype, m, k, codes, x_scale, s);
-    dense_product p = product(kInt8, codes, weight, y, x_dtype == PLM_BF16, m, n, k);
-    p.p_scale = x_scale, p.q_scale = scale;
+    p.p = codes, p.p_scale = x_scale;
     run_int8(p, codes + tokens_bytes(m, k), s);
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;

@@ -226,6 +226,9 @@ void launch_tiles_grad_w(const dense_product& p, hipStream_t s);
 void launch_combine_int8(const dense_product& p, hipStream_t s);
 // The kernel for few rows, forward.
 void launch_dense_rows(const dense_product& p, dense_mode mode, hipStream_t s);
+// The same on 16-bit x [rows][depth] (p.p), quantized in the kernel, for dense 8-bit products that it takes.
+bool dense_rows_quantizes(const dense_product& p);
+void launch_dense_rows_quantize(const dense_product& p, hipStream_t s);
 
 // Rows of codes and their scales.
 void launch_quantize_int8(const void* x, plm_dtype dtype, int64_t m, int64_t k, int8_t* codes, float* scale, hipStream_t s);

@@ -35,11 +35,9 @@ constexpr double kStart = 3.3, kRowsRate = 33e3, kMemoryRate = 5.2e6;
 // A split sum's parts: a kernel more, and their way through memory and back.
 constexpr double kCombine = 3.5, kPartRate = 4.5e6;
 
-}  // namespace
-
 // By rows, how the rows fall on the experts is known on the device only. Taken: 1 - e^-a of them have any, with a rows
 // an expert on average, and those have half a block more than whole ones, one at least.
-dense_plan plan_dense(const dense_product& p, dense_mode mode, bool rows_kernel, bool may_split) {
+dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, bool may_split) {
     const int64_t size = p.type == kInt8 ? 1 : 2, cus = cu_count();
     const int64_t depth = mode == kByRanges ? ceil_div(p.depth, p.experts) : p.depth;
     const int64_t stages = std::max<int64_t>(1, ceil_div(depth * size, 128));
@@ -88,6 +86,14 @@ dense_plan plan_dense(const dense_product& p, dense_mode mode, bool rows_kernel,
         if (time < least) least = time, best = {0, 1, block};
     }
     return best;
+}
+
+}  // namespace
+
+dense_plan plan_dense(const dense_product& p, dense_mode mode, bool rows_kernel, bool may_split) {
+    static thread_local plan_cache<dense_plan> cache;
+    const int kind = mode * 8 + (p.type == kInt8 ? 4 : 0) + (rows_kernel ? 2 : 0) + (may_split ? 1 : 0);
+    return cache.get(kind, p.rows, p.cols, p.depth, p.experts, [&] { return make_plan(p, mode, rows_kernel, may_split); });
 }
 
 namespace {

@@ -4,23 +4,32 @@
 //
 // * A workgroup owns 16 MT rows by 16 NS columns. Its NW wavefronts take chunks of 64 U bytes of K in turn, each with the
 //   next chunk's loads in flight, and their sums meet in LDS in wavefront order: results do not depend on timing.
+// * QUANT: a few rows of 16-bit x, quantized by every workgroup for itself while its first weights are on their way: each
+//   reads the rows for their largest magnitudes, and keeps their codes in LDS. A launch less: N 6144, K 4096, one row.
 #pragma once
 
 #include <algorithm>
 
 #include "dense_gemm.hpp"
+#include "int8_rows.hpp"
 
 namespace plm {
 
 namespace {
 
-template <dense_type T, dense_mode MODE, int MT, int NS, int U, int NW>
+constexpr int kQuantRows = 4, kQuantBytes = 64 * 1024;  // QUANT: rows and bytes of their codes at most
+
+template <dense_type T, dense_mode MODE, int MT, int NS, int U, int NW, bool QUANT>
 __global__ void __launch_bounds__(NW * 64) dense_rows_kernel(dense_args a) {
     using acc_t = dense_acc<T>;
     constexpr int SIZE = T == kInt8 ? 1 : 2, CHUNK = 64 * U, BM = 16 * MT;
     constexpr int SHIFT = MT == 1 ? 4 : MT == 2 ? 5 : 6;
     static_assert(1 << SHIFT == BM, "row blocks are powers of two");
+    static_assert(!QUANT || (T == kInt8 && MODE == kDense && MT == 1), "a few rows of the dense product");
     __shared__ acc_t sums[NW][MT * NS][64];
+    extern __shared__ __attribute__((aligned(16))) uint8_t codes[];  // QUANT: [rows][K]
+    __shared__ uint32_t tops[QUANT ? NW : 1];
+    __shared__ float tokens[QUANT ? kQuantRows : 1];
 
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int col16 = lane & 15, kq = lane >> 4;
@@ -52,7 +61,8 @@ __global__ void __launch_bounds__(NW * 64) dense_rows_kernel(dense_args a) {
 #pragma unroll
             for (int j = 0; j < NS; ++j) c.q[j][u] = buffer_load16(qr, q_at + past, from + j * 16 * a.pitch_q);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) c.p[i][u] = buffer_load16(pr, p_at + past, from + i * 16 * a.pitch_p);
+            for (int i = 0; i < MT; ++i)
+                if constexpr (!QUANT) c.p[i][u] = buffer_load16(pr, p_at + past, from + i * 16 * a.pitch_p);
         }
     };
     acc_t acc[MT][NS];
@@ -60,6 +70,14 @@ __global__ void __launch_bounds__(NW * 64) dense_rows_kernel(dense_args a) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NS; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+    // The rows' codes of chunk `at`.
+    auto take_codes = [&](chunk& c, int at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = at * CHUNK + u * 64 + kq * 16;
+            c.p[0][u] = col16 < rows && k < bytes ? *reinterpret_cast<const u32x4_t*>(codes + col16 * bytes + k) : u32x4_t{0, 0, 0, 0};
+        }
+    };
     auto multiply = [&](const chunk& c) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -70,10 +88,52 @@ __global__ void __launch_bounds__(NW * 64) dense_rows_kernel(dense_args a) {
     };
     chunk even, odd;
     load(even, wave);
+    if constexpr (QUANT) {
+        // A row's wavefronts (all of them; half; a quarter) take its pieces of eight values in turn; the first HELD of a
+        // lane wait in registers for the row's largest, what is past them is read again, from the caches.
+        constexpr int HELD = 4;
+        const int row_waves = rows == 1 ? NW : rows == 2 ? NW / 2 : NW / 4;
+        const int r = wave / row_waves, step = row_waves * 64, first = (wave % row_waves) * 64 + lane, pieces = depth / 8;
+        auto piece = [&](int i) { return buffer_load16(pr, i < pieces ? r * a.pitch_p + i * 16 : kOOB); };  // past the rows zeros
+        u32x4_t held[HELD];
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) held[h] = piece(first + h * step);
+        uint32_t top = 0;
+        auto count = [&](const u32x4_t& v) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = top_16(top, v[i]);
+        };
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) count(held[h]);
+        for (int i = first + HELD * step; i < pieces; i += step) count(piece(i));
+        top = a.bf16 ? top_bits<true>(top) : top_bits<false>(top);
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), s)));
+        if (lane == 0) tops[wave] = top;
+        __syncthreads();
+        for (int w = r * row_waves; w < (r + 1) * row_waves; ++w) top = max(top, tops[w]);
+        const int8_scale k = make_int8_scale(top);
+        if (lane == 0 && r < kQuantRows) tokens[r] = k.s;
+        auto put = [&](int i, const u32x4_t& v) {
+            if (r >= rows || i >= pieces) return;
+            uint32_t q[2] = {0, 0};
+            float x[8];
+            if (a.bf16) eight_values<true>(v, x);
+            else eight_values<false>(v, x);
+            if (k.finite) int8_codes<8>(x, k, q);
+            *reinterpret_cast<uint2*>(codes + r * depth + i * 8) = make_uint2(q[0], q[1]);
+        };
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) put(first + h * step, held[h]);
+        for (int i = first + HELD * step; i < pieces; i += step) put(i, piece(i));
+        __syncthreads();
+    }
     for (int c = wave; c < chunks; c += 2 * NW) {
         load(odd, c + NW);
+        if constexpr (QUANT) take_codes(even, c);
         multiply(even);
         load(even, c + 2 * NW);
+        if constexpr (QUANT) take_codes(odd, c + NW);
         multiply(odd);
     }
 #pragma unroll
@@ -91,7 +151,13 @@ __global__ void __launch_bounds__(NW * 64) dense_rows_kernel(dense_args a) {
             for (int w = 1; w < NW; ++w) v = v + sums[w][s][lane];
             if (r >= rows) continue;
             f32x4_t f;
-            if constexpr (T == kInt8) f = dense_scaled(v, dense_channels(a.q_scale + static_cast<int64_t>(expert) * a.cols, col, a.cols), a.p_scale[row0 + r]);
+            float token = 0.f;
+            if constexpr (QUANT) {
+                token = tokens[r];
+            } else if constexpr (T == kInt8) {
+                token = a.p_scale[row0 + r];
+            }
+            if constexpr (T == kInt8) f = dense_scaled(v, dense_channels(a.q_scale + static_cast<int64_t>(expert) * a.cols, col, a.cols), token);
             else f = v;
             if (T == kInt8 && rest) f = f32x4_t{0.f, 0.f, 0.f, 0.f};
             dense_store4<BF16>(a.y + (static_cast<int64_t>(row0) + r) * a.cols, col, a.cols, a.wide, f);
@@ -103,11 +169,13 @@ __global__ void __launch_bounds__(NW * 64) dense_rows_kernel(dense_args a) {
     else finish(std::false_type{});
 }
 
-template <dense_type T, dense_mode MODE, int MT, int NS, int U, int NW> void launch_rows(const dense_product& p, hipStream_t s) {
+template <dense_type T, dense_mode MODE, int MT, int NS, int U, int NW, bool QUANT = false> void launch_rows(const dense_product& p, hipStream_t s) {
     dense_args a = make_dense_args(p, false, false);
     a.n_blocks = static_cast<int>(ceil_div(p.cols, 16 * NS));
     a.m_blocks = static_cast<int>(dense_row_blocks(p, MODE, 16 * MT));
-    dense_rows_kernel<T, MODE, MT, NS, U, NW><<<static_cast<unsigned>(a.n_blocks) * a.m_blocks, NW * 64, 0, s>>>(a);
+    if (QUANT) a.pitch_p = 2 * a.depth;
+    dense_rows_kernel<T, MODE, MT, NS, U, NW, QUANT>
+        <<<static_cast<unsigned>(a.n_blocks) * a.m_blocks, NW * 64, QUANT ? static_cast<unsigned>(p.rows * p.depth) : 0u, s>>>(a);
 }
 
 }  // namespace

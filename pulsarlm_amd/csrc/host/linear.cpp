@@ -1,5 +1,5 @@
 // linear over the pulsarlm_amd ops: the reference's dense/fp8 linear
-// (pulsarlm-core/src/engine/model/linear.cpp:14-41) plus int4 and MXFP4 alternatives.
+// (pulsarlm-core/src/engine/model/linear.cpp:14-41) plus int4, MXFP4 and int8 alternatives.
 // Quantized weights are repacked once, at construction, as the reference does.
 #include "linear.hpp"
 
@@ -10,7 +10,7 @@
 
 namespace pulsarlm {
 
-linear::linear(std::variant<at::Tensor, quant_weight, mxfp4_weight> weight) : weight(std::move(weight)) {}
+linear::linear(std::variant<at::Tensor, quant_weight, mxfp4_weight, int8_weight> weight) : weight(std::move(weight)) {}
 
 linear linear::dense(at::Tensor weight) { return linear(std::move(weight)); }
 
@@ -41,6 +41,12 @@ linear linear::mxfp4(const at::Tensor& codes, const at::Tensor& scale, bool w4a4
     return linear(mxfp4_weight{std::move(w), std::move(s), codes.size(0), w4a4});
 }
 
+linear linear::int8(const at::Tensor& codes, const at::Tensor& scale) {
+    TORCH_CHECK(codes.scalar_type() == at::kChar && codes.dim() == 2 && scale.scalar_type() == at::kFloat && scale.numel() == codes.size(0),
+                "linear: codes must be int8 [N, K] and scale fp32 [N]");
+    return linear(int8_weight{codes.contiguous(), scale.reshape({-1}).contiguous()});
+}
+
 at::Tensor linear::apply(const at::Tensor& x) const {
     if (const auto* dense = std::get_if<at::Tensor>(&weight)) return at::linear(x, *dense);
     std::vector<std::int64_t> sizes = x.sizes().vec();
@@ -49,6 +55,10 @@ at::Tensor linear::apply(const at::Tensor& x) const {
         sizes.back() = mx->n;
         return (mx->w4a4 ? gemm_mxfp4_w4a4_cuda(rows, mx->weight, mx->scale, mx->n) : gemm_mxfp4_cuda(rows, mx->weight, mx->scale, mx->n))
             .view(sizes);
+    }
+    if (const auto* w8 = std::get_if<int8_weight>(&weight)) {
+        sizes.back() = w8->codes.size(0);
+        return gemm_int8_w8a8_cuda(rows, w8->codes, w8->scale).view(sizes);
     }
     const quant_weight& w = std::get<quant_weight>(weight);
     sizes.back() = w.n;

@@ -1,6 +1,6 @@
-// y = x @ W^T over x's last dim for a dense, fp8, int4 or MXFP4 weight: the reference's
+// y = x @ W^T over x's last dim for a dense, fp8, int4, MXFP4 or int8 weight: the reference's
 // linear (pulsarlm-core/inc/pulsarlm/engine/model/linear.hpp:13-35,
-// src/engine/model/linear.cpp:19-41) with int4 and MXFP4 alternatives next to fp8.
+// src/engine/model/linear.cpp:19-41) with int4, MXFP4 and int8 alternatives next to fp8.
 #pragma once
 
 #include <ATen/ATen.h>
@@ -26,9 +26,14 @@ class linear {
         bool w4a4;
     };
 
-    std::variant<at::Tensor, quant_weight, mxfp4_weight> weight;
+    struct int8_weight {
+        at::Tensor codes;
+        at::Tensor scale;
+    };
 
-    explicit linear(std::variant<at::Tensor, quant_weight, mxfp4_weight> weight);
+    std::variant<at::Tensor, quant_weight, mxfp4_weight, int8_weight> weight;
+
+    explicit linear(std::variant<at::Tensor, quant_weight, mxfp4_weight, int8_weight> weight);
 
   public:
     // weight [N, K] in x's dtype.
@@ -50,6 +55,9 @@ class linear {
 
     // codes uint8 [N, K/2], scale uint8 [N, K/32] (quantize_mxfp4_cuda's form); w4a4: x is quantized so, too.
     static linear mxfp4(const at::Tensor& codes, const at::Tensor& scale, bool w4a4);
+
+    // codes int8 [N, K], scale fp32 [N] (quantize_rows_int8_cuda's form); x is quantized so, too, a scale for each token.
+    static linear int8(const at::Tensor& codes, const at::Tensor& scale);
 
     at::Tensor apply(const at::Tensor& x) const;
 };

@@ -31,11 +31,20 @@ PYBIND11_MODULE(_host, m) {
     m.def("gated_mxfp4_cuda", &pulsarlm::gated_mxfp4_cuda);
     m.def("gated_mxfp4_grad_cuda", &pulsarlm::gated_mxfp4_grad_cuda);
     m.def("mlp_mxfp4_w4a4_cuda", &pulsarlm::mlp_mxfp4_w4a4_cuda);
+    m.def("quantize_rows_int8_cuda", &pulsarlm::quantize_rows_int8_cuda);
+    m.def("dequantize_rows_int8_cuda", &pulsarlm::dequantize_rows_int8_cuda);
+    m.def("gemm_int8_cuda", &pulsarlm::gemm_int8_cuda);
+    m.def("gemm_int8_w8a8_cuda", &pulsarlm::gemm_int8_w8a8_cuda);
+    m.def("grouped_gemm_int8_cuda", &pulsarlm::grouped_gemm_int8_cuda);
+    m.def("grouped_gemm_cuda", &pulsarlm::grouped_gemm_cuda);
+    m.def("grouped_gemm_grad_x_cuda", &pulsarlm::grouped_gemm_grad_x_cuda);
+    m.def("grouped_gemm_grad_w_cuda", &pulsarlm::grouped_gemm_grad_w_cuda);
     py::class_<pulsarlm::linear>(m, "linear")
         .def_static("dense", &pulsarlm::linear::dense)
         .def_static("fp8", &pulsarlm::linear::fp8)
         .def_static("fp8_rows", &pulsarlm::linear::fp8_rows)
         .def_static("int4", &pulsarlm::linear::int4)
         .def_static("mxfp4", &pulsarlm::linear::mxfp4)
+        .def_static("int8", &pulsarlm::linear::int8)
         .def("apply", &pulsarlm::linear::apply);
 }

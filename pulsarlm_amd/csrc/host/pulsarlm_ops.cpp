@@ -554,4 +554,192 @@ at::Tensor mlp_mxfp4_w4a4_cuda(const at::Tensor& x, const at::Tensor& gate_weigh
     return y;
 }
 
+// ---- 8-bit integers, and experts in 8 and 16 bits ----
+
+namespace {
+
+bool any_records(std::initializer_list<at::Tensor> inputs) {
+    return std::any_of(inputs.begin(), inputs.end(), [](const at::Tensor& t) { return mx_records(t); });
+}
+
+// As mx_no_gradient, for the quantizer's two outputs.
+struct no_gradient_pair : torch::autograd::Function<no_gradient_pair> {
+    static variable_list forward(AutogradContext* ctx, const char* op, const std::function<variable_list()>& call, const at::Tensor&) {
+        ctx->saved_data["op"] = std::string(op);
+        variable_list out = call();
+        ctx->mark_non_differentiable({out[0]});  // integers
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list&) {
+        TORCH_CHECK(false, ctx->saved_data["op"].toStringRef(), ": has no gradient");
+    }
+};
+
+void int8_rows(const char* op, const char* name, const at::Tensor& codes, const at::Tensor& scale, int64_t dim) {
+    TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kChar && codes.dim() == dim && codes.is_contiguous(), op, ": ", name,
+                " must be a contiguous CUDA int8 tensor of ", dim, " dimensions");
+    TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.device() == codes.device() && scale.is_contiguous() && scale.dim() == dim - 1 &&
+                    scale.sizes() == codes.sizes().slice(0, dim - 1),
+                op, ": ", name, "'s scale must be contiguous fp32, one for each row, on its device");
+}
+void expert_offsets(const char* op, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
+    TORCH_CHECK(weight.device() == x.device() && offsets.device() == x.device(), op, ": x, weight and offsets must be on one device");
+    TORCH_CHECK(offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.size(0) == weight.size(0) && offsets.is_contiguous(), op,
+                ": offsets must be contiguous int32 [E]");
+}
+void expert_weight(const char* op, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
+    TORCH_CHECK(weight.dim() == 3 && weight.scalar_type() == x.scalar_type() && weight.is_contiguous(), op,
+                ": weight must be contiguous [E, N, K] of the rows' type");
+    expert_offsets(op, x, weight, offsets);
+}
+const int8_t* int8_of(const at::Tensor& t) { return static_cast<const int8_t*>(t.data_ptr()); }
+const float* float_of(const at::Tensor& t) { return static_cast<const float*>(t.data_ptr()); }
+const int32_t* int_of(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
+
+struct grouped_linear : torch::autograd::Function<grouped_linear> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
+        ctx->save_for_backward({x, weight, offsets});
+        return grouped_gemm_cuda(x, weight, offsets);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list dy) {
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor d = dy[0].contiguous();
+        return {ctx->needs_input_grad(0) ? grouped_gemm_grad_x_cuda(d, saved[1], saved[2]) : at::Tensor(),
+                ctx->needs_input_grad(1) ? grouped_gemm_grad_w_cuda(d, saved[0], saved[2]) : at::Tensor(), {}};
+    }
+};
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> quantize_rows_int8_cuda(const at::Tensor& x) {
+    const char* op = "quantize_rows_int8";
+    if (mx_records(x)) {
+        const variable_list out = no_gradient_pair::apply(
+            op,
+            [&] {
+                auto [codes, scale] = quantize_rows_int8_cuda(x);
+                return variable_list{codes, scale};
+            },
+            x);
+        return {out[0], out[1]};
+    }
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(), op, ": x must be a contiguous CUDA [M, K]");
+    const plm_dtype dtype = dtype_of(op, x.scalar_type());
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
+    at::Tensor scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+    check_rc(plm_quantize_rows_int8(x.data_ptr(), dtype, x.size(0), x.size(1), static_cast<int8_t*>(codes.data_ptr()),
+                                    static_cast<float*>(scale.data_ptr()), stream_of(x)));
+    return {codes, scale};
+}
+
+at::Tensor dequantize_rows_int8_cuda(const at::Tensor& codes, const at::Tensor& scale, at::ScalarType dtype) {
+    const char* op = "dequantize_rows_int8";
+    if (mx_records(scale))
+        return mx_no_gradient::apply(op, [&] { return dequantize_rows_int8_cuda(codes, scale, dtype); }, scale, scale);
+    int8_rows(op, "codes", codes, scale, 2);
+    const plm_dtype out_dtype = dtype_of(op, dtype);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+    at::Tensor out = at::empty(codes.sizes(), codes.options().dtype(dtype));
+    check_rc(plm_dequantize_rows_int8(int8_of(codes), float_of(scale), codes.size(0), codes.size(1), out.data_ptr(), out_dtype, stream_of(codes)));
+    return out;
+}
+
+at::Tensor gemm_int8_cuda(const at::Tensor& codes, const at::Tensor& x_scale, const at::Tensor& weight, const at::Tensor& scale,
+                          at::ScalarType dtype) {
+    const char* op = "gemm_int8";
+    if (any_records({x_scale, scale}))
+        return mx_no_gradient::apply(op, [&] { return gemm_int8_cuda(codes, x_scale, weight, scale, dtype); }, x_scale, scale);
+    int8_rows(op, "codes", codes, x_scale, 2);
+    int8_rows(op, "weight", weight, scale, 2);
+    TORCH_CHECK(weight.size(1) == codes.size(1) && weight.device() == codes.device(), op,
+                ": weight must be [N, K] for codes [M, K], on their device");
+    TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, op, ": dtype must be fp16 or bf16");
+    const int64_t m = codes.size(0), n = weight.size(0), k = codes.size(1);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+    at::Tensor y = at::empty({m, n}, codes.options().dtype(dtype));
+    const at::Tensor ws = mx_scratch(codes, plm_gemm_int8_workspace_bytes(m, n, k));
+    check_rc(plm_gemm_int8(int8_of(codes), float_of(x_scale), int8_of(weight), float_of(scale), m, n, k, y.data_ptr(), dtype_of(op, dtype),
+                           ptr(ws), mx_bytes(ws), stream_of(codes)));
+    return y;
+}
+
+at::Tensor gemm_int8_w8a8_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale) {
+    const char* op = "gemm_int8_w8a8";
+    if (any_records({x, scale})) return mx_no_gradient::apply(op, [&] { return gemm_int8_w8a8_cuda(x, weight, scale); }, x, scale);
+    mx_rows(op, "x", x);
+    int8_rows(op, "weight", weight, scale, 2);
+    TORCH_CHECK(weight.size(1) == x.size(1) && weight.device() == x.device(), op, ": weight must be [N, K] for x [M, K], on its device");
+    const int64_t m = x.size(0), n = weight.size(0), k = x.size(1);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor y = at::empty({m, n}, x.options());
+    const at::Tensor ws = mx_scratch(x, plm_gemm_int8_w8a8_workspace_bytes(m, n, k));
+    check_rc(plm_gemm_int8_w8a8(x.data_ptr(), dtype_of(op, x.scalar_type()), int8_of(weight), float_of(scale), m, n, k, y.data_ptr(), ptr(ws),
+                                mx_bytes(ws), stream_of(x)));
+    return y;
+}
+
+at::Tensor grouped_gemm_int8_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, const at::Tensor& offsets) {
+    const char* op = "grouped_gemm_int8";
+    if (any_records({x, scale}))
+        return mx_no_gradient::apply(op, [&] { return grouped_gemm_int8_cuda(x, weight, scale, offsets); }, x, scale);
+    mx_rows(op, "x", x);
+    int8_rows(op, "weight", weight, scale, 3);
+    expert_offsets(op, x, weight, offsets);
+    TORCH_CHECK(weight.size(2) == x.size(1), op, ": weight must be [E, N, K] for x [rows, K]");
+    const int64_t rows = x.size(0), n = weight.size(1), k = x.size(1);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor y = at::empty({rows, n}, x.options());
+    const at::Tensor ws = mx_scratch(x, plm_grouped_gemm_int8_workspace_bytes(rows, n, k));
+    check_rc(plm_grouped_gemm_int8(x.data_ptr(), dtype_of(op, x.scalar_type()), int8_of(weight), float_of(scale), int_of(offsets),
+                                   weight.size(0), rows, n, k, y.data_ptr(), 1, ptr(ws), mx_bytes(ws), stream_of(x)));
+    return y;
+}
+
+at::Tensor grouped_gemm_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
+    const char* op = "grouped_gemm";
+    if (any_records({x, weight})) {
+        TORCH_CHECK(weight.dim() != 3 || weight.size(1) % 8 == 0, op, ": N must be a multiple of 8 for the gradients");
+        return grouped_linear::apply(x, weight, offsets);
+    }
+    mx_rows(op, "x", x);
+    expert_weight(op, x, weight, offsets);
+    TORCH_CHECK(weight.size(2) == x.size(1), op, ": weight must be [E, N, K] for x [rows, K]");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    at::Tensor y = at::empty({x.size(0), weight.size(1)}, x.options());
+    check_rc(plm_grouped_gemm_16(x.data_ptr(), dtype_of(op, x.scalar_type()), weight.data_ptr(), int_of(offsets), weight.size(0), x.size(0),
+                                 weight.size(1), x.size(1), y.data_ptr(), 1, stream_of(x)));
+    return y;
+}
+
+at::Tensor grouped_gemm_grad_x_cuda(const at::Tensor& dy, const at::Tensor& weight, const at::Tensor& offsets) {
+    const char* op = "grouped_gemm_grad_x";
+    if (any_records({dy, weight}))
+        return mx_no_gradient::apply(op, [&] { return grouped_gemm_grad_x_cuda(dy, weight, offsets); }, dy, weight);
+    mx_rows(op, "dy", dy);
+    expert_weight(op, dy, weight, offsets);
+    TORCH_CHECK(weight.size(1) == dy.size(1), op, ": weight must be [E, N, K] for dy [rows, N]");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
+    at::Tensor dx = at::empty({dy.size(0), weight.size(2)}, dy.options());
+    check_rc(plm_grouped_gemm_grad_x(dy.data_ptr(), dtype_of(op, dy.scalar_type()), weight.data_ptr(), int_of(offsets), weight.size(0), dy.size(0),
+                                     dy.size(1), weight.size(2), dx.data_ptr(), 1, stream_of(dy)));
+    return dx;
+}
+
+at::Tensor grouped_gemm_grad_w_cuda(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& offsets) {
+    const char* op = "grouped_gemm_grad_w";
+    if (any_records({dy, x})) return mx_no_gradient::apply(op, [&] { return grouped_gemm_grad_w_cuda(dy, x, offsets); }, dy, x);
+    mx_rows(op, "dy", dy);
+    mx_rows(op, "x", x);
+    TORCH_CHECK(x.scalar_type() == dy.scalar_type() && x.size(0) == dy.size(0), op, ": dy and x must have one type and as many rows");
+    TORCH_CHECK(offsets.dim() == 1, op, ": offsets must be contiguous int32 [E]");
+    TORCH_CHECK(x.device() == dy.device() && offsets.device() == dy.device(), op, ": dy, x and offsets must be on one device");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
+    at::Tensor dw = at::empty({offsets.size(0), dy.size(1), x.size(1)}, dy.options());
+    expert_offsets(op, dy, dw, offsets);
+    check_rc(plm_grouped_gemm_grad_w(dy.data_ptr(), x.data_ptr(), dtype_of(op, dy.scalar_type()), int_of(offsets), offsets.size(0), dy.size(0),
+                                     dy.size(1), x.size(1), dw.data_ptr(), stream_of(dy)));
+    return dw;
+}
+
 }  // namespace pulsarlm

@@ -120,4 +120,25 @@ at::Tensor mlp_mxfp4_w4a4_cuda(const at::Tensor& x, const at::Tensor& gate_weigh
                                const at::Tensor& up_weight, const at::Tensor& up_scale, const at::Tensor& down_weight,
                                const at::Tensor& down_scale, int64_t intermediate);
 
+// ---- 8-bit integers with a scale for each token and channel, and experts in 8 and 16 bits (no counterpart in ops.hpp;
+// include/pulsarlm_amd.h has the rules). Weights are row-major: int8 [N, K] with scale fp32 [N], or 16-bit; by expert
+// [E, N, K], offsets int32 [E] the inclusive ends of the experts' rows. grouped_gemm_cuda records its x's and weight's
+// gradients for autograd; a backward pass that reaches another of these raises. ----
+
+// x [M, K] fp32, fp16 or bf16 -> (codes int8 [M, K], scale fp32 [M]), and back.
+std::tuple<at::Tensor, at::Tensor> quantize_rows_int8_cuda(const at::Tensor& x);
+at::Tensor dequantize_rows_int8_cuda(const at::Tensor& codes, const at::Tensor& scale, at::ScalarType dtype);
+
+// y [M, N] = x @ W^T in dtype for quantized x, and with 16-bit x quantized on the way.
+at::Tensor gemm_int8_cuda(const at::Tensor& codes, const at::Tensor& x_scale, const at::Tensor& weight, const at::Tensor& scale,
+                          at::ScalarType dtype);
+at::Tensor gemm_int8_w8a8_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale);
+
+// Each expert's rows of x times its W^T: 8-bit experts as gemm_int8_w8a8_cuda, 16-bit experts, and the latter's gradients.
+// Rows past the last expert's give zeros.
+at::Tensor grouped_gemm_int8_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, const at::Tensor& offsets);
+at::Tensor grouped_gemm_cuda(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets);
+at::Tensor grouped_gemm_grad_x_cuda(const at::Tensor& dy, const at::Tensor& weight, const at::Tensor& offsets);
+at::Tensor grouped_gemm_grad_w_cuda(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& offsets);
+
 }  // namespace pulsarlm

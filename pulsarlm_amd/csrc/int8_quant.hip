@@ -1,46 +1,18 @@
-// Rows of 8-bit integers: quantizer (tokens' activations, a weight's output channels) and its inverse.
-//
-// s = max(amax, 1e-12) / 127 in fp32, q the integer nearest to x / s, ties to even, of the exact quotient: the fp32
-// quotient of a value next to the border between two codes can round onto the border. With q0 = rint(x * (1 / s)), off by
-// at most one, r = x - q0 s is exact in fp32 wherever |r| is near s / 2 (x, q0 s and so r are multiples of s's last bit,
-// of s / 2's where q0 = 0), and says on which side of the border x lies.
-// A row with an infinity or NaN gets s = NaN and codes 0: every product with it is NaN.
-// What bounds it: memory. M = 4096, K 12288, bf16.
+// Rows of 8-bit integers: quantizer (tokens' activations, a weight's output channels; the rule: int8_rows.hpp) and its
+// inverse.
+// What bounds it: memory. M = 4096, K 12288, bf16: quantizer 34 us, 4.5 TB/s; back to fp32 48 us, 5.2 TB/s.
 #include <algorithm>
 
 #include "dense_gemm.hpp"
+#include "int8_rows.hpp"
 
 namespace plm {
 
 namespace {
 
-// Magnitude bits, ordered as the values; infinity is 0x7f800000 and NaNs lie above.
-__device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
-
-struct row_scale {
-    float s, inv, half;  // inv == 0: a row that is not finite
-};
-__device__ __forceinline__ row_scale make_row_scale(uint32_t top) {
-    if (top >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f, 0.f};
-    const float s = fmaxf(__uint_as_float(top), 1e-12f) / 127.f;
-    return {s, 1.f / s, 0.5f * s};
-}
-__device__ __forceinline__ int quantized(float x, const row_scale& k) {
-    if (k.inv == 0.f) return 0;
-    float q = rintf(x * k.inv);
-    const float r = fmaf(-q, k.s, x), a = fabsf(r);
-    const bool odd = static_cast<int>(q) & 1;
-    if (a > k.half || (a == k.half && odd)) q += copysignf(1.f, r);
-    return static_cast<int>(q);
-}
-
 // Eight consecutive values.
 template <plm_dtype D> struct eight {
     u32x4_t v[D == PLM_FP32 ? 2 : 1];
-    __device__ __forceinline__ float get(int i) const {
-        if constexpr (D == PLM_FP32) return __uint_as_float(v[i >> 2][i & 3]);
-        else return from_bits16<D == PLM_BF16>((v[0][i >> 1] >> (16 * (i & 1))) & 0xffffu);
-    }
 };
 template <plm_dtype D> __device__ __forceinline__ eight<D> load_eight(const uint8_t* row, int64_t chunk, bool in) {
     eight<D> e{};
@@ -51,50 +23,68 @@ template <plm_dtype D> __device__ __forceinline__ eight<D> load_eight(const uint
     }
     return e;
 }
+// The running largest magnitude: fp32 bits, or those of both halves of a dword.
 template <plm_dtype D> __device__ __forceinline__ uint32_t top_of(const eight<D>& e, uint32_t top) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, magnitude(e.get(i)));
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (D == PLM_FP32) top = max(top, max(e.v[0][i] & 0x7fffffffu, e.v[1][i] & 0x7fffffffu));
+        else top = top_16(top, e.v[0][i]);
+    }
     return top;
 }
-template <plm_dtype D> __device__ __forceinline__ uint2 codes_of(const eight<D>& e, const row_scale& k) {
-    uint32_t w[2] = {0, 0};
+template <plm_dtype D> __device__ __forceinline__ uint2 codes_of(const eight<D>& e, const int8_scale& k) {
+    if (!k.finite) return make_uint2(0u, 0u);
+    float x[8];
+    if constexpr (D == PLM_FP32) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= (static_cast<uint32_t>(quantized(e.get(i), k)) & 0xffu) << (8 * (i & 3));
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(e.v[i >> 2][i & 3]);
+    } else {
+        eight_values<D == PLM_BF16>(e.v[0], x);
+    }
+    uint32_t w[2];
+    int8_codes<8>(x, k, w);
     return make_uint2(w[0], w[1]);
 }
 
-template <int T> __device__ __forceinline__ uint32_t block_top(uint32_t top, uint32_t* part) {
+__device__ __forceinline__ uint32_t wave_top(uint32_t top) {
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), s)));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < T / 64; ++w) top = max(top, part[w]);
     return top;
 }
 
-// A workgroup a row. The first CAP chunks of eight a thread wait in registers for the row's largest; what is past them
-// is read again.
-template <plm_dtype D, int T, int CAP>
-__global__ void __launch_bounds__(T) quantize_int8_kernel(const uint8_t* __restrict__ x, int64_t k, int8_t* __restrict__ codes,
-                                                          float* __restrict__ scale) {
+// T threads a row, ROWS rows a workgroup (T == 64: a wavefront each, which needs no barrier). The first CAP chunks of
+// eight a thread wait in registers for the row's largest; what is past them is read again.
+template <plm_dtype D, int T, int ROWS, int CAP>
+__global__ void __launch_bounds__(T * ROWS) quantize_int8_kernel(const uint8_t* __restrict__ x, int64_t m, int64_t k, int8_t* __restrict__ codes,
+                                                                 float* __restrict__ scale) {
+    static_assert(ROWS == 1 || T == 64, "rows of a wavefront each");
     __shared__ uint32_t part[T / 64];
-    const int64_t row = blockIdx.x, chunks = k >> 3;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / T, chunks = k >> 3;
+    const int at = threadIdx.x % T;
+    if (ROWS > 1 && row >= m) return;
     const uint8_t* from = x + row * k * (D == PLM_FP32 ? 4 : 2);
     uint2* to = reinterpret_cast<uint2*>(codes + row * k);
     eight<D> held[CAP];
 #pragma unroll
-    for (int c = 0; c < CAP; ++c) held[c] = load_eight<D>(from, threadIdx.x + c * T, threadIdx.x + c * T < chunks);
+    for (int c = 0; c < CAP; ++c) held[c] = load_eight<D>(from, at + c * T, at + c * T < chunks);
     uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < CAP; ++c) top = top_of(held[c], top);
-    for (int64_t c = threadIdx.x + CAP * T; c < chunks; c += T) top = top_of(load_eight<D>(from, c, true), top);
-    const row_scale s = make_row_scale(block_top<T>(top, part));
-    if (threadIdx.x == 0) scale[row] = s.s;
+    for (int64_t c = at + CAP * T; c < chunks; c += T) top = top_of(load_eight<D>(from, c, true), top);
+    if constexpr (D != PLM_FP32) top = top_bits<D == PLM_BF16>(top);
+    top = wave_top(top);
+    if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) top = max(top, part[w]);
+    }
+    const int8_scale s = make_int8_scale(top);
+    if (at == 0) scale[row] = s.s;
 #pragma unroll
     for (int c = 0; c < CAP; ++c)
-        if (threadIdx.x + c * T < chunks) to[threadIdx.x + c * T] = codes_of(held[c], s);
-    for (int64_t c = threadIdx.x + CAP * T; c < chunks; c += T) to[c] = codes_of(load_eight<D>(from, c, true), s);
+        if (at + c * T < chunks) to[at + c * T] = codes_of(held[c], s);
+    for (int64_t c = at + CAP * T; c < chunks; c += T) to[c] = codes_of(load_eight<D>(from, c, true), s);
 }
 
 template <plm_dtype D> __device__ __forceinline__ float load_one(const void* x, int64_t at) {
@@ -108,10 +98,18 @@ __global__ void __launch_bounds__(256) quantize_int8_any_kernel(const void* __re
     __shared__ uint32_t part[4];
     const int64_t row = blockIdx.x;
     uint32_t top = 0;
-    for (int64_t i = threadIdx.x; i < k; i += 256) top = max(top, magnitude(load_one<D>(x, row * k + i)));
-    const row_scale s = make_row_scale(block_top<256>(top, part));
+    for (int64_t i = threadIdx.x; i < k; i += 256) top = max(top, int8_magnitude(load_one<D>(x, row * k + i)));
+    top = wave_top(top);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    const int8_scale s = make_int8_scale(max(max(part[0], part[1]), max(part[2], part[3])));
     if (threadIdx.x == 0) scale[row] = s.s;
-    for (int64_t i = threadIdx.x; i < k; i += 256) codes[row * k + i] = static_cast<int8_t>(quantized(load_one<D>(x, row * k + i), s));
+    for (int64_t i = threadIdx.x; i < k; i += 256) {
+        const float v[4] = {load_one<D>(x, row * k + i), 0.f, 0.f, 0.f};
+        uint32_t code[1] = {0};
+        if (s.finite) int8_codes<4>(v, s, code);
+        codes[row * k + i] = static_cast<int8_t>(code[0]);
+    }
 }
 
 template <plm_dtype D> void launch_quantize(const void* x, int64_t m, int64_t k, int8_t* codes, float* scale, hipStream_t s) {
@@ -121,50 +119,68 @@ template <plm_dtype D> void launch_quantize(const void* x, int64_t m, int64_t k,
         quantize_int8_any_kernel<D><<<grid, 256, 0, s>>>(x, k, codes, scale);
         return;
     }
-    // Few rows: many threads each, for loads in flight; many rows fill the GPU by themselves.
+    // Few rows: many threads each, for loads in flight. Enough of them: a wavefront each, where it holds the row. M = 512,
+    // K 4096: 5.6 us with 256 threads, 8.6 with wavefronts; M = 32768, K 2048: 83 and 42.
     constexpr int CAP = D == PLM_FP32 ? 4 : 8;
-    if (m < 2 * cu_count()) quantize_int8_kernel<D, 1024, CAP / 2><<<grid, 1024, 0, s>>>(bytes, k, codes, scale);
-    else quantize_int8_kernel<D, 256, CAP><<<grid, 256, 0, s>>>(bytes, k, codes, scale);
+    if (m < cu_count()) quantize_int8_kernel<D, 1024, 1, CAP / 2><<<grid, 1024, 0, s>>>(bytes, m, k, codes, scale);
+    else if (m >= 8 * cu_count() && k <= 64 * 8 * CAP)
+        quantize_int8_kernel<D, 64, 4, CAP><<<static_cast<unsigned>(ceil_div(m, 4)), 256, 0, s>>>(bytes, m, k, codes, scale);
+    else quantize_int8_kernel<D, 256, 1, CAP><<<grid, 256, 0, s>>>(bytes, m, k, codes, scale);
 }
 
-// Sixteen codes a thread, or one.
-template <plm_dtype D, bool WIDE>
-__global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scale, int64_t total,
-                                                              int64_t k, void* __restrict__ out) {
-    constexpr int N = WIDE ? 16 : 1;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total / N; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t at = i * N;
-        const float s = scale[at / k];
-        if constexpr (WIDE) {
-            const u32x4_t c = *reinterpret_cast<const u32x4_t*>(codes + at);
-            float f[16];
+// Items of N codes, 16 bytes of output (or one value, where rows are not whole items or not aligned): four a thread, a
+// workgroup's width apart, so that a wavefront's loads and stores are contiguous. INDEX: 32 bits where the items fit, for
+// the division by the items of a row.
+template <plm_dtype D, int N, typename INDEX>
+__global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scale, INDEX items,
+                                                              INDEX per_row, void* __restrict__ out) {
+    constexpr int EACH = 4;
+    const INDEX first = static_cast<INDEX>(blockIdx.x) * (256 * EACH) + threadIdx.x;
+    uint32_t c[EACH][N == 8 ? 2 : 1];
+    float s[EACH];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] = static_cast<float>(static_cast<int8_t>(c[j >> 2] >> (8 * (j & 3)))) * s;
-            if constexpr (D == PLM_FP32) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) reinterpret_cast<f32x4_t*>(static_cast<float*>(out) + at)[j] = f32x4_t{f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]};
-            } else {
-                u32x4_t* to = reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(out) + at);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float* g = f + 8 * j;
-                    to[j] = u32x4_t{pack2<D == PLM_BF16>(g[0], g[1]), pack2<D == PLM_BF16>(g[2], g[3]), pack2<D == PLM_BF16>(g[4], g[5]), pack2<D == PLM_BF16>(g[6], g[7])};
-                }
-            }
+    for (int e = 0; e < EACH; ++e) {
+        const INDEX i = first + e * 256;
+        if (i >= items) continue;
+        if constexpr (N == 8) {
+            const uint2 w = reinterpret_cast<const uint2*>(codes)[i];
+            c[e][0] = w.x, c[e][1] = w.y;
+        } else if constexpr (N == 4) {
+            c[e][0] = reinterpret_cast<const uint32_t*>(codes)[i];
         } else {
-            const float f = static_cast<float>(codes[at]) * s;
-            if constexpr (D == PLM_FP32) static_cast<float*>(out)[at] = f;
-            else static_cast<uint16_t*>(out)[at] = static_cast<uint16_t>(to_bits16<D == PLM_BF16>(f));
+            c[e][0] = static_cast<uint8_t>(codes[i]);
         }
+        s[e] = scale[i / per_row];
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const INDEX i = first + e * 256;
+        if (i >= items) continue;
+        float f[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = static_cast<float>(static_cast<int8_t>(c[e][j >> 2] >> (8 * (j & 3)))) * s[e];
+        if constexpr (N == 8) reinterpret_cast<u32x4_t*>(out)[i] = u32x4_t{pack2<D == PLM_BF16>(f[0], f[1]), pack2<D == PLM_BF16>(f[2], f[3]), pack2<D == PLM_BF16>(f[4], f[5]), pack2<D == PLM_BF16>(f[6], f[7])};
+        else if constexpr (N == 4) reinterpret_cast<f32x4_t*>(out)[i] = f32x4_t{f[0], f[1], f[2], f[3]};
+        else if constexpr (D == PLM_FP32) static_cast<float*>(out)[i] = f[0];
+        else static_cast<uint16_t*>(out)[i] = static_cast<uint16_t>(to_bits16<D == PLM_BF16>(f[0]));
     }
 }
 
+template <plm_dtype D, int N> void launch_items(const int8_t* codes, const float* scale, int64_t m, int64_t k, void* out, hipStream_t s) {
+    // Whole rows at a time, as many as a grid holds.
+    const int64_t most = std::max<int64_t>(1, (int64_t{1} << 33) / k);
+    for (int64_t row = 0; row < m; row += most) {
+        const int64_t rows = std::min(most, m - row), items = rows * k / N, at = row * k;
+        const unsigned grid = static_cast<unsigned>(ceil_div(items, 1024));
+        void* to = static_cast<uint8_t*>(out) + at * (D == PLM_FP32 ? 4 : 2);
+        if (items < int64_t{1} << 31) dequantize_int8_kernel<D, N, uint32_t><<<grid, 256, 0, s>>>(codes + at, scale + row, items, k / N, to);
+        else dequantize_int8_kernel<D, N, uint64_t><<<grid, 256, 0, s>>>(codes + at, scale + row, items, k / N, to);
+    }
+}
 template <plm_dtype D> void launch_dequantize(const int8_t* codes, const float* scale, int64_t m, int64_t k, void* out, hipStream_t s) {
-    const int64_t total = m * k;
-    const bool wide = k % 16 == 0 && aligned(codes, 16) && aligned(out, 16);
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(total / (wide ? 16 : 1), 256), int64_t{64} * cu_count()));
-    if (wide) dequantize_int8_kernel<D, true><<<grid, 256, 0, s>>>(codes, scale, total, k, out);
-    else dequantize_int8_kernel<D, false><<<grid, 256, 0, s>>>(codes, scale, total, k, out);
+    constexpr int N = D == PLM_FP32 ? 4 : 8;
+    if (k % N == 0 && aligned(codes, N) && aligned(out, 16)) launch_items<D, N>(codes, scale, m, k, out, s);
+    else launch_items<D, 1>(codes, scale, m, k, out, s);
 }
 
 }  // namespace
