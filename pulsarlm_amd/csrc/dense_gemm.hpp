@@ -66,18 +66,31 @@ struct expert_range {
     int expert, lo, hi;
 };
 
-// Expert e's rows.
-__device__ __forceinline__ expert_range find_expert(const int32_t* __restrict__ offsets, int e, int rows) {
+// The rows of the expert at place `slot`. Up to 64 experts are placed by their rows, most first (their products' times go
+// by them, and the longest should not begin last), more of them as they come.
+__device__ __forceinline__ expert_range find_expert(const int32_t* __restrict__ offsets, int n, int rows, int slot) {
     const int lane = __lane_id();
+    if (n <= 64) {
+        const int hi = wave_inclusive_max(lane < n ? min(max(offsets[lane], 0), rows) : 0);
+        int lo = __shfl_up(hi, 1);
+        if (lane == 0) lo = 0;
+        const int count = lane < n ? hi - lo : -1;
+        int place = 0;
+        for (int i = 0; i < n; ++i) {
+            const int other = __builtin_amdgcn_readlane(count, i);
+            place += other > count || (other == count && i < lane) ? 1 : 0;
+        }
+        const int e = __ffsll(static_cast<unsigned long long>(__ballot(lane < n && place == slot))) - 1;
+        return {e, __builtin_amdgcn_readlane(lo, e), __builtin_amdgcn_readlane(hi, e)};
+    }
     int lo = 0, hi = 0;
-    for (int base = 0; base <= e; base += 64) {
+    for (int base = 0; base <= slot; base += 64) {
         const int i = base + lane;
-        const int v = i <= e ? min(max(offsets[i], 0), rows) : 0;
-        const int before = i < e ? v : 0;
-        lo = max(lo, __builtin_amdgcn_readlane(wave_inclusive_max(before), 63));
+        const int v = i <= slot ? min(max(offsets[i], 0), rows) : 0;
+        lo = max(lo, __builtin_amdgcn_readlane(wave_inclusive_max(i < slot ? v : 0), 63));
         hi = max(hi, __builtin_amdgcn_readlane(wave_inclusive_max(v), 63));
     }
-    return {e, lo, hi};
+    return {slot, lo, hi};
 }
 
 // Row blocks of `1 << shift` rows, expert by expert; where rest is set, the rows past the last expert's count as

@@ -17,7 +17,17 @@ struct tile_cost {
     double one_few, one_all, two;
 };
 constexpr tile_cost kTileCosts[] = {{256, 256, 512, 1.28, 1.54, 0.}, {128, 256, 512, .88, .98, 0.}, {128, 128, 256, .57, .66, 0.},
-                                    {128, 128, 256, .87, .92, 1.12}, {64, 128, 256, .47, .52, .80}, {64, 64, 256, .31, .33, .55}};
+                                    {128, 128, 256, .87, .92, 1.12}, {64, 128, 256, .47, .52, .80}, {64, 64, 256, .31, .33, .55},
+                                    {128, 256, 256, 1.2, 1.2, 1.84}};
+constexpr int kRowShapes = 6;  // the last is for sums over the experts' rows only, which are short: pairs hide each other's ends
+// There a round's own time comes on top, and operands across the sum take longer.
+double ranges_time(int shape, const tile_cost& c, double tiles, int64_t stages) {
+    const double each = tiles / cu_count() > 1. ? static_cast<double>(static_cast<int64_t>(tiles / cu_count() + .999)) : 1.;
+    if (shape == 0) return each * (1.8 * stages + 7.);
+    if (shape == 6) return each * (.92 * stages + 3.2);
+    if (shape == 1) return each * (1.1 * stages + 3.6);
+    return (c.two > 0. ? each / 2. * c.two : each * c.one_all) * (stages + 4) + 2. * each;
+}
 // Workgroups of the busiest CU; past a few, and where their number is a guess, the average and a half.
 double rounds_of(double tiles, bool guess) {
     const double each = tiles / cu_count();
@@ -53,7 +63,7 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
         return best;
     }
     const double used = mode == kByRows ? p.experts * (1. - std::exp(-static_cast<double>(p.rows) / p.experts)) : 1.;
-    const double memory = mode == kByRanges ? 0. : kStart + used * p.cols * depth * size / kMemoryRate;
+    const double memory = kStart + (mode == kByRanges ? 1. * p.experts * p.rows * p.cols : used * p.cols * depth) * size / kMemoryRate;
     auto blocks_of = [&](int64_t rows) {
         if (mode != kByRows) return static_cast<double>(ceil_div(p.rows, rows));
         return used + std::max(0., static_cast<double>(p.rows) / rows - .5 * used);
@@ -61,7 +71,7 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
     // What takes longer hides most of the other.
     auto together = [](double a, double b) { return std::max(a, b) + .3 * std::min(a, b); };
     double least = 1e300;
-    for (int i = 0; i < 6; ++i) {
+    for (int i = 0; i < (mode == kByRanges ? 7 : kRowShapes); ++i) {
         const tile_cost& c = kTileCosts[i];
         const int64_t cols = ceil_div(p.cols, c.cols), experts = mode == kByRanges ? p.experts : 1;
         if (i > 0 && !dense_grid_fits(dense_row_blocks(p, mode, c.rows) * cols * experts, c.threads)) continue;
@@ -70,7 +80,8 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
         for (int64_t splits = 1; splits <= most; ++splits) {
             const int64_t each = ceil_div(stages, splits);
             if (ceil_div(stages, each) != splits) continue;  // no part without a stage
-            double time = together(memory, rounds_time(c, tiles * splits, mode == kByRows) * (each + 4));
+            double time = mode == kByRanges ? together(memory, ranges_time(i, c, tiles, stages))
+                                            : together(memory, rounds_time(c, tiles * splits, mode == kByRows) * (each + 4));
             if (splits > 1) time += kCombine + splits * p.rows * p.cols * 8 / kPartRate;
             if (time < least) least = time, best = {i, static_cast<int>(splits), 0};
         }

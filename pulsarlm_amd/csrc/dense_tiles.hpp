@@ -1,11 +1,11 @@
 // The tile kernel of the products on unpacked weights (dense_gemm.hpp): a workgroup owns a tile of (WM MT 16) rows by
 // (WN NT 16) columns, its WM x WN wavefronts MT x NT products of 16 x 16 each.
 //
-// * A stage is 128 bytes of K (64 values in 16 bits, 128 in 8), two slices of the matrix instruction's. P's and Q's
+// * A stage is 64 SL bytes of K, SL slices of the matrix instruction's (32 values in 16 bits, 64 in 8). P's and Q's
 //   parts of it go from memory straight into LDS, into rings of S + PX and S. Where an operand lies along the sum, its
-//   rows are there with their 16-byte pieces XOR-swizzled by row; where it lies across (gradients), 64 rows of the sum's
+//   rows are there with their 16-byte pieces XOR-swizzled by row; where it lies across (gradients), 32 SL rows of the sum's
 //   index, 32-byte pieces swizzled, and the fragments are read with the transposing LDS read.
-// * One barrier a stage, before its second slice's matrix instructions, whose operands are in registers by then: past it
+// * One barrier a stage, before its last slice's matrix instructions, whose operands are in registers by then: past it
 //   the stage's room is free for loads, and stage kt + 1 has landed and is read while they run.
 // * Q is the A operand and P the B operand: a lane ends with four neighbouring columns of a row.
 #pragma once
@@ -44,12 +44,12 @@ template <int N, typename F> __device__ __forceinline__ void unrolled(F f) {
 
 
 // One operand: BLOCK rows or columns of the tile.
-template <bool CROSS, int BLOCK, int NW> struct dense_operand {
-    static constexpr int kBytes = BLOCK * 128;          // of a stage
+template <bool CROSS, int BLOCK, int NW, int SL> struct dense_operand {
+    static constexpr int kBytes = BLOCK * 64 * SL;      // of a stage
     static constexpr int kLoads = kBytes / 1024 / NW;   // of a wavefront
     static_assert(kBytes % (1024 * NW) == 0, "every wavefront loads as much");
-    // Along: 8 rows a load. Across: rows of the sum's index, BLOCK values each.
-    static constexpr int kPitch = CROSS ? BLOCK * 2 : 128;
+    // Along: rows of 64 SL bytes. Across: rows of the sum's index, BLOCK values each.
+    static constexpr int kPitch = CROSS ? BLOCK * 2 : 64 * SL;
     static constexpr int kRowsLoad = 1024 / kPitch;
     static_assert(!CROSS || (NW * kRowsLoad) % 8 == 0, "the swizzle repeats");
 };
@@ -60,24 +60,22 @@ __device__ __forceinline__ constexpr int cross_swizzle(int k, int pieces) {
     return pieces >= 8 ? (k & 3) << 1 | (((k >> 2) ^ (k >> 3)) & 1) : pieces == 4 ? (k & 2) | ((k >> 3) & 1) : (k >> 3) & 1;
 }
 
-// KG: groups of WM x WN wavefronts that take the stages in turn, each with rings of its own; their sums meet in LDS.
-template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX, int KG>
-__global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_args a) {
+// SL: slices of a stage. EU: wavefronts that a SIMD is to hold.
+template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX, int SL, int EU>
+__global__ void __launch_bounds__(WM * WN * 64, EU) dense_tile_kernel(dense_args a) {
     constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
-    using P = dense_operand<PC, BM, NW>;
-    using Q = dense_operand<QC, BN, NW>;
+    using P = dense_operand<PC, BM, NW, SL>;
+    using Q = dense_operand<QC, BN, NW, SL>;
     using acc_t = dense_acc<T>;
     constexpr int P_RING = (S + PX) * P::kBytes, LDS = P_RING + S * Q::kBytes;
     constexpr int SIZE = T == kInt8 ? 1 : 2;
-    constexpr int DEPTH = 128 / SIZE;  // of the sum, a stage
-    constexpr bool SPLITS = T == kInt8 && MODE == kDense && KG == 1;
+    constexpr int STAGE = 64 * SL, DEPTH = STAGE / SIZE;  // of the sum, bytes and elements
+    constexpr bool SPLITS = T == kInt8 && MODE == kDense;
     static_assert(T != kInt8 || (!PC && !QC), "8-bit operands lie along the sum");
-    static_assert(KG * LDS <= 160 * 1024, "LDS");
-    __shared__ __attribute__((aligned(1024))) uint8_t all_lds[KG * LDS];
+    static_assert(LDS <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
 
-    const int lane = threadIdx.x & 63;
-    const int group = KG == 1 ? 0 : uniform(threadIdx.x >> 6) / NW, wave = uniform(threadIdx.x >> 6) % NW;
-    uint8_t* lds = all_lds + group * LDS;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN, col16 = lane & 15, kq = lane >> 4;
 
     // The workgroup's tile. Workgroups go round the 8 XCDs by id: each takes one run of the tiles, which are ordered in
@@ -86,13 +84,12 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
     static_assert(1 << SHIFT == BM, "row blocks are powers of two");
     int m_blocks = a.m_blocks;
     if constexpr (MODE == kByRows) m_blocks = count_blocks(a.offsets, a.experts, a.rows, a.zero_rest, SHIFT);
-    const int per_expert = m_blocks * a.n_blocks, tiles = MODE == kByRanges ? per_expert * a.experts : per_expert;
-    const int id = blockIdx.x;
+    // (By ranges, of an expert's tiles: experts can differ in depth by far.)
+    int id = blockIdx.x, expert = 0;
+    const int tiles = m_blocks * a.n_blocks;
+    if constexpr (MODE == kByRanges) expert = id / tiles, id -= expert * tiles;
     if (id >= tiles) return;
-    const int xcd = id & 7;
-    int lin = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (id >> 3);
-    int expert = 0;
-    if constexpr (MODE == kByRanges) expert = lin / per_expert, lin -= expert * per_expert;
+    const int xcd = id & 7, lin = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (id >> 3);
     const int band0 = lin / (a.band * a.n_blocks) * a.band;
     const int band_rows = min(a.band, m_blocks - band0), in_band = lin - band0 * a.n_blocks;
     const int nb = in_band / band_rows, mb = band0 + in_band % band_rows;
@@ -103,8 +100,8 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
         expert = r.expert, row0 = r.lo, rows = r.hi - r.lo;
         if (expert == a.experts) rest = true, expert = 0, depth = 0;
     } else if constexpr (MODE == kByRanges) {
-        const expert_range r = find_expert(a.offsets, expert, a.depth);
-        first = r.lo, depth = r.hi - r.lo;
+        const expert_range r = find_expert(a.offsets, a.experts, a.depth, expert);
+        expert = r.expert, first = r.lo, depth = r.hi - r.lo;
     }
     const int col0 = nb * BN;
     // The workgroup's part of the sum: from stage `skipped` on, `depth` to its end.
@@ -118,8 +115,8 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
     const uint8_t* q_base = a.q + (MODE == kByRows ? expert * a.q_expert : 0) +
                             (QC ? static_cast<int64_t>(first) * a.pitch_q + col0 * 2 : static_cast<int64_t>(col0) * a.pitch_q);
     const int q_rows = min(BN, a.cols - col0);
-    // Along: the lane's row and 16-byte piece of a load, swizzled.
-    const int along_row = lane >> 3, along_piece = (lane & 7) ^ along_row;
+    // Along: the lane's row and 16-byte piece of a load, swizzled (rows of 64 bytes by pairs).
+    const int along_row = lane / (4 * SL), along_piece = lane % (4 * SL) ^ (SL == 2 ? along_row & 7 : (along_row >> 1) & 3);
     // Across: its row of the sum and where its 16 bytes lie in it; the swizzle of loads an odd number apart differs by 4
     // where a turn of the wavefronts is 8 rows.
     auto across = [&](auto operand, int parity, int limit) {
@@ -146,26 +143,26 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
         int v[2];  // of even and odd loads
     };
     auto along = [&](int kt, const uint8_t* base, int block_rows, int pitch) {
-        const int left = depth * SIZE - kt * 128;  // bytes of the sum
+        const int left = depth * SIZE - kt * STAGE;  // bytes of the sum
         const int v = along_piece * 16 < left ? along_row * pitch + along_piece * 16 : kOOB;
-        return source{buffer_words(base + kt * 128, left > 0 ? static_cast<uint32_t>(block_rows) * pitch - kt * 128 : 0u), {v, v}};
+        return source{buffer_words(base + kt * STAGE, left > 0 ? static_cast<uint32_t>(block_rows) * pitch - kt * STAGE : 0u), {v, v}};
     };
     auto cross = [&](int kt, const uint8_t* base, int pitch, int column, const int (&v)[2]) {
         const int left = min(depth - kt * DEPTH, DEPTH);
         return source{buffer_words(base + static_cast<int64_t>(kt) * DEPTH * pitch, left > 0 ? static_cast<uint32_t>(left) * pitch - column * 2 : 0u), {v[0], v[1]}};
     };
     auto source_p = [&](int turn) {
-        const int kt = skipped + turn * KG + group;
+        const int kt = skipped + turn;
         if constexpr (PC) return cross(kt, p_base, a.pitch_p, row0, p_cross);
         else return along(kt, p_base, rows, a.pitch_p);
     };
     auto source_q = [&](int turn) {
-        const int kt = skipped + turn * KG + group;
+        const int kt = skipped + turn;
         if constexpr (QC) return cross(kt, q_base, a.pitch_q, col0, q_cross);
         else return along(kt, q_base, q_rows, a.pitch_q);
     };
     // Load l of the wavefront's.
-    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)all_lds)) + group * LDS + wave * 1024;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds)) + wave * 1024;
     auto issue_p = [&](const source& s, auto l, int slot) {
         constexpr int n = decltype(l)::value;
         dma16(s.buffer, lds0 + slot * P::kBytes, n * NW * 1024, s.v[n & 1], (n * NW + wave) * P::kRowsLoad * a.pitch_p);
@@ -177,7 +174,7 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
 
     // Fragment f of slice t.
     auto read_along = [&](const uint8_t* base, int f, int t) {
-        return *reinterpret_cast<const u32x4_t*>(base + (f * 16 + col16) * 128 + (((4 * t + kq) ^ (col16 & 7)) << 4));
+        return *reinterpret_cast<const u32x4_t*>(base + (f * 16 + col16) * STAGE + (((4 * t + kq) ^ (SL == 2 ? col16 & 7 : (col16 >> 1) & 3)) << 4));
     };
     auto read_across = [&](const uint8_t* base, int f, int t, auto operand) {
         using O = decltype(operand);
@@ -218,7 +215,7 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
     }
     // Stage 0 has landed; later, at stage kt's barrier, stage kt + 1, when only these are left:
     constexpr int LEFT = (S - 2) * (P::kLoads + Q::kLoads) + PX * P::kLoads, LEFT0 = (S - 1) * (P::kLoads + Q::kLoads);
-    static_assert(S >= 2 && LEFT0 <= 63 && LEFT <= 63, "the counter's range");
+    static_assert(S >= 2 && (SL == 2 || PX == 0) && LEFT0 <= 63 && LEFT <= 63, "the counter's range");
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LEFT0) : "memory");
     u32x4_t p[2][MT], q[2][NT];
 #pragma unroll
@@ -230,22 +227,24 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
     // fragments, over the first three quarters, so that they are there when it begins, and the loads: a wavefront issues
     // in order, and two such in a row would take longer than a matrix instruction and leave its unit idle.
     constexpr int STEPS = MT * NT, READS = MT + NT, EARLY = STEPS * 3 / 4;
-    auto slice = [&](auto second, int turn) {
-        constexpr int t = decltype(second)::value;
-        constexpr int PL = PX != t ? P::kLoads : 0, QL = t ? Q::kLoads : 0, LOADS = PL + QL;
-        const int pn = t ? (ps + 1 == S + PX ? 0 : ps + 1) : ps, qn = t ? (qs + 1 == S ? 0 : qs + 1) : qs;
+    // slice: which of the two sets of fragments is multiplied; last: it ends a stage.
+    auto slice = [&](auto which, auto ends, int turn) {
+        constexpr int w = decltype(which)::value, last = decltype(ends)::value;
+        constexpr int next_t = last ? 0 : 1;
+        constexpr int PL = PX != last ? P::kLoads : 0, QL = last ? Q::kLoads : 0, LOADS = PL + QL;
+        const int pn = last ? (ps + 1 == S + PX ? 0 : ps + 1) : ps, qn = last ? (qs + 1 == S ? 0 : qs + 1) : qs;
         source from_p, from_q;
         if constexpr (PL > 0) from_p = source_p(turn + S);
         if constexpr (QL > 0) from_q = source_q(turn + S);
-        if constexpr (t) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+        if constexpr (last) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
         unrolled<STEPS>([&](auto step) {
             constexpr int s = decltype(step)::value, i = s / NT, j = s % NT;
-            acc[i][j] = dense_mfma<T>(q[t][j], p[t][i], acc[i][j]);
+            acc[i][j] = dense_mfma<T>(q[w][j], p[w][i], acc[i][j]);
             unrolled<READS>([&](auto read) {
                 constexpr int f = decltype(read)::value;
                 if constexpr (f * EARLY / READS == s) {
-                    if constexpr (f < NT) q[t ^ 1][f] = read_q(f, qn, t ^ 1);
-                    else p[t ^ 1][f - NT] = read_p(f - NT, pn, t ^ 1);
+                    if constexpr (f < NT) q[w ^ 1][f] = read_q(f, qn, next_t);
+                    else p[w ^ 1][f - NT] = read_p(f - NT, pn, next_t);
                 }
             });
             unrolled<LOADS>([&](auto load) {
@@ -257,38 +256,19 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
             });
             __builtin_amdgcn_sched_barrier(0);
         });
-        if constexpr (t) {
+        if constexpr (last) {
             p_to = ps;
             ps = pn, qs = qn;
         }
     };
-    const int turns = (stages + KG - 1) / KG;  // past the last stage of zeros
-    for (int turn = 0; turn < turns; ++turn) {
-        slice(std::integral_constant<int, 0>{}, turn);
-        slice(std::integral_constant<int, 1>{}, turn);
+    constexpr std::integral_constant<int, 0> zero{};
+    constexpr std::integral_constant<int, 1> one{};
+    for (int turn = 0; turn < stages; turn += 3 - SL) {
+        slice(zero, std::integral_constant<int, SL == 1>{}, turn);
+        if constexpr (SL == 2) slice(one, one, turn);
+        else slice(one, one, turn + 1);  // past an odd number of stages one of zeros
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // requests past the end; LDS is free
-
-    if constexpr (KG > 1) {
-        // In group order, so that the result does not depend on which is done first.
-        static_assert((KG - 1) * NW * MT * NT * 1024 <= KG * LDS, "the sums fit");
-        acc_t* sums = reinterpret_cast<acc_t*>(all_lds);
-        if (group > 0)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) sums[(((group - 1) * NW + wave) * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
-        __syncthreads();
-        if (group == 0)
-#pragma unroll
-            for (int g = 0; g < KG - 1; ++g)
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = acc[i][j] + sums[((g * NW + wave) * MT * NT + i * NT + j) * 64 + lane];
-        __syncthreads();
-        if (group > 0) return;
-    }
 
     if constexpr (SPLITS) {
         if (a.partial != nullptr) {
@@ -312,9 +292,9 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
     auto finish = [&](auto bf16) {
         constexpr bool BF16 = decltype(bf16)::value;
         constexpr int COLS = NT * 16, PITCH = COLS * 2 + 16, CH = COLS / 8;
-        constexpr int FIT = KG * LDS / (NW * 16 * PITCH), RB = FIT >= MT ? MT : (FIT >= 4 ? 4 : (FIT >= 2 ? 2 : 1));
+        constexpr int FIT = LDS / (NW * 16 * PITCH), RB = FIT >= MT ? MT : (FIT >= 4 ? 4 : (FIT >= 2 ? 2 : 1));
         static_assert(FIT >= 1 && MT % RB == 0, "the rows fit");
-        uint8_t* mine = all_lds + wave * RB * 16 * PITCH;
+        uint8_t* mine = lds + wave * RB * 16 * PITCH;
         const int c0 = col0 + wn * COLS;
         uint16_t* y = a.y + (MODE == kByRanges ? expert * static_cast<int64_t>(a.rows) * a.cols : 0);
         f32x4_t channel[NT];
@@ -369,7 +349,7 @@ __global__ void __launch_bounds__(WM * WN * 64 * KG) dense_tile_kernel(dense_arg
     else finish(std::false_type{});
 }
 
-template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX, int KG = 1>
+template <dense_type T, dense_mode MODE, bool PC, bool QC, int WM, int WN, int MT, int NT, int S, int PX, int SL = 2, int EU = 1>
 void launch_tile(const dense_product& p, hipStream_t s) {
     constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
     dense_args a = make_dense_args(p, PC, QC);
@@ -380,12 +360,12 @@ void launch_tile(const dense_product& p, hipStream_t s) {
     dim3 grid(static_cast<unsigned>(tiles));
     if (T == kInt8 && MODE == kDense && p.plan.splits > 1) {
         grid.y = static_cast<unsigned>(p.plan.splits);
-        a.split_stages = static_cast<int>(ceil_div(ceil_div(p.depth, 128), p.plan.splits));
+        a.split_stages = static_cast<int>(ceil_div(ceil_div(p.depth, 64 * SL), p.plan.splits));
         a.partial = p.partial;
     } else {
         a.split_stages = 1 << 20;
     }
-    dense_tile_kernel<T, MODE, PC, QC, WM, WN, MT, NT, S, PX, KG><<<grid, WM * WN * 64 * KG, 0, s>>>(a);
+    dense_tile_kernel<T, MODE, PC, QC, WM, WN, MT, NT, S, PX, SL, EU><<<grid, WM * WN * 64, 0, s>>>(a);
 }
 
 template <dense_type T, dense_mode MODE, bool PC, bool QC> void launch_shape(const dense_product& p, hipStream_t s) {
@@ -395,6 +375,9 @@ template <dense_type T, dense_mode MODE, bool PC, bool QC> void launch_shape(con
         case 2: return launch_tile<T, MODE, PC, QC, 2, 2, 4, 4, 5, 0>(p, s);
         case 3: return launch_tile<T, MODE, PC, QC, 2, 2, 4, 4, 2, 0>(p, s);
         case 4: return launch_tile<T, MODE, PC, QC, 2, 2, 2, 4, 3, 0>(p, s);
+        case 6:
+            if constexpr (MODE == kByRanges) return launch_tile<T, MODE, PC, QC, 2, 2, 4, 8, 3, 0, 1, 2>(p, s);
+            [[fallthrough]];
         default: return launch_tile<T, MODE, PC, QC, 2, 2, 2, 2, 4, 0>(p, s);
     }
 }
