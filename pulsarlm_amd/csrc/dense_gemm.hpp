@@ -66,9 +66,12 @@ struct expert_range {
     int expert, lo, hi;
 };
 
-// The rows of the expert at place `slot`. Up to 64 experts are placed by their rows, most first (their products' times go
-// by them, and the longest should not begin last), more of them as they come.
-__device__ __forceinline__ expert_range find_expert(const int32_t* __restrict__ offsets, int n, int rows, int slot) {
+// A lane's value from lane `at`.
+__device__ __forceinline__ int from_lane(int v, int at) { return __builtin_amdgcn_ds_bpermute(at * 4, v); }
+
+// The rows of the expert at each lane's place `slot`. Up to 64 experts are placed by their rows, most first (their
+// products' times go by them, and the longest should not begin last), more of them as they come. By a whole wavefront.
+__device__ __forceinline__ expert_range find_experts(const int32_t* __restrict__ offsets, int n, int rows, int slot) {
     const int lane = __lane_id();
     if (n <= 64) {
         const int hi = wave_inclusive_max(lane < n ? min(max(offsets[lane], 0), rows) : 0);
@@ -80,17 +83,21 @@ __device__ __forceinline__ expert_range find_expert(const int32_t* __restrict__ 
             const int other = __builtin_amdgcn_readlane(count, i);
             place += other > count || (other == count && i < lane) ? 1 : 0;
         }
-        const int e = __ffsll(static_cast<unsigned long long>(__ballot(lane < n && place == slot))) - 1;
-        return {e, __builtin_amdgcn_readlane(lo, e), __builtin_amdgcn_readlane(hi, e)};
+        int e = 0;
+        for (int i = 0; i < n; ++i) e = __builtin_amdgcn_readlane(place, i) == slot ? i : e;
+        return {e, from_lane(lo, e), from_lane(hi, e)};
     }
-    int lo = 0, hi = 0;
-    for (int base = 0; base <= slot; base += 64) {
+    expert_range r{slot, 0, 0};
+    for (int base = 0, end = 0; base < n; base += 64) {
         const int i = base + lane;
-        const int v = i <= slot ? min(max(offsets[i], 0), rows) : 0;
-        lo = max(lo, __builtin_amdgcn_readlane(wave_inclusive_max(i < slot ? v : 0), 63));
-        hi = max(hi, __builtin_amdgcn_readlane(wave_inclusive_max(v), 63));
+        const int hi = max(wave_inclusive_max(i < n ? min(max(offsets[i], 0), rows) : 0), end);
+        int lo = __shfl_up(hi, 1);
+        if (lane == 0) lo = end;
+        const int at_lo = from_lane(lo, slot & 63), at_hi = from_lane(hi, slot & 63);
+        if ((slot & ~63) == base) r.lo = at_lo, r.hi = at_hi;
+        end = __builtin_amdgcn_readlane(hi, 63);
     }
-    return {slot, lo, hi};
+    return r;
 }
 
 // Row blocks of `1 << shift` rows, expert by expert; where rest is set, the rows past the last expert's count as
@@ -132,6 +139,23 @@ __device__ __forceinline__ expert_range find_block(const int32_t* offsets, int n
         const int row = __builtin_amdgcn_readlane(lo, at) + ((b - __builtin_amdgcn_readlane(first, at)) << shift);
         r = {base + at, row, min(row + (1 << shift), __builtin_amdgcn_readlane(hi, at))};
         return true;
+    });
+    return r;
+}
+
+// The same for each lane's own b (a result is only used where b < count_blocks(...)).
+__device__ __forceinline__ expert_range find_blocks(const int32_t* offsets, int n, int rows, bool rest, int shift, int b) {
+    expert_range r{0, 0, 0};
+    int before = 0;  // blocks of the experts seen before
+    scan_blocks(offsets, n, rows, rest, shift, [&](int base, int lo, int hi, int first, int past) {
+        int at = 0;  // the first expert whose blocks end past b
+#pragma unroll
+        for (int step = 32; step > 0; step >>= 1) at += from_lane(past, at + step - 1) <= b ? step : 0;
+        const int row = from_lane(lo, at) + ((b - from_lane(first, at)) << shift), end = min(row + (1 << shift), from_lane(hi, at));
+        const int blocks = __builtin_amdgcn_readlane(past, 63);
+        if (b >= before && b < blocks) r = {base + at, row, end};
+        before = blocks;
+        return false;
     });
     return r;
 }

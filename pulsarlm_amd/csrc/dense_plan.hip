@@ -10,40 +10,40 @@ namespace {
 
 // Times in us, fitted to calls of 1 to 4096 rows, N 1000 to 24576, K 2048 to 17408 from captured graphs, weights cold.
 //
-// A tile shape's time is (stages + 4) x the time of a stage for each round of its workgroups: `one` with one workgroup a
-// CU, from few of them to one on every CU; `two` for a pair on a CU, where two fit.
+// A tile shape's time is that of a stage, for each of its stages, one and a half a tile and two and a half a launch: `one`
+// with one workgroup a CU, from few of them to one on every CU; `two` for a pair on a CU, where two fit.
 struct tile_cost {
     int rows, cols, threads;
     double one_few, one_all, two;
 };
-constexpr tile_cost kTileCosts[] = {{256, 256, 512, 1.28, 1.54, 0.}, {128, 256, 512, .88, .98, 0.}, {128, 128, 256, .57, .66, 0.},
-                                    {128, 128, 256, .87, .92, 1.12}, {64, 128, 256, .47, .52, .80}, {64, 64, 256, .31, .33, .55},
-                                    {128, 256, 256, 1.2, 1.2, 1.84}};
-constexpr int kRowShapes = 6;  // the last is for sums over the experts' rows only, which are short: pairs hide each other's ends
-// There a round's own time comes on top, and operands across the sum take longer.
-double ranges_time(int shape, const tile_cost& c, double tiles, int64_t stages) {
-    const double each = tiles / cu_count() > 1. ? static_cast<double>(static_cast<int64_t>(tiles / cu_count() + .999)) : 1.;
-    if (shape == 0) return each * (1.8 * stages + 7.);
-    if (shape == 6) return each * (.92 * stages + 3.2);
-    if (shape == 1) return each * (1.1 * stages + 3.6);
-    return (c.two > 0. ? each / 2. * c.two : each * c.one_all) * (stages + 4) + 2. * each;
+constexpr tile_cost kTileCosts[] = {{256, 256, 512, 1.28, 1.58, 0.}, {128, 256, 512, .88, .94, 0.}, {128, 128, 256, .62, .63, 0.},
+                                    {128, 128, 256, .87, .87, 1.06}, {64, 128, 256, .47, .50, .68}, {64, 64, 256, .31, .33, .52}};
+constexpr double kTileEnds = 1.5, kLaunchEnds = 2.5;
+// Experts' weights through tiles with few rows: E 128, N 1536, K 2048 in 16 bits, 64 rows 74 to 67 us of the kernel for few
+// rows, 256 rows 136 to 123, 512 rows 141 to 144.
+constexpr double kRaggedTiles = 1.1;
+// By ranges: both operands lie across the sum, sums of unequal length, of which the longest is taken as three times the
+// average.
+constexpr double kRangesStage = 1.13, kRangesEnds = 3.;
+double ranges_time(const tile_cost& c, double tiles, int64_t stages) {
+    const double each = std::max(1., tiles / cu_count() / (c.two > 0. ? 2. : 1.)), all = c.two > 0. ? c.two : c.one_all;
+    return kRangesStage * std::max((each * (stages + kRangesEnds) + kLaunchEnds) * all, (3 * stages + kRangesEnds + kLaunchEnds) * c.one_all);
 }
 // Workgroups of the busiest CU; past a few, and where their number is a guess, the average and a half.
 double rounds_of(double tiles, bool guess) {
     const double each = tiles / cu_count();
     return std::max(1., guess && each > 4. ? each + .5 : static_cast<double>(static_cast<int64_t>(each + .999)));
 }
-double rounds_time(const tile_cost& c, double tiles, bool guess) {
+double rounds_time(const tile_cost& c, double tiles, bool guess, int64_t stages) {
     const double each = rounds_of(tiles, guess), one = c.one_few + (c.one_all - c.one_few) * std::min(1., tiles / cu_count());
-    if (c.two == 0.) return each * one;
-    const double pairs = static_cast<double>(static_cast<int64_t>(each) / 2);
-    return pairs * c.two + (each - 2 * pairs) * one;
+    const double pairs = c.two > 0. ? static_cast<double>(static_cast<int64_t>(each) / 2) : 0.;
+    return (pairs * c.two + (each - 2 * pairs) * one) * (stages + kTileEnds) + kLaunchEnds * one;
 }
 // The kernel for few rows: a CU takes in 33 GB/s of its workgroups' x and weights (64 bytes of a row a request), all of
 // them 5.2 TB/s of weights.
 constexpr double kStart = 3.3, kRowsRate = 33e3, kMemoryRate = 5.2e6;
 // A split sum's parts: a kernel more, and their way through memory and back.
-constexpr double kCombine = 3.5, kPartRate = 4.5e6;
+constexpr double kCombine = 4.0, kPartRate = 4.5e6;
 
 // By rows, how the rows fall on the experts is known on the device only. Taken: 1 - e^-a of them have any, with a rows
 // an expert on average, and those have half a block more than whole ones, one at least.
@@ -71,7 +71,7 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
     // What takes longer hides most of the other.
     auto together = [](double a, double b) { return std::max(a, b) + .3 * std::min(a, b); };
     double least = 1e300;
-    for (int i = 0; i < (mode == kByRanges ? 7 : kRowShapes); ++i) {
+    for (int i = 0; i < 6; ++i) {
         const tile_cost& c = kTileCosts[i];
         const int64_t cols = ceil_div(p.cols, c.cols), experts = mode == kByRanges ? p.experts : 1;
         if (i > 0 && !dense_grid_fits(dense_row_blocks(p, mode, c.rows) * cols * experts, c.threads)) continue;
@@ -80,8 +80,8 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
         for (int64_t splits = 1; splits <= most; ++splits) {
             const int64_t each = ceil_div(stages, splits);
             if (ceil_div(stages, each) != splits) continue;  // no part without a stage
-            double time = mode == kByRanges ? together(memory, ranges_time(i, c, tiles, stages))
-                                            : together(memory, rounds_time(c, tiles * splits, mode == kByRows) * (each + 4));
+            double time = mode == kByRanges ? together(memory, ranges_time(c, tiles, stages))
+                                            : together(memory * (mode == kByRows ? kRaggedTiles : 1.), rounds_time(c, tiles * splits, mode == kByRows, each));
             if (splits > 1) time += kCombine + splits * p.rows * p.cols * 8 / kPartRate;
             if (time < least) least = time, best = {i, static_cast<int>(splits), 0};
         }
