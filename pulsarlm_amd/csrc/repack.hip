@@ -85,7 +85,7 @@ tuning parse_tuning() {
     if (const char* e = env("PLM_DENSE")) {
         int v = -1, splits = 1;
         const int got = e[0] != 0 ? sscanf(e + 1, "%d,%d", &v, &splits) : 0;
-        if (got >= 1 && e[0] == 't' && v >= 0 && v < 7) t.dense_tile = v, t.dense_rows = 0, t.dense_splits = std::max(1, splits);
+        if (got >= 1 && e[0] == 't' && v >= 0 && v < 6) t.dense_tile = v, t.dense_rows = 0, t.dense_splits = std::max(1, splits);
         if (got >= 1 && e[0] == 'r' && (v == 0 || v == 16 || v == 32 || v == 64)) t.dense_rows = v;
     }
     return t;

@@ -10,7 +10,7 @@ from tests import _dense as dense
 
 pytestmark = pytest.mark.gpu
 
-KERNELS = [None, "r16", "r32", "r64", *(f"t{i}" for i in range(7))]
+KERNELS = [None, "r16", "r32", "r64", *(f"t{i}" for i in range(6))]
 # Rows of each expert: none, one, whole and part blocks; one expert; more experts than a wavefront's lanes.
 COUNTS = {
     "few": [3, 0, 1, 17],
