@@ -1,6 +1,6 @@
 // Rows of 8-bit integers: quantizer (tokens' activations, a weight's output channels; the rule: int8_rows.hpp) and its
 // inverse.
-// What bounds it: memory. M = 4096, K 12288, bf16: quantizer 34 us, 4.5 TB/s; back to fp32 48 us, 5.2 TB/s.
+// What bounds it: memory. M = 4096, K 12288, bf16: quantizer 31.6 us, 4.8 TB/s; back to fp32 48 us, 5.2 TB/s.
 #include <algorithm>
 
 #include "dense_gemm.hpp"
@@ -119,13 +119,18 @@ template <plm_dtype D> void launch_quantize(const void* x, int64_t m, int64_t k,
         quantize_int8_any_kernel<D><<<grid, 256, 0, s>>>(x, k, codes, scale);
         return;
     }
-    // Few rows: many threads each, for loads in flight. Enough of them: a wavefront each, where it holds the row. M = 512,
-    // K 4096: 5.6 us with 256 threads, 8.6 with wavefronts; M = 32768, K 2048: 83 and 42.
-    constexpr int CAP = D == PLM_FP32 ? 4 : 8;
-    if (m < cu_count()) quantize_int8_kernel<D, 1024, 1, CAP / 2><<<grid, 1024, 0, s>>>(bytes, m, k, codes, scale);
-    else if (m >= 8 * cu_count() && k <= 64 * 8 * CAP)
-        quantize_int8_kernel<D, 64, 4, CAP><<<static_cast<unsigned>(ceil_div(m, 4)), 256, 0, s>>>(bytes, m, k, codes, scale);
-    else quantize_int8_kernel<D, 256, 1, CAP><<<grid, 256, 0, s>>>(bytes, m, k, codes, scale);
+    // As many threads a row as hold it in two chunks each: fewer hold more each and have fewer rows in flight, more spend
+    // their time on the row's maximum. bf16, us: M = 4096, K 4096 with 64, 128, 256, 512 and 1024 threads 13.7, 12.3, 11.4,
+    // 12.2 and 16.3; K 12288 with 256, 512 and 1024 30.1, 29.5 and 27.4; M = 32768, K 1024 with 64, 128 and 256 20.1, 21.4
+    // and 29.9; M = 333, K 12288 with 256, 512 and 1024 5.5, 5.2 and 5.1. A wavefront's rows need no barrier: four of them
+    // a workgroup.
+    const int64_t chunks = k / 8;
+    if (chunks <= 64 * 2) quantize_int8_kernel<D, 64, 4, 2><<<static_cast<unsigned>(ceil_div(m, 4)), 256, 0, s>>>(bytes, m, k, codes, scale);
+    else if (chunks <= 128 * 2) quantize_int8_kernel<D, 128, 1, 2><<<grid, 128, 0, s>>>(bytes, m, k, codes, scale);
+    else if (chunks <= 256 * 2) quantize_int8_kernel<D, 256, 1, 2><<<grid, 256, 0, s>>>(bytes, m, k, codes, scale);
+    else if (chunks <= 512 * 2) quantize_int8_kernel<D, 512, 1, 2><<<grid, 512, 0, s>>>(bytes, m, k, codes, scale);
+    else if (chunks <= 1024 * 2) quantize_int8_kernel<D, 1024, 1, 2><<<grid, 1024, 0, s>>>(bytes, m, k, codes, scale);
+    else quantize_int8_kernel<D, 1024, 1, 4><<<grid, 1024, 0, s>>>(bytes, m, k, codes, scale);
 }
 
 // Items of N codes, 16 bytes of output (or one value, where rows are not whole items or not aligned): four a thread, a
