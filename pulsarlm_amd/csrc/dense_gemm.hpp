@@ -79,12 +79,13 @@ __device__ __forceinline__ expert_range find_experts(const int32_t* __restrict__
         if (lane == 0) lo = 0;
         const int count = lane < n ? hi - lo : -1;
         int place = 0;
+#pragma unroll 4
         for (int i = 0; i < n; ++i) {
             const int other = __builtin_amdgcn_readlane(count, i);
             place += other > count || (other == count && i < lane) ? 1 : 0;
         }
-        int e = 0;
-        for (int i = 0; i < n; ++i) e = __builtin_amdgcn_readlane(place, i) == slot ? i : e;
+        place = lane < n ? place : lane;
+        const int e = from_lane(__builtin_amdgcn_ds_permute(place * 4, lane), slot);  // the lane that goes to the place
         return {e, from_lane(lo, e), from_lane(hi, e)};
     }
     expert_range r{slot, 0, 0};

@@ -90,3 +90,16 @@ def test_the_same_bits_on_every_call():
         out = ops.grouped_gemm_cuda(x, w, off), ops.grouped_gemm_grad_x_cuda(dy, w, off), ops.grouped_gemm_grad_w_cuda(dy, x, off)
         first = first or out
         assert all(torch.equal(a, b) for a, b in zip(first, out))
+
+
+@pytest.mark.parametrize("kernel", [None, "t0", "t2", "t5"])
+@pytest.mark.parametrize("experts", [1, 2, 7, 8, 9, 31, 32, 33, 39, 40, 63, 64, 65, 127, 128, 129, 257])
+def test_weights_gradient_of_any_number_of_experts(experts, kernel, tuning_env):
+    """Their tiles are shared out by expert from some number on, and by their rows up to another."""
+    tuning_env("PLM_DENSE", kernel)
+    rng = random.Random(experts)
+    counts = [rng.choice([0, 1, 3, 70, 130]) for _ in range(experts)]
+    rows, n, k = sum(counts), 520, 264
+    dy, x = dense.values((rows + 5, n), torch.bfloat16, 1), dense.values((rows + 5, k), torch.bfloat16, 2)
+    dw = ops.grouped_gemm_grad_w_cuda(dy, x, dense.offsets(counts))
+    dense.within(dw, *dense.grad_w(dy[:rows], x[:rows], counts), kernel)
