@@ -23,16 +23,16 @@ constexpr double kTileEnds = 1.5, kLaunchEnds = 2.5;
 // rows, 256 rows 136 to 123, 512 rows 141 to 144.
 constexpr double kRaggedTiles = 1.1;
 // By ranges: both operands lie across the sum, sums of unequal length, of which the longest is taken as three times the
-// average.
+// average, or all there is.
 constexpr double kRangesStage = 1.13, kRangesEnds = 3.;
-double ranges_time(const tile_cost& c, double tiles, int64_t stages) {
+double ranges_time(const tile_cost& c, double tiles, int64_t stages, int64_t experts) {
     const double each = std::max(1., tiles / cu_count() / (c.two > 0. ? 2. : 1.)), all = c.two > 0. ? c.two : c.one_all;
-    return kRangesStage * std::max((each * (stages + kRangesEnds) + kLaunchEnds) * all, (3 * stages + kRangesEnds + kLaunchEnds) * c.one_all);
+    return kRangesStage * std::max((each * (stages + kRangesEnds) + kLaunchEnds) * all, (std::min<int64_t>(3, experts) * stages + kRangesEnds + kLaunchEnds) * c.one_all);
 }
-// Workgroups of the busiest CU; past a few, and where their number is a guess, the average and a half.
+// Workgroups of the busiest CU; where their number is a guess, the average and a half.
 double rounds_of(double tiles, bool guess) {
     const double each = tiles / cu_count();
-    return std::max(1., guess && each > 4. ? each + .5 : static_cast<double>(static_cast<int64_t>(each + .999)));
+    return std::max(1., guess && each > 1. ? each + .5 : static_cast<double>(static_cast<int64_t>(each + .999)));
 }
 double rounds_time(const tile_cost& c, double tiles, bool guess, int64_t stages) {
     const double each = rounds_of(tiles, guess), one = c.one_few + (c.one_all - c.one_few) * std::min(1., tiles / cu_count());
@@ -64,8 +64,9 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
     }
     const double used = mode == kByRows ? p.experts * (1. - std::exp(-static_cast<double>(p.rows) / p.experts)) : 1.;
     const double memory = kStart + (mode == kByRanges ? 1. * p.experts * p.rows * p.cols : used * p.cols * depth) * size / kMemoryRate;
+    const bool guess = mode == kByRows && p.experts > 1;
     auto blocks_of = [&](int64_t rows) {
-        if (mode != kByRows) return static_cast<double>(ceil_div(p.rows, rows));
+        if (!guess) return static_cast<double>(ceil_div(p.rows, rows));
         return used + std::max(0., static_cast<double>(p.rows) / rows - .5 * used);
     };
     // What takes longer hides most of the other.
@@ -80,8 +81,8 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
         for (int64_t splits = 1; splits <= most; ++splits) {
             const int64_t each = ceil_div(stages, splits);
             if (ceil_div(stages, each) != splits) continue;  // no part without a stage
-            double time = mode == kByRanges ? together(memory, ranges_time(c, tiles, stages))
-                                            : together(memory * (mode == kByRows ? kRaggedTiles : 1.), rounds_time(c, tiles * splits, mode == kByRows, each));
+            double time = mode == kByRanges ? together(memory, ranges_time(c, tiles, stages, p.experts))
+                                            : together(memory * (mode == kByRows ? kRaggedTiles : 1.), rounds_time(c, tiles * splits, guess, each));
             if (splits > 1) time += kCombine + splits * p.rows * p.cols * 8 / kPartRate;
             if (time < least) least = time, best = {i, static_cast<int>(splits), 0};
         }
@@ -93,7 +94,7 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
         const int64_t strips = dense_rows_strips(blocks, p.cols);
         const double groups = blocks_of(block) * ceil_div(p.cols, 16 * strips);
         const double rows = std::min<double>(block, p.rows / used);
-        const double time = together(memory, kStart + rounds_of(groups, mode == kByRows) * (16 * strips + rows) * depth * size / kRowsRate);
+        const double time = together(memory, kStart + rounds_of(groups, guess) * (16 * strips + rows) * depth * size / kRowsRate);
         if (time < least) least = time, best = {0, 1, block};
     }
     return best;
