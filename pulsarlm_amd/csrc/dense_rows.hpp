@@ -5,7 +5,10 @@
 // * A workgroup owns 16 MT rows by 16 NS columns. Its NW wavefronts take chunks of 64 U bytes of K in turn, each with the
 //   next chunk's loads in flight, and their sums meet in LDS in wavefront order: results do not depend on timing.
 // * QUANT: a few rows of 16-bit x, quantized by every workgroup for itself while its first weights are on their way: each
-//   reads the rows for their largest magnitudes, and keeps their codes in LDS. A launch less: N 6144, K 4096, one row.
+//   reads the rows for their largest magnitudes, and keeps their codes in LDS. A launch less: N 6144, K 4096, one row 10.2 us for
+//   12.4.
+// What bounds it: memory, 16 rows of 8 bits, N 4096, K 12288 13.1 us (50 MB); 64 rows over 128 experts in 16 bits, N 1536,
+// K 2048 53.6 us (284 MB). With more rows x: every workgroup reads them again, from the caches, at 33 GB/s a CU.
 #pragma once
 
 #include <algorithm>
