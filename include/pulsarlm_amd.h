@@ -339,7 +339,8 @@ int plm_mlp_mxfp4_w4a4(const void* x, plm_dtype x_dtype, const void* gate_weight
  * max(amax(x[m, :]), 1e-12) / 127 in fp32, codes[m, k] the integer nearest to x[m, k] / x_scale[m] (the exact quotient),
  * ties to even, so within [-127, 127]. A row with an infinity or NaN gets scale NaN and codes 0. x fp32, fp16 or bf16,
  * K at most 2^28, any alignment; M below 2^24. plm_dequantize_rows_int8 is the inverse: codes times scale in fp32, rounded to
- * out_dtype. The reference has no counterpart of these and the following entry points' formats.
+ * out_dtype. The reference has no counterpart of these and the following entry points' formats. Here and below outputs may not
+ * overlap inputs or the workspace.
  */
 int plm_quantize_rows_int8(const void* x, plm_dtype x_dtype, int64_t m, int64_t k, int8_t* codes, float* x_scale, void* stream);
 int plm_dequantize_rows_int8(const int8_t* codes, const float* x_scale, int64_t m, int64_t k, void* out, plm_dtype out_dtype,

@@ -12,8 +12,7 @@ namespace {
 
 bool sixteen(plm_dtype t) { return t == PLM_BF16 || t == PLM_FP16; }
 
-// These keep offsets of one workgroup below kOOB, and the grid of 256 x 256 tiles below 2^32 work-items: rows cols /
-// 2^16 of them are whole, and with experts, whose last ones can be parts, E cols / 2^8 more.
+// These keep offsets of one workgroup below kOOB, and the numbers of 64 x 64 tiles within 31 bits.
 bool takes_rows(int64_t rows, int64_t n, int64_t k) { return rows <= kDenseMaxRows && rows * std::max(n, k) <= (int64_t{1} << 36); }
 int check_sizes(const char* op, const char* m, int64_t rows, int64_t n, int64_t k) {
     PLM_CHECK_ARG(rows >= 0 && n >= 0 && k >= 0, op, "sizes must be non-negative");

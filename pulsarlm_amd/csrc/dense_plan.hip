@@ -13,11 +13,11 @@ namespace {
 // A tile shape's time is that of a stage, for each of its stages, one and a half a tile and two and a half a launch: `one`
 // with one workgroup a CU, from few of them to one on every CU; `two` for a pair on a CU, where two fit.
 struct tile_cost {
-    int rows, cols, threads;
+    int rows, cols;
     double one_few, one_all, two;
 };
-constexpr tile_cost kTileCosts[] = {{256, 256, 512, 1.28, 1.58, 0.}, {128, 256, 512, .88, .94, 0.}, {128, 128, 256, .62, .63, 0.},
-                                    {128, 128, 256, .87, .87, 1.06}, {64, 128, 256, .47, .50, .68}, {64, 64, 256, .31, .33, .52}};
+constexpr tile_cost kTileCosts[] = {{256, 256, 1.28, 1.58, 0.}, {128, 256, .88, .94, 0.}, {128, 128, .62, .63, 0.},
+                                    {128, 128, .87, .87, 1.06}, {64, 128, .47, .50, .68}, {64, 64, .31, .33, .52}};
 constexpr double kTileEnds = 1.5, kLaunchEnds = 2.5;
 // Experts' weights through tiles with few rows: E 128, N 1536, K 2048 in 16 bits, 64 rows 74 to 67 us of the kernel for few
 // rows, 256 rows 136 to 123, 512 rows 141 to 144.
@@ -75,7 +75,6 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
     for (int i = 0; i < 6; ++i) {
         const tile_cost& c = kTileCosts[i];
         const int64_t cols = ceil_div(p.cols, c.cols), experts = mode == kByRanges ? p.experts : 1;
-        if (i > 0 && !dense_grid_fits(dense_row_blocks(p, mode, c.rows) * cols * experts, c.threads)) continue;
         const double tiles = blocks_of(c.rows) * cols * experts;
         const int64_t most = may_split ? std::max<int64_t>(1, std::min<int64_t>({16, stages / 4, static_cast<int64_t>(2 * cus / tiles)})) : 1;
         for (int64_t splits = 1; splits <= most; ++splits) {

@@ -123,11 +123,11 @@ template <plm_dtype D> void launch_quantize(const void* x, int64_t m, int64_t k,
     // their time on the row's maximum. bf16, us: M = 4096, K 4096 with 64, 128, 256, 512 and 1024 threads 13.7, 12.3, 11.4,
     // 12.2 and 16.3; K 12288 with 256, 512 and 1024 30.1, 29.5 and 27.4; M = 32768, K 1024 with 64, 128 and 256 20.1, 21.4
     // and 29.9; M = 333, K 12288 with 256, 512 and 1024 5.5, 5.2 and 5.1. A wavefront's rows need no barrier: four of them
-    // a workgroup.
+    // a workgroup. More rows than a grid of such workgroups has: 256 threads each, which read the rest of a row twice.
     const int64_t chunks = k / 8;
     if (chunks <= 64 * 2) quantize_int8_kernel<D, 64, 4, 2><<<static_cast<unsigned>(ceil_div(m, 4)), 256, 0, s>>>(bytes, m, k, codes, scale);
     else if (chunks <= 128 * 2) quantize_int8_kernel<D, 128, 1, 2><<<grid, 128, 0, s>>>(bytes, m, k, codes, scale);
-    else if (chunks <= 256 * 2) quantize_int8_kernel<D, 256, 1, 2><<<grid, 256, 0, s>>>(bytes, m, k, codes, scale);
+    else if (chunks <= 256 * 2 || !dense_grid_fits(m, 1024)) quantize_int8_kernel<D, 256, 1, 2><<<grid, 256, 0, s>>>(bytes, m, k, codes, scale);
     else if (chunks <= 512 * 2) quantize_int8_kernel<D, 512, 1, 2><<<grid, 512, 0, s>>>(bytes, m, k, codes, scale);
     else if (chunks <= 1024 * 2) quantize_int8_kernel<D, 1024, 1, 2><<<grid, 1024, 0, s>>>(bytes, m, k, codes, scale);
     else quantize_int8_kernel<D, 1024, 1, 4><<<grid, 1024, 0, s>>>(bytes, m, k, codes, scale);

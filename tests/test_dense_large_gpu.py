@@ -36,6 +36,21 @@ def test_quantizer():
     assert torch.equal(back[at].cpu(), (q.float() * s[:, None]).bfloat16())
 
 
+def test_quantizer_of_more_rows_than_a_grid_of_wide_workgroups():
+    m, k = (1 << 22) + 3, 8200  # 69 GB
+    x = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1 << 21, (1 << 22) - 1, 1 << 22, m - 1], device="cuda")
+    x[at] = device_values((5, k), 1)
+    codes, scale = ops.quantize_rows_int8_cuda(x)
+    q, s = dense.quantize(x[at])
+    assert torch.equal(codes[at].cpu(), q) and torch.equal(scale[at].cpu(), s)
+    others = torch.ones(m, dtype=torch.bool, device="cuda")
+    others[at] = False
+    assert (scale[others] == dense.row_scale(torch.zeros(1, 8))[0].item()).all()
+    used = torch.cat([part.view(torch.int64).any(dim=1) for part in codes.split(1 << 19)])
+    assert torch.equal(used.nonzero()[:, 0], at)
+
+
 def test_rows():
     m, n, k = 140001, 16400, 64  # 2.3e9 outputs
     q, xs, w, ws = device_codes((m, k), 1), dense.scales(m, 2), device_codes((n, k), 3), dense.scales(n, 4)
