@@ -216,3 +216,39 @@ def test_same_bits_on_every_call():
         out = ops.grouped_gemm_cuda(x, w, off), ops.grouped_gemm_grad_x_cuda(dy, w, off), ops.grouped_gemm_grad_w_cuda(dy, x, off)
         first = first or out
         assert all(torch.equal(a, b) for a, b in zip(first, out))
+
+
+def test_on_two_streams_at_once():
+    """Calls on other streams than the tensors' own, each with scratch of its own."""
+    counts, n, k = [60, 0, 211, 5], 264, 144
+    x, w, dy, off = inputs(counts, n, k, torch.bfloat16)
+    w8, ws = dense.codes(4 * n, k, 2).view(4, n, k), dense.scales(4 * n, 3).view(4, n)
+
+    def step():
+        return (ops.grouped_gemm_cuda(x, w, off), ops.grouped_gemm_grad_x_cuda(dy, w, off), ops.grouped_gemm_grad_w_cuda(dy, x, off),
+                ops.grouped_gemm_int8_cuda(x, w8, ws, off))
+
+    want = step()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(10):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+def test_a_weight_shared_by_every_expert():
+    """A broadcast weight: refused as it is, and its gradient the sum of the copies'."""
+    counts, n, k = [7, 30, 0, 63], 40, 64
+    x, _, dy, off = inputs(counts, n, k, torch.bfloat16)
+    one = dense.values((1, n, k), torch.float32, 5).requires_grad_()
+    with pytest.raises(RuntimeError, match="weight must be contiguous"):
+        ops.grouped_gemm_cuda(x, one.detach().bfloat16().expand(4, n, k), off)
+    y = ops.grouped_gemm_cuda(x, one.bfloat16().expand(4, n, k).contiguous(), off)
+    y.backward(dy)
+    ref = dy.double().t() @ x.double()
+    # Each expert's sum rounded to bf16, then three additions of them, rounded as well: six half steps of what they add up to.
+    bound = dense.sums(100) * (dy.double().abs().t() @ x.double().abs())
+    parts = sum((dy[lo:hi].double().t() @ x[lo:hi].double()).abs() for _, lo, hi in dense.by_expert(counts))
+    assert ((one.grad[0].double() - ref).abs() <= bound + 6 * 2.0**-8 * (parts + bound)).all()

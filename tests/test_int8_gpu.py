@@ -188,6 +188,16 @@ def test_w8a8(m, n, k, dtype):
     dense.within(y, *dense.int8_product(q.cuda(), xs.cuda(), w, ws))
 
 
+@pytest.mark.parametrize("m,k", [(1, 16), (1, 65536), (1, 65552), (2, 32768), (2, 32784), (3, 2720), (3, 2736), (4, 2048), (4, 2064), (5, 1024)])
+def test_w8a8_where_the_product_quantizes_and_where_not(m, k):
+    x, w, ws = dense.values((m, k), torch.bfloat16, 1), dense.codes(72, k, 2), dense.scales(72, 3)
+    x[-1] = 0
+    q, xs = ops.quantize_rows_int8_cuda(x)
+    y = ops.gemm_int8_w8a8_cuda(x, w, ws)
+    dense.within(y, *dense.int8_product(q, xs, w, ws))
+    assert not y[-1].any()
+
+
 @pytest.mark.parametrize("m", [3, 100])
 def test_w8a8_keeps_rows_apart(m):
     """A row that is not finite is NaN, the others do not change."""
