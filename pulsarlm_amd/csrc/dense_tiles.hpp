@@ -21,6 +21,7 @@
 #include <utility>
 
 #include "dense_gemm.hpp"
+#include "dense_turns.hpp"
 
 namespace plm {
 
@@ -82,9 +83,7 @@ __global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) 
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN, col16 = lane & 15, kq = lane >> 4;
 
-    // The workgroup's tiles, one a lane: every gridDim.x-th of the launch's. Workgroups go round the 8 XCDs by id: each
-    // takes one run of the tiles, which are ordered in bands of `band` row blocks, row block fastest, so that an XCD's L2
-    // holds what its tiles share.
+    // The workgroup's tiles, one a lane: every gridDim.x-th of the launch's (dense_turns.hpp).
     constexpr int SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : BM == 64 ? 6 : 5;
     static_assert(1 << SHIFT == BM, "row blocks are powers of two");
     int m_blocks = a.m_blocks;
@@ -92,18 +91,14 @@ __global__ void __launch_bounds__(WM * WN * 64) dense_tile_kernel(dense_args a) 
     // (By ranges, of an expert's tiles: experts can differ in depth by far.)
     const int block_tiles = m_blocks * a.n_blocks, all_tiles = block_tiles * (MODE == kByRanges ? a.experts : 1);
     const int each = static_cast<int>(gridDim.x), self = static_cast<int>(blockIdx.x);
-    // The workgroup's place in turn i of all of them: by ranges, whose longest sums come first, back and forth.
-    auto place = [&](int i) { return MODE == kByRanges && (i & 1) ? each - 8 - (self & ~7) + (self & 7) : self; };
-    const int turns = all_tiles / each, tiles = turns + (all_tiles - turns * each > place(turns) ? 1 : 0);  // <= 64
+    // By ranges, whose longest sums come first, the turns go back and forth.
+    const int tiles = dense_turns(all_tiles, each, self, MODE == kByRanges);  // <= 64
     if (tiles == 0) return;
     int lane_expert = 0, lane_row0, lane_col0, lane_lo, lane_hi;  // rows of the output (by ranges, of the sum): lo .. hi
     {
-        int id = min(lane * each + place(lane), all_tiles - 1);
+        int id = min(lane * each + dense_place(lane, each, self, MODE == kByRanges), all_tiles - 1);
         if constexpr (MODE == kByRanges) lane_expert = id / block_tiles, id -= lane_expert * block_tiles;
-        const int xcd = id & 7, lin = xcd * (block_tiles >> 3) + min(xcd, block_tiles & 7) + (id >> 3);
-        const int band0 = lin / (a.band * a.n_blocks) * a.band;
-        const int band_rows = min(a.band, m_blocks - band0), in_band = lin - band0 * a.n_blocks;
-        const int nb = in_band / band_rows, mb = band0 + in_band - nb * band_rows;
+        const auto [mb, nb] = dense_block_of(id, m_blocks, a.n_blocks, a.band);
         lane_col0 = nb * BN, lane_row0 = lane_lo = mb * BM, lane_hi = min(lane_lo + BM, a.rows);
         if constexpr (MODE == kByRows) {
             const expert_range r = find_blocks(a.offsets, a.experts, a.rows, a.zero_rest, SHIFT, mb);
@@ -411,10 +406,10 @@ void launch_tile(const dense_product& p, hipStream_t s) {
     a.n_blocks = static_cast<int>(ceil_div(p.cols, BN));
     a.m_blocks = static_cast<int>(dense_row_blocks(p, MODE, BM));
     const int64_t tiles = int64_t{1} * a.m_blocks * a.n_blocks * (MODE == kByRanges ? p.experts : 1);
-    // As many workgroups as are resident at once, in whole rounds of the XCDs; a workgroup keeps count of up to 64 tiles.
+    // As many workgroups as are resident at once, which is in whole rounds of the XCDs, or as there are tiles.
     constexpr int LDS = 128 * ((S + PX) * BM + S * BN);
     const int64_t resident = ceil_div(int64_t{cu_count()} * (2 * LDS <= 160 * 1024 ? 2 : 1), 8) * 8;
-    dim3 grid(static_cast<unsigned>(std::min(tiles, std::max(resident, ceil_div(tiles, 512) * 8))));
+    dim3 grid(static_cast<unsigned>(dense_grid(tiles, resident, MODE == kByRanges)));
     if (T == kInt8 && MODE == kDense && p.plan.splits > 1) {
         grid.y = static_cast<unsigned>(p.plan.splits);
         a.split_stages = static_cast<int>(ceil_div(ceil_div(p.depth, 128), p.plan.splits));
