@@ -603,7 +603,8 @@ struct grouped_linear : torch::autograd::Function<grouped_linear> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list dy) {
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor d = dy[0].contiguous();
+        at::Tensor d = dy[0].contiguous();
+        if (reinterpret_cast<uintptr_t>(d.data_ptr()) % 16 != 0) d = d.clone();  // a part of a longer gradient (at::cat's), from any element on
         return {ctx->needs_input_grad(0) ? grouped_gemm_grad_x_cuda(d, saved[1], saved[2]) : at::Tensor(),
                 ctx->needs_input_grad(1) ? grouped_gemm_grad_w_cuda(d, saved[0], saved[2]) : at::Tensor(), {}};
     }

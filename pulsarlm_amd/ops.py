@@ -788,6 +788,8 @@ class _Grouped(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, offsets = ctx.saved_tensors
         dy = dy.contiguous()
+        if dy.data_ptr() % 16 != 0:  # a part of a longer gradient (torch.cat's), from any element on
+            dy = dy.clone()
         dx = grouped_gemm_grad_x_cuda(dy, weight, offsets) if ctx.needs_input_grad[0] else None
         dw = grouped_gemm_grad_w_cuda(dy, x, offsets) if ctx.needs_input_grad[1] else None
         return dx, dw, None
