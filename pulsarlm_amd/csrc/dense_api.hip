@@ -54,12 +54,13 @@ dense_product product(dense_type type, const void* p, const void* q, void* y, bo
     return d;
 }
 // The dense 8-bit product, and the workspace of a split sum's parts.
-int64_t partial_bytes(int64_t m, int64_t n, int64_t k) {
-    const dense_product p = product(kInt8, nullptr, nullptr, nullptr, true, m, n, k);
+int64_t partial_bytes(int64_t m, int64_t n, int64_t k, bool to_quantize = false) {
+    dense_product p = product(kInt8, nullptr, nullptr, nullptr, true, m, n, k);
+    p.to_quantize = to_quantize;
     return dense_partial_bytes(plan_dense(p, kDense, true, true), m, n);
 }
+// p.plan is set.
 void run_int8(dense_product p, void* partial, hipStream_t s) {
-    p.plan = plan_dense(p, kDense, true, true);
     if (p.plan.rows_block > 0) return launch_dense_rows(p, kDense, s);
     p.partial = static_cast<i32x4_t*>(partial);
     launch_tiles_int8(p, kDense, s);
@@ -87,6 +88,11 @@ int check_workspace(const char* op, const void* workspace, size_t have, int64_t 
     }
     PLM_CHECK_ARG(aligned(workspace, 256), op, "workspace must be 256-byte aligned");
     return PLM_OK;
+}
+
+// W8A8: that, and the parts of a sum, whose plan goes by x's alignment.
+int64_t w8a8_bytes(int64_t m, int64_t n, int64_t k) {
+    return tokens_bytes(m, k) + std::max(partial_bytes(m, n, k, true), partial_bytes(m, n, k, false));
 }
 
 }  // namespace
@@ -144,13 +150,14 @@ int plm_gemm_int8(const int8_t* codes, const float* x_scale, const int8_t* weigh
     if (int rc = check_workspace(op, workspace, workspace_bytes, partial_bytes(m, n, k))) return rc;
     dense_product p = product(kInt8, codes, weight, y, y_dtype == PLM_BF16, m, n, k);
     p.p_scale = x_scale, p.q_scale = scale;
+    p.plan = plan_dense(p, kDense, true, true);
     run_int8(p, workspace, s);
     PLM_HIP_LAUNCH_CHECK(op);
     return PLM_OK;
 }
 
 int64_t plm_gemm_int8_w8a8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return counts(m, n, k) ? tokens_bytes(m, k) + partial_bytes(m, n, k) : 0;
+    return counts(m, n, k) ? w8a8_bytes(m, n, k) : 0;
 }
 
 int plm_gemm_int8_w8a8(const void* x, plm_dtype x_dtype, const int8_t* weight, const float* scale, int64_t m, int64_t n, int64_t k, void* y,
@@ -167,11 +174,11 @@ int plm_gemm_int8_w8a8(const void* x, plm_dtype x_dtype, const int8_t* weight, c
     if (int rc = check_pointer(op, "x", x, 2)) return rc;
     if (int rc = check_pointer(op, "weight", weight, 16)) return rc;
     if (int rc = check_pointer(op, "scale", scale, 4)) return rc;
-    if (int rc = check_workspace(op, workspace, workspace_bytes, tokens_bytes(m, k) + partial_bytes(m, n, k))) return rc;
+    if (int rc = check_workspace(op, workspace, workspace_bytes, w8a8_bytes(m, n, k))) return rc;
     dense_product p = product(kInt8, x, weight, y, x_dtype == PLM_BF16, m, n, k);
-    p.q_scale = scale;
+    p.q_scale = scale, p.to_quantize = aligned(x, 16);
     p.plan = plan_dense(p, kDense, true, true);
-    if (dense_rows_quantizes(p)) {
+    if (dense_rows_quantizes(p, p.plan.rows_block)) {
         launch_dense_rows_quantize(p, s);
         PLM_HIP_LAUNCH_CHECK(op);
         return PLM_OK;

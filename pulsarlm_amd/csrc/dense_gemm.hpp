@@ -219,6 +219,7 @@ struct dense_product {
     int64_t experts;
     dense_type type;
     bool bf16, zero_rest;
+    bool to_quantize;  // dense 8-bit: p is 16 bits and 16-byte aligned, quantized by the kernel for few rows or before
     dense_plan plan;
     i32x4_t* partial;
 };
@@ -269,8 +270,8 @@ void launch_tiles_grad_w(const dense_product& p, hipStream_t s);
 void launch_combine_int8(const dense_product& p, hipStream_t s);
 // The kernel for few rows, forward.
 void launch_dense_rows(const dense_product& p, dense_mode mode, hipStream_t s);
-// The same on 16-bit x [rows][depth] (p.p), quantized in the kernel, for dense 8-bit products that it takes.
-bool dense_rows_quantizes(const dense_product& p);
+// The same on 16-bit x [rows][depth] (p.p, 16-byte aligned), quantized in the kernel, for dense 8-bit products that it takes.
+bool dense_rows_quantizes(const dense_product& p, int rows_block);
 void launch_dense_rows_quantize(const dense_product& p, hipStream_t s);
 
 // Rows of codes and their scales.

@@ -42,6 +42,10 @@ double rounds_time(const tile_cost& c, double tiles, bool guess, int64_t stages)
 // The kernel for few rows: a CU takes in 33 GB/s of its workgroups' x and weights (64 bytes of a row a request), all of
 // them 5.2 TB/s of weights.
 constexpr double kStart = 3.3, kRowsRate = 33e3, kMemoryRate = 5.2e6;
+// The launch that quantizes 16-bit rows, where the product does not; and where it does, a value a thread past the 32 that wait
+// in registers, which is read again. M 1: N 1024, K 1024 4.3 us in the kernel for few rows and 7.5 through tiles, N 12288, K 16384 57
+// and 52; M 2: N 4096, K 512 4.5 and 7.0, N 24576, K 12288 74 and 82, K 16384 99 and 89.
+constexpr double kQuantizer = 2.2, kReadAgain = .06;
 // A split sum's parts: a kernel more, and their way through memory and back.
 constexpr double kCombine = 4.0, kPartRate = 4.5e6;
 
@@ -83,6 +87,7 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
             double time = mode == kByRanges ? together(memory, ranges_time(c, tiles, stages, p.experts))
                                             : together(memory * (mode == kByRows ? kRaggedTiles : 1.), rounds_time(c, tiles * splits, guess, each));
             if (splits > 1) time += kCombine + splits * p.rows * p.cols * 8 / kPartRate;
+            if (p.to_quantize) time += kQuantizer;
             if (time < least) least = time, best = {i, static_cast<int>(splits), 0};
         }
     }
@@ -93,7 +98,11 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
         const int64_t strips = dense_rows_strips(blocks, p.cols);
         const double groups = blocks_of(block) * ceil_div(p.cols, 16 * strips);
         const double rows = std::min<double>(block, p.rows / used);
-        const double time = together(memory, kStart + rounds_of(groups, guess) * (16 * strips + rows) * depth * size / kRowsRate);
+        double time = together(memory, kStart + rounds_of(groups, guess) * (16 * strips + rows) * depth * size / kRowsRate);
+        if (p.to_quantize) {
+            const double values = static_cast<double>(p.rows) * p.depth / (strips == 2 ? 256 : 512);  // a thread's
+            time += dense_rows_quantizes(p, block) ? kReadAgain * std::max(0., values - 32) : kQuantizer;
+        }
         if (time < least) least = time, best = {0, 1, block};
     }
     return best;
@@ -103,7 +112,7 @@ dense_plan make_plan(const dense_product& p, dense_mode mode, bool rows_kernel, 
 
 dense_plan plan_dense(const dense_product& p, dense_mode mode, bool rows_kernel, bool may_split) {
     static thread_local plan_cache<dense_plan> cache;
-    const int kind = mode * 8 + (p.type == kInt8 ? 4 : 0) + (rows_kernel ? 2 : 0) + (may_split ? 1 : 0);
+    const int kind = mode * 16 + (p.to_quantize ? 8 : 0) + (p.type == kInt8 ? 4 : 0) + (rows_kernel ? 2 : 0) + (may_split ? 1 : 0);
     return cache.get(kind, p.rows, p.cols, p.depth, p.experts, [&] { return make_plan(p, mode, rows_kernel, may_split); });
 }
 

@@ -21,9 +21,9 @@ template <dense_type T, dense_mode MODE> void launch_blocks(const dense_product&
 // 16-bit x of a dense 8-bit product quantized in the kernel, by every workgroup for itself. Against a launch more, us: one
 // row of N 6144, K 4096 10.2 and 12.4, two 12.2 and 12.4; N 4096, K 12288 one 13.2 and 15.3, four 19.2 and 15.3; N 1000,
 // K 2048 four 4.9 and 6.5.
-bool dense_rows_quantizes(const dense_product& p) {
+bool dense_rows_quantizes(const dense_product& p, int rows_block) {
     const int64_t bytes = p.rows * p.depth;
-    return p.plan.rows_block == 16 && p.rows <= kQuantRows && bytes <= (p.rows <= 2 ? kQuantBytes : 8192) && aligned(p.p, 16);
+    return p.to_quantize && rows_block == 16 && p.rows <= kQuantRows && bytes <= (p.rows <= 2 ? kQuantBytes : 8192);
 }
 void launch_dense_rows_quantize(const dense_product& p, hipStream_t s) {
     if (dense_rows_strips(1, p.cols) == 2) launch_rows<kInt8, kDense, 1, 2, 4, 4, true>(p, s);
