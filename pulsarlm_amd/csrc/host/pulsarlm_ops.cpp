@@ -267,8 +267,53 @@ std::tuple<at::Tensor, at::Tensor> routed_experts_int4_cuda(const at::Tensor& h,
     return {out, offsets};
 }
 
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool mx_records(const at::Tensor& x) { return x.requires_grad() && at::GradMode::is_enabled(); }
+
+// call(): an output in the graph of its two inputs (or one, twice) whose gradient is asked for in vain, and says so then.
+struct mx_no_gradient : torch::autograd::Function<mx_no_gradient> {
+    static at::Tensor forward(AutogradContext* ctx, const char* op, const std::function<at::Tensor()>& call, const at::Tensor&,
+                              const at::Tensor&) {
+        ctx->saved_data["op"] = std::string(op);
+        return call();
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list&) {
+        TORCH_CHECK(false, ctx->saved_data["op"].toStringRef(), ": has no gradient");
+    }
+};
+
+// As mx_no_gradient, for two outputs, of which whole numbers are in no graph.
+struct no_gradient_pair : torch::autograd::Function<no_gradient_pair> {
+    static variable_list forward(AutogradContext* ctx, const char* op, const std::function<variable_list()>& call, const at::Tensor&) {
+        ctx->saved_data["op"] = std::string(op);
+        variable_list out = call();
+        for (const at::Tensor& t : out)
+            if (!t.is_floating_point()) ctx->mark_non_differentiable({t});
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list&) {
+        TORCH_CHECK(false, ctx->saved_data["op"].toStringRef(), ": has no gradient");
+    }
+};
+
+}  // namespace
+
 std::tuple<at::Tensor, at::Tensor> route_top_k_cuda(const at::Tensor& logits, int64_t k) {
     const char* op = "route_top_k";
+    if (mx_records(logits)) {
+        const variable_list out = no_gradient_pair::apply(
+            op,
+            [&] {
+                auto [weights, chosen] = route_top_k_cuda(logits, k);
+                return variable_list{weights, chosen};
+            },
+            logits);
+        return {out[0], out[1]};
+    }
     TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, op,
                 ": logits must be CUDA [tokens, experts], each row contiguous");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
@@ -283,6 +328,7 @@ std::tuple<at::Tensor, at::Tensor> route_top_k_cuda(const at::Tensor& logits, in
 
 at::Tensor silu_mul_cuda(const at::Tensor& x) {
     const char* op = "silu_mul";
+    if (mx_records(x)) return mx_no_gradient::apply(op, [&] { return silu_mul_cuda(x); }, x, x);
     TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous() && x.size(1) % 2 == 0, op,
                 ": x must be contiguous CUDA [tokens, 2 * n]");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
@@ -364,11 +410,6 @@ at::Tensor mx_scratch(const at::Tensor& x, int64_t bytes) {
 }
 size_t mx_bytes(const at::Tensor& t) { return t.defined() ? static_cast<size_t>(t.numel()) : 0; }
 
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-bool mx_records(const at::Tensor& x) { return x.requires_grad() && at::GradMode::is_enabled(); }
-
 struct mx_linear : torch::autograd::Function<mx_linear> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& scale, int64_t n) {
         at::Tensor y = gemm_mxfp4_cuda(x, weight, scale, n);
@@ -396,18 +437,6 @@ struct mx_gated : torch::autograd::Function<mx_gated> {
         if (!dh[0].defined()) return variable_list(6);
         const variable_list w = ctx->get_saved_variables();
         return {gated_mxfp4_grad_cuda(dh[0].contiguous(), w[0], w[1], w[2], w[3], w[4], ctx->saved_data["k"].toInt()), {}, {}, {}, {}, {}};
-    }
-};
-
-// call(): an output in the graph of its two inputs (or one, twice) whose gradient is asked for in vain, and says so then.
-struct mx_no_gradient : torch::autograd::Function<mx_no_gradient> {
-    static at::Tensor forward(AutogradContext* ctx, const char* op, const std::function<at::Tensor()>& call, const at::Tensor&,
-                              const at::Tensor&) {
-        ctx->saved_data["op"] = std::string(op);
-        return call();
-    }
-    static variable_list backward(AutogradContext* ctx, const variable_list&) {
-        TORCH_CHECK(false, ctx->saved_data["op"].toStringRef(), ": has no gradient");
     }
 };
 
@@ -561,19 +590,6 @@ namespace {
 bool any_records(std::initializer_list<at::Tensor> inputs) {
     return std::any_of(inputs.begin(), inputs.end(), [](const at::Tensor& t) { return mx_records(t); });
 }
-
-// As mx_no_gradient, for the quantizer's two outputs.
-struct no_gradient_pair : torch::autograd::Function<no_gradient_pair> {
-    static variable_list forward(AutogradContext* ctx, const char* op, const std::function<variable_list()>& call, const at::Tensor&) {
-        ctx->saved_data["op"] = std::string(op);
-        variable_list out = call();
-        ctx->mark_non_differentiable({out[0]});  // integers
-        return out;
-    }
-    static variable_list backward(AutogradContext* ctx, const variable_list&) {
-        TORCH_CHECK(false, ctx->saved_data["op"].toStringRef(), ": has no gradient");
-    }
-};
 
 void int8_rows(const char* op, const char* name, const at::Tensor& codes, const at::Tensor& scale, int64_t dim) {
     TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kChar && codes.dim() == dim && codes.is_contiguous(), op, ": ", name,

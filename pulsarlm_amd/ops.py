@@ -314,8 +314,11 @@ def routed_experts_int4_cuda(h: torch.Tensor, top_experts: torch.Tensor, top_wei
 def route_top_k_cuda(logits: torch.Tensor, k: int, experts_i32: bool = False):
     """route_top_k_cuda (ops.hpp:37-40): (weights fp32 [T, k], experts int64 [T, k]) for
     logits [T, E] whose rows may lie apart (unit column stride); experts_i32 gives int32
-    experts (what routed_experts_int4_cuda / plm_moe take) instead."""
+    experts (what routed_experts_int4_cuda / plm_moe take) instead. Has no gradient: a backward pass that reaches the
+    weights raises."""
     op = "route_top_k"
+    if _records(logits):
+        return _MxNoGradient.apply(op, lambda: route_top_k_cuda(logits, k, experts_i32), logits)
     _require(logits.is_cuda and logits.dim() == 2 and logits.stride(1) == 1, op,
              "logits must be CUDA [tokens, experts], each row contiguous")
     _require(logits.dtype in _DTYPES, op, "logits must be fp32, fp16 or bf16")
@@ -330,8 +333,11 @@ def route_top_k_cuda(logits: torch.Tensor, k: int, experts_i32: bool = False):
 
 
 def silu_mul_cuda(x: torch.Tensor) -> torch.Tensor:
-    """silu_mul_cuda (ops.hpp:42-43): silu(x[:, :n]) * x[:, n:], silu rounded to the dtype."""
+    """silu_mul_cuda (ops.hpp:42-43): silu(x[:, :n]) * x[:, n:], silu rounded to the dtype. Has no
+    gradient: a backward pass that reaches it raises."""
     op = "silu_mul"
+    if _records(x):
+        return _MxNoGradient.apply(op, lambda: silu_mul_cuda(x), x)
     _require(x.is_cuda and x.dim() == 2 and x.is_contiguous() and x.size(1) % 2 == 0, op,
              "x must be contiguous CUDA [tokens, 2 * n]")
     _require(x.dtype in _DTYPES, op, "x must be fp32, fp16 or bf16")
