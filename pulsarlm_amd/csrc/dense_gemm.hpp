@@ -79,7 +79,6 @@ __device__ __forceinline__ expert_range find_experts(const int32_t* __restrict__
         if (lane == 0) lo = 0;
         const int count = lane < n ? hi - lo : -1;
         int place = 0;
-#pragma unroll 4
         for (int i = 0; i < n; ++i) {
             const int other = __builtin_amdgcn_readlane(count, i);
             place += other > count || (other == count && i < lane) ? 1 : 0;

@@ -29,7 +29,8 @@ namespace {
 
 // 16 bytes a lane from memory straight to LDS, as buffer_load_lds16, but written out: the compiler would wait for every
 // such load in flight before a transposing LDS read, as it cannot tell their addresses apart. No register is written;
-// the kernel counts these loads itself. `lds` and `soffset` are wave-uniform.
+// the kernel counts these loads itself. `lds` and `soffset` are wave-uniform. m0 is these loads' own: the compiler takes no
+// clobber of a reserved register, so nothing else in the kernel may use it (a builtin that loads to LDS, indexed registers).
 __device__ __forceinline__ void dma16(i32x4_t buffer, uint32_t lds, int lds_more, int voffset, int soffset) {
     asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds" ::"s"(lds), "i"(lds_more), "v"(voffset), "s"(buffer), "s"(soffset) : "memory", "scc");
 }
