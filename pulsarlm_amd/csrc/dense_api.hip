@@ -90,11 +90,6 @@ int check_workspace(const char* op, const void* workspace, size_t have, int64_t 
     return PLM_OK;
 }
 
-// W8A8: that, and the parts of a sum, whose plan goes by x's alignment.
-int64_t w8a8_bytes(int64_t m, int64_t n, int64_t k) {
-    return tokens_bytes(m, k) + std::max(partial_bytes(m, n, k, true), partial_bytes(m, n, k, false));
-}
-
 }  // namespace
 }  // namespace plm
 
@@ -157,7 +152,8 @@ int plm_gemm_int8(const int8_t* codes, const float* x_scale, const int8_t* weigh
 }
 
 int64_t plm_gemm_int8_w8a8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return counts(m, n, k) ? w8a8_bytes(m, n, k) : 0;
+    // Of both plans, one for x that is 16-byte aligned and one for x that is not.
+    return counts(m, n, k) ? tokens_bytes(m, k) + std::max(partial_bytes(m, n, k, true), partial_bytes(m, n, k)) : 0;
 }
 
 int plm_gemm_int8_w8a8(const void* x, plm_dtype x_dtype, const int8_t* weight, const float* scale, int64_t m, int64_t n, int64_t k, void* y,
@@ -174,10 +170,10 @@ int plm_gemm_int8_w8a8(const void* x, plm_dtype x_dtype, const int8_t* weight, c
     if (int rc = check_pointer(op, "x", x, 2)) return rc;
     if (int rc = check_pointer(op, "weight", weight, 16)) return rc;
     if (int rc = check_pointer(op, "scale", scale, 4)) return rc;
-    if (int rc = check_workspace(op, workspace, workspace_bytes, w8a8_bytes(m, n, k))) return rc;
     dense_product p = product(kInt8, x, weight, y, x_dtype == PLM_BF16, m, n, k);
     p.q_scale = scale, p.to_quantize = aligned(x, 16);
     p.plan = plan_dense(p, kDense, true, true);
+    if (int rc = check_workspace(op, workspace, workspace_bytes, tokens_bytes(m, k) + dense_partial_bytes(p.plan, m, n))) return rc;
     if (dense_rows_quantizes(p, p.plan.rows_block)) {
         launch_dense_rows_quantize(p, s);
         PLM_HIP_LAUNCH_CHECK(op);

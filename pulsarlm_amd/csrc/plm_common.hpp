@@ -482,7 +482,7 @@ template <typename P> struct plan_cache {
     template <typename Fn> const P& get(int kind, int64_t m, int64_t n, int64_t k, int64_t limit, Fn make) {
         const uint64_t h = (static_cast<uint64_t>(m) * 0x9E3779B97F4A7C15u) ^ (static_cast<uint64_t>(n) * 0xC2B2AE3D27D4EB4Fu) ^
                            (static_cast<uint64_t>(k) * 0x165667B19E3779F9u) ^ (static_cast<uint64_t>(limit) * 0x27D4EB2F165667C5u) ^
-                           static_cast<uint64_t>(kind);
+                           (static_cast<uint64_t>(kind) * 0x85EBCA77C2B2AE63u);
         entry& e = entries[(h ^ (h >> 29)) >> 7 & 63];
         const unsigned epoch = knobs().epoch;
         if (e.m != m || e.n != n || e.k != k || e.limit != limit || e.kind != kind || e.epoch != epoch) {
