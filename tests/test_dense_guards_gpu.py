@@ -1,5 +1,5 @@
-"""The grouped products write their outputs and nothing beside them: each output inside a larger buffer of a known value,
-from one tile in all on."""
+"""The products and the quantizer write their outputs and nothing beside them: each output inside a larger buffer of a known
+value, from one tile in all on, and a workspace of the size that the query names inside one, too."""
 
 import pytest
 import torch
@@ -23,6 +23,15 @@ def guarded(shape, call):
     _lib.check(call(room.data_ptr() + 64 * size * 2))
     assert (room[: 64 * size] == GUARD).all() and (room[65 * size :] == GUARD).all()
     return room[64 * size : 65 * size].view(shape)
+
+
+def guarded_bytes(size, call):
+    """call(pointer) on `size` bytes, 256-byte aligned, between two times 4 KiB; those bytes."""
+    room = torch.full((size + 8192 + 256,), 0x5A, dtype=torch.uint8, device="cuda")
+    at = 4096 + -(room.data_ptr() + 4096) % 256
+    _lib.check(call(room.data_ptr() + at))
+    assert (room[:at] == 0x5A).all() and (room[at + size :] == 0x5A).all()
+    return room[at : at + size]
 
 
 def sizes(experts):
@@ -65,3 +74,41 @@ def test_products(experts, kernel, tuning_env):
         q, xs = (t.cuda() for t in dense.quantize(x))
         for e, lo, hi in dense.by_expert(counts):
             dense.within(y[lo:hi], *dense.int8_product(q[lo:hi], xs[lo:hi], w8[e], ws[e]), f"8 bits {n} {k}, expert {e}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 16), (3, 7), (5, 1024), (2, 8200), (7, 20000), (130, 72)])
+def test_quantizer(m, k, dtype):
+    lib, x = _lib.load(), dense.values((m, k), dense.DT[dtype], 1)
+    kind, q, s = {"bf16": _lib.PLM_BF16, "fp32": _lib.PLM_FP32}[dtype], *dense.quantize(x)
+    scale = torch.empty(m, device="cuda")
+    codes = guarded_bytes(m * k, lambda to: lib.plm_quantize_rows_int8(x.data_ptr(), kind, m, k, to, scale.data_ptr(), stream()))
+    assert torch.equal(codes.view(torch.int8).view(m, k).cpu(), q)
+    to_scale = guarded_bytes(4 * m, lambda to: lib.plm_quantize_rows_int8(x.data_ptr(), kind, m, k, codes.data_ptr(), to, stream()))
+    assert torch.equal(to_scale.view(torch.float32).cpu(), s) and torch.equal(scale.cpu(), s)
+    back = guarded_bytes(x.nbytes, lambda to: lib.plm_dequantize_rows_int8(codes.data_ptr(), scale.data_ptr(), m, k, to, kind, stream()))
+    assert torch.equal(back.view(x.dtype).view(m, k).cpu(), (q.float() * s[:, None]).to(x.dtype))
+
+
+@pytest.mark.parametrize("kernel", [None, "r16", "r64", "t0", "t3", "t5", "t2,3", "t5,4"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 16), (2, 8, 208), (3, 200, 2720), (20, 37, 528), (70, 136, 1040), (1, 4100, 64)])
+def test_dense_products(m, n, k, kernel, tuning_env):
+    tuning_env("PLM_DENSE", kernel)
+    lib = _lib.load()
+    x, w, ws = dense.values((m, k), torch.bfloat16, 1), dense.codes(n, k, 2), dense.scales(n, 3)
+    q, xs = (t.cuda() for t in dense.quantize(x))
+    want, shape = dense.int8_product(q, xs, w, ws), torch.Size((m, n))
+    size = lib.plm_gemm_int8_workspace_bytes(m, n, k)
+
+    def on_codes(to):
+        guarded_bytes(size, lambda ws8: lib.plm_gemm_int8(q.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), m, n, k, to, BF, ws8, size, stream()))
+        return _lib.PLM_OK
+
+    dense.within(guarded(shape, on_codes), *want, "codes")
+    size8 = lib.plm_gemm_int8_w8a8_workspace_bytes(m, n, k)
+
+    def on_x(to):
+        guarded_bytes(size8, lambda ws8: lib.plm_gemm_int8_w8a8(x.data_ptr(), BF, w.data_ptr(), ws.data_ptr(), m, n, k, to, ws8, size8, stream()))
+        return _lib.PLM_OK
+
+    dense.within(guarded(shape, on_x), *want, "w8a8")
