@@ -350,10 +350,10 @@ int plm_dequantize_rows_int8(const int8_t* codes, const float* x_scale, int64_t 
  * y [M, N] = x_scale[m] scale[n] sum_k codes[m, k] weight[n, k], in y_dtype (PLM_BF16 or PLM_FP16). The sum is exact;
  * it and its products with the two scales are rounded to fp32, the result once more to y_dtype, and only a result that is out of
  * range itself passes fp32's, whatever the scales are. weight int8 [N, K] row-major, read in place, its scale fp32 [N];
- * any codes, -128 too. K a multiple of 16, at most 131056; N at most 2^19, M below 2^24, M N and M K at most 2^36. codes and weight 16-byte aligned, y at any
- * element. M == 0 or N == 0 returns PLM_OK without touching y; K == 0 sets y to zero. The workspace, where the query
- * names one, holds the parts of a sum that is split over workgroups (256-byte aligned; its contents need not be set and
- * mean nothing after the call).
+ * any codes, -128 too. K a multiple of 16, at most 131056; N at most 2^19, M below 2^24, M N and M K at most 2^36. codes
+ * and weight 16-byte aligned, y at any element. M == 0 or N == 0 returns PLM_OK without touching y; K == 0 sets y to zero.
+ * The workspace, where the query names one, holds the parts of a sum that is split over workgroups (256-byte aligned; its
+ * contents need not be set and mean nothing after the call).
  */
 int64_t plm_gemm_int8_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int plm_gemm_int8(const int8_t* codes, const float* x_scale, const int8_t* weight, const float* scale, int64_t m, int64_t n,

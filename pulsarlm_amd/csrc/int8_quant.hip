@@ -1,6 +1,7 @@
 // Rows of 8-bit integers: quantizer (tokens' activations, a weight's output channels; the rule: int8_rows.hpp) and its
 // inverse.
-// What bounds it: memory. M = 4096, K 12288, bf16: quantizer 31.6 us, 4.8 TB/s; back to fp32 48 us, 5.2 TB/s.
+// What bounds it: memory. M = 4096, K 12288, bf16, x and codes not in the caches: quantizer 30 us, 5.0 TB/s; back to fp32 43 us,
+// 5.9 TB/s.
 #include <algorithm>
 
 #include "dense_gemm.hpp"
@@ -120,9 +121,9 @@ template <plm_dtype D> void launch_quantize(const void* x, int64_t m, int64_t k,
         return;
     }
     // As many threads a row as hold it in two chunks each: fewer hold more each and have fewer rows in flight, more spend
-    // their time on the row's maximum. bf16, us: M = 4096, K 4096 with 64, 128, 256, 512 and 1024 threads 13.7, 12.3, 11.4,
-    // 12.2 and 16.3; K 12288 with 256, 512 and 1024 30.1, 29.5 and 27.4; M = 32768, K 1024 with 64, 128 and 256 20.1, 21.4
-    // and 29.9; M = 333, K 12288 with 256, 512 and 1024 5.5, 5.2 and 5.1. A wavefront's rows need no barrier: four of them
+    // their time on the row's maximum. bf16, x not in the caches, us: M = 4096, K 4096 with 64, 128, 256, 512 and 1024 threads
+    // that hold the row 16.2, 13.4, 12.1, 13.1 and 18.9; K 12288 with 256, 512 and 1024 30.3, 28.4 and 29.7; M = 32768, K 1024 with
+    // 64, 128 and 256 19.3, 22.0 and 31.3; M = 333, K 12288 with 256, 512 and 1024 8.7, 7.0 and 6.4. A wavefront's rows need no barrier: four of them
     // a workgroup. More rows than a grid of such workgroups has: 256 threads each, which read the rest of a row twice.
     const int64_t chunks = k / 8;
     if (chunks <= 64 * 2) quantize_int8_kernel<D, 64, 4, 2><<<static_cast<unsigned>(ceil_div(m, 4)), 256, 0, s>>>(bytes, m, k, codes, scale);

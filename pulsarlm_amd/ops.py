@@ -663,7 +663,8 @@ def mlp_mxfp4_w4a4_cuda(x: torch.Tensor, gate: tuple, up: tuple, down: tuple, in
 # 8-bit integers with a scale for each token and channel, and experts in 8 and 16 bits (formats that the reference has no
 # kernels of its own for). Weights are row-major and read in place: int8 [N, K] with scale fp32 [N], or 16-bit; by expert
 # [E, N, K]. A grouped call's rows are sorted by expert, offsets int32 [E] their inclusive ends, as in grouped_gemm_int4_cuda.
-# An out may not overlap an input.
+# Operands of the products begin at 16 bytes (16-bit x of an 8-bit product: at any element), outputs at any element. An out may not
+# overlap an input.
 # ---------------------------------------------------------------------------
 
 
